@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_void_p
 from pathlib import Path
 
 _PKG_DIR = Path(__file__).resolve().parent
@@ -20,6 +20,7 @@ _P = c_void_p
 _I = c_int
 _L = c_int64
 _F = c_float
+_D = c_double
 
 # name -> (restype, argtypes); mirrors include/coda_b200.h one to one.
 SIGNATURES = {
@@ -76,6 +77,14 @@ SIGNATURES = {
         _I,
         [_P, _L, _P, _L, _P, _L, _I, _P, _L, _P, _P, _P, _I, _P, _I, _I, _I, _F, _P, _L, _P, _I, _P],
     ),
+    "coda_b200_dropout": (_I, [_P, _P, _L, _L, _I, _D, _P, _L, _P, _P]),
+    "coda_b200_add_rmsnorm_fwd": (_I, [_P, _P, _P, _F, _D, _P, _L, _P, _P, _P, _P, _L, _L, _I, _P]),
+    "coda_b200_add_rmsnorm_bwd_scratch_bytes": (_L, [_L, _L]),
+    "coda_b200_add_rmsnorm_bwd": (_I, [_P, _P, _P, _P, _P, _D, _P, _L, _P, _P, _P, _P, _L, _L, _L, _I, _P]),
+    "coda_b200_rows_e4m3": (_I, [_P, _P, _P, _F, _P, _P, _P, _L, _L, _I, _P]),
+    "coda_b200_gemm_e4m3": (_I, [_P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P, _P]),
+    "coda_b200_ce_loss": (_I, [_P, _L, _L, _P, _L, _L, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P]),
+    "coda_b200_gemm_softmax_grad": (_I, [_P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _P, _L, _I, _I, _I, _P, _P]),
 }
 
 

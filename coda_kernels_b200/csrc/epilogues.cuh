@@ -418,6 +418,99 @@ struct EpiLse {
   }
 };
 
+// ------------------------------------------------------------------ softmax gradient of one vocabulary piece
+// G[r, j] = exp(z_rj - lse_r) - (j + col0 == target_r) in bf16, zero in rows whose target is ignored: the gradient of the
+// summed row losses w.r.t. the logits of columns col0 .. col0 + N - 1, given the log-sum-exp over ALL columns.  The logits
+// exist only as this tile's accumulator.  bf16 holds a probability to half a step (2^-9 relative), which is also what
+// the two GEMMs behind it take; the subtraction is done before that rounding.
+struct EpiSoftmaxGrad {
+  static constexpr uint32_t kLoadRingBytes = 0;
+  struct Params {
+    alignas(64) CUtensorMap tm_g;  // G as [M, N], box 32 x 32
+    __nv_bfloat16* G;  // [M, N], ldg a multiple of 8
+    long long ldg;
+    const float* lse;   // [M]
+    const int* target;  // [M]
+    int ignore_index;
+    int col0;
+    int use_tma;
+  };
+
+  template <int kBN>
+  __device__ static void run(const Params& p, EpiCtx& c) {
+    constexpr float kLog2e = 1.4426950408889634f;
+    const bool row_ok = c.row < c.M;
+    const int tgt = row_ok ? __ldg(p.target + c.row) : p.ignore_index;
+    const bool live = tgt != p.ignore_index;
+    const float shift = live ? __ldg(p.lse + c.row) * -kLog2e : 0.f;
+    const int tcol = live ? tgt - p.col0 - c.n0 : -1;  // target column relative to this tile
+    __nv_bfloat16* grow = p.G + static_cast<long long>(c.row) * p.ldg + c.n0;
+    for_chunks(c.taddr, valid_chunks<kBN>(c.n0, c.N), [&](int ch, float* v) {
+      const int trel = tcol - ch * 32;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = live ? fast_exp2(fmaf(v[j], kLog2e, shift)) : 0.f;
+      if (trel >= 0 && trel < 32) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j == trel) v[j] -= 1.0f;
+      }
+      if (p.use_tma) {
+        const uint32_t tile = ring_acquire(c);
+        stage_row_bf16<32>(tile, c.lane, v);
+        ring_publish();
+        if (c.lane == 0) store_tile(c, &p.tm_g, tile, c.n0 + ch * 32);
+        ring_commit(c);
+      } else if (row_ok) {
+        store_row32(grow + ch * 32, v, c.N - c.n0 - ch * 32);  // whole groups of 8: ldg covers the last one
+      }
+    });
+  }
+};
+
+// ------------------------------------------------------------------ product of scaled 8-bit rows
+// D = acc * row_scale[row] * col_scale[col]: the operands are e4m3 values, each row of either with one fp32 scale.
+template <typename OutT>
+struct EpiScaled {
+  static constexpr uint32_t kLoadRingBytes = 0;
+  struct Params {
+    alignas(64) CUtensorMap tm_d;  // D as [M, N], box 32 x 32
+    OutT* D;
+    long long ldd;
+    const float* row_scale;  // [M]
+    const float* col_scale;  // [N], 16-byte aligned
+    int use_tma;
+  };
+
+  template <int kBN>
+  __device__ static void run(const Params& p, EpiCtx& c) {
+    const bool row_ok = c.row < c.M;
+    const float rs = row_ok ? __ldg(p.row_scale + c.row) : 0.f;
+    OutT* drow = p.D + static_cast<long long>(c.row) * p.ldd + c.n0;
+    for_chunks(c.taddr, valid_chunks<kBN>(c.n0, c.N), [&](int ch, float* v) {
+      const int col = c.n0 + ch * 32;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (col + 4 * j < c.N) {  // N is a multiple of 8: a group of 4 is all in or all out
+          const float4 s = __ldg(reinterpret_cast<const float4*>(p.col_scale + col) + j);
+          v[4 * j] *= rs * s.x;
+          v[4 * j + 1] *= rs * s.y;
+          v[4 * j + 2] *= rs * s.z;
+          v[4 * j + 3] *= rs * s.w;
+        }
+      }
+      if (p.use_tma) {
+        const uint32_t tile = ring_acquire(c);
+        stage_row(tile, c.lane, v, static_cast<OutT*>(nullptr));
+        ring_publish();
+        if (c.lane == 0) store_tile(c, &p.tm_d, tile, col);
+        ring_commit(c);
+      } else if (row_ok) {
+        store_row32(drow + ch * 32, v, c.N - col);
+      }
+    });
+  }
+};
+
 // ------------------------------------------------------------------ per-head RMSNorm + RoPE on q,k; plain store for v
 // Columns are [q heads | k heads | v heads], each head kHD wide.  For q and k:
 //   ms = mean(acc^2) over the head (fp32, unrounded acc), r = rsqrt(ms + eps)

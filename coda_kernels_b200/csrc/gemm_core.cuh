@@ -182,7 +182,14 @@ __device__ __forceinline__ void probe_lsu_traffic(const GemmShape& shape, const 
 struct ProNone {
   static constexpr int kWarps = 0;
   static constexpr uint32_t kStageExtraBytes = 0;
+  static constexpr bool kE4M3 = false;
   struct Params {};
+};
+
+// No prologue, but e4m3 operands (both K-major).  Everything in front of the MMA moves bytes, so a k-block of 64 two-byte
+// elements simply holds 128 e4m3 elements: the host describes the operands, and GemmShape::K, in two-byte units.
+struct ProE4M3 : ProNone {
+  static constexpr bool kE4M3 = true;
 };
 
 // G = dout * out * (1 - out), the gradient of a sigmoid through its stored output, formed on the fly as the A operand
@@ -193,6 +200,7 @@ struct ProNone {
 // G, for the weight-gradient GEMM that follows.
 struct ProDSigmoid {
   static constexpr int kWarps = 4;
+  static constexpr bool kE4M3 = false;
   static constexpr uint32_t kStageExtraBytes = kBlockM * kBlockK * 2;  // the dout tile
   struct Params {
     alignas(64) CUtensorMap tm_dout;  // dout as [M, Kc], box 64 x 128, 128-byte swizzle (the A operand's geometry)
@@ -223,6 +231,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
   using Cfg = GemmCfg<kCtaGroup, kBN, Epi::kLoadRingBytes, Pro::kStageExtraBytes>;
   constexpr bool kProlog = Pro::kWarps > 0;
   static_assert(!kProlog || !kAMn, "transform warps build a K-major A tile");
+  static_assert(!Pro::kE4M3 || (!kAMn && !kBMn), "e4m3 operands are K-major");
   constexpr int kStages = Cfg::kStages;
   constexpr int kBNcta = Cfg::kBNcta;
   constexpr uint32_t kABytes = Cfg::kABytes;
@@ -359,7 +368,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
   } else if (warp == 1) {
     // ============================================================ MMA issuer
     if (leader && lane == 0) {
-      constexpr uint32_t idesc = make_idesc_bf16(kBlockM * kCtaGroup, kBN, kAMn, kBMn);
+      constexpr uint32_t idesc = Pro::kE4M3 ? make_idesc_e4m3(kBlockM * kCtaGroup, kBN) : make_idesc_bf16(kBlockM * kCtaGroup, kBN, kAMn, kBMn);
       constexpr uint32_t lbo_mn = kBlockK * 128, sbo_mn = 1024u;
       // K-major: 8-row groups 1024 B apart, one MMA step = 32 B along the swizzled row.
       // MN-major: 64-element column blocks kBlockK*128 B apart, 8-k groups 1024 B apart, one MMA step = 2 groups.
@@ -389,7 +398,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
           for (int k = 0; k < kBlockK / kUmmaK; ++k) {
             const uint64_t adesc = make_smem_desc(a_addr + k * a_step, a_lbo, a_sbo);
             const uint64_t bdesc = make_smem_desc(b_addr + k * b_step, b_lbo, b_sbo);
-            umma_bf16<kCtaGroup>(d_tmem, adesc, bdesc, idesc, (kb != w.kb0 || k != 0) ? 1u : 0u);
+            if constexpr (Pro::kE4M3) umma_f8<kCtaGroup>(d_tmem, adesc, bdesc, idesc, (kb != w.kb0 || k != 0) ? 1u : 0u);
+            else umma_bf16<kCtaGroup>(d_tmem, adesc, bdesc, idesc, (kb != w.kb0 || k != 0) ? 1u : 0u);
           }
           umma_commit<kCtaGroup>(bar_empty + 8 * s);  // frees the stage (in both CTAs) once these MMAs retire
           if (++s == kStages) {

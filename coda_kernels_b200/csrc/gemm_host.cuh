@@ -90,14 +90,14 @@ inline EncodeTiledFn encode_tiled_fn() {
 
 // bf16 matrix with `inner` contiguous elements per line and `outer` lines
 // `ld` elements apart; box = 64 x box_outer, 128-byte swizzle, zero fill.
+// `inner` may be any length (elements beyond it read as zero); only the lines must start on 16-byte boundaries.
 inline int make_tmap_bf16(CUtensorMap* m, const void* ptr, long long inner, long long outer, long long ld, int box_outer) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return fail(kNoDriverEntry, "cuTensorMapEncodeTiled not available from the CUDA driver");
   if ((reinterpret_cast<uintptr_t>(ptr) & 15u) != 0) return fail(kBadArgument, "operand base address must be 16-byte aligned");
   if (outer > 1 && (ld * 2) % 16 != 0) return fail(kBadArgument, "operand leading dimension must be a multiple of 8 elements");
-  if (inner % 8 != 0) return fail(kBadArgument, "operand contiguous extent must be a multiple of 8 elements");
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
-  cuuint64_t strides[1] = {static_cast<cuuint64_t>((outer > 1 ? ld : inner) * 2)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>((outer > 1 ? ld : (inner + 7) / 8 * 8) * 2)};
   cuuint32_t box[2] = {64u, static_cast<cuuint32_t>(box_outer)};
   cuuint32_t estr[2] = {1u, 1u};
   CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,

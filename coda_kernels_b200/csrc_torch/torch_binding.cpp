@@ -291,6 +291,167 @@ std::tuple<OptTensor, OptTensor, Tensor> qknorm_rope_bwd(const Tensor& dq, const
   return {dx, dw, dgamma.to(gamma.scalar_type())};
 }
 
+// ---------------------------------------------------------------------------------------- around the fused linears
+
+inline int row_dtype(const Tensor& t) {
+  return t.scalar_type() == at::kBFloat16 ? 0 : t.scalar_type() == at::kHalf ? 1 : 2;
+}
+// [rows, cols] of a tensor that is taken as dense rows along its last dimension
+inline std::tuple<int64_t, int64_t> row_extents(const Tensor& t) {
+  TORCH_CHECK(t.is_cuda() && t.is_contiguous() && t.dim() >= 1 && t.size(-1) > 0, "a contiguous CUDA tensor with a last dimension is expected");
+  const auto dt = t.scalar_type();
+  TORCH_CHECK(dt == at::kBFloat16 || dt == at::kHalf || dt == at::kFloat, "bfloat16, float16 or float32 expected");
+  return {t.numel() / t.size(-1), t.size(-1)};
+}
+inline void require_like(const Tensor& t, const Tensor& like, const char* name) {
+  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == like.scalar_type() && t.is_contiguous() && t.sizes() == like.sizes(), name,
+              " must be contiguous and match x in shape, dtype and device");
+}
+inline void require_weight(const Tensor& w, const Tensor& x) {
+  TORCH_CHECK(w.device() == x.device() && w.scalar_type() == x.scalar_type() && w.is_contiguous() && w.dim() == 1 && w.size(0) == x.size(-1),
+              "weight must hold one entry per column of x, in x's dtype, on x's device");
+}
+inline const int64_t* rng_ptr(const OptTensor& rng, const Tensor& x) {
+  if (!rng.has_value()) return nullptr;
+  TORCH_CHECK(rng->device() == x.device() && rng->scalar_type() == at::kLong && rng->numel() == 2 && rng->is_contiguous(),
+              "rng must be a contiguous int64 tensor [seed, step] on x's device");
+  return rng->data_ptr<int64_t>();
+}
+
+// (out, the [seed, step] the mask was made from)
+std::tuple<Tensor, Tensor> dropout(const Tensor& x, double p, const OptTensor& rng, int64_t stream_id) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const auto [rows, cols] = row_extents(x);
+  Tensor out = at::empty_like(x), used = at::empty({2}, x.options().dtype(at::kLong));
+  check(coda_b200_dropout(x.data_ptr(), out.data_ptr(), rows, cols, row_dtype(x), p, rng_ptr(rng, x), stream_id, used.data_ptr<int64_t>(),
+                          stream_of(x)),
+        "dropout");
+  return {out, used};
+}
+
+// (out, h or nothing, rstd, the [seed, step] used or nothing); without a residual and dropout h is x itself
+std::tuple<Tensor, OptTensor, Tensor, OptTensor> add_rmsnorm_fwd(const Tensor& x, const OptTensor& residual, const Tensor& weight, double eps,
+                                                                 double p, const OptTensor& rng, int64_t stream_id) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const auto [rows, cols] = row_extents(x);
+  require_weight(weight, x);
+  if (residual.has_value()) require_like(*residual, x, "residual");
+  Tensor out = at::empty_like(x), rstd = at::empty({rows}, x.options().dtype(at::kFloat));
+  OptTensor h, used;
+  if (residual.has_value() || p > 0.0) h = at::empty_like(x);
+  if (p > 0.0) used = at::empty({2}, x.options().dtype(at::kLong));
+  check(coda_b200_add_rmsnorm_fwd(x.data_ptr(), ptr_or_null(residual), weight.data_ptr(), static_cast<float>(eps), p, rng_ptr(rng, x), stream_id,
+                                  used.has_value() ? used->data_ptr<int64_t>() : nullptr, h.has_value() ? h->data_ptr() : nullptr,
+                                  out.data_ptr(), rstd.data_ptr<float>(), rows, cols, row_dtype(x), stream_of(x)),
+        "add_rmsnorm");
+  return {out, h, rstd, used};
+}
+
+// (dx or nothing, dres or nothing, dweight or nothing)
+std::tuple<OptTensor, OptTensor, OptTensor> add_rmsnorm_bwd(const Tensor& dout, const OptTensor& dh, const Tensor& h, const Tensor& rstd,
+                                                            const Tensor& weight, double p, const OptTensor& rng, int64_t stream_id,
+                                                            bool need_dx, bool need_dres, bool need_dw) {
+  const c10::cuda::CUDAGuard guard(h.device());
+  const auto [rows, cols] = row_extents(h);
+  require_like(dout, h, "dout");
+  if (dh.has_value()) require_like(*dh, h, "dh");
+  OptTensor dx, dres, dw;
+  if (need_dx) dx = at::empty_like(h);
+  if (need_dres) dres = at::empty_like(h);
+  Tensor scratch;
+  if (need_dw) {
+    dw = rows > 0 ? at::empty_like(weight) : at::zeros_like(weight);
+    scratch = at::empty({coda_b200_add_rmsnorm_bwd_scratch_bytes(rows, cols) / 4}, h.options().dtype(at::kFloat));
+  }
+  check(coda_b200_add_rmsnorm_bwd(dout.data_ptr(), ptr_or_null(dh), h.data_ptr(), rstd.data_ptr<float>(), weight.data_ptr(), p, rng_ptr(rng, h),
+                                  stream_id, need_dx ? dx->data_ptr() : nullptr, need_dres ? dres->data_ptr() : nullptr,
+                                  need_dw ? dw->data_ptr() : nullptr, need_dw ? scratch.data_ptr() : nullptr,
+                                  need_dw ? scratch.numel() * 4 : 0, rows, cols, row_dtype(h), stream_of(h)),
+        "add_rmsnorm backward");
+  return {dx, dres, dw};
+}
+
+// (q, scale, h or nothing)
+std::tuple<Tensor, Tensor, OptTensor> rows_e4m3(const Tensor& x, const OptTensor& residual, const OptTensor& weight, double eps) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const auto [rows, cols] = row_extents(x);
+  if (weight.has_value()) require_weight(*weight, x);
+  OptTensor h;
+  if (residual.has_value()) {
+    require_like(*residual, x, "residual");
+    h = at::empty_like(x);
+  }
+  Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  check(coda_b200_rows_e4m3(x.data_ptr(), ptr_or_null(residual), ptr_or_null(weight), static_cast<float>(eps),
+                            h.has_value() ? h->data_ptr() : nullptr, q.data_ptr(), scale.data_ptr<float>(), rows, cols, row_dtype(x),
+                            stream_of(x)),
+        "rows_e4m3");
+  return {q, scale, h};
+}
+
+Tensor linear_e4m3(const Tensor& x, const Tensor& x_scale, const Tensor& weight, const Tensor& weight_scale, bool out_fp32,
+                   const Tensor& status) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t M = x.size(0), N = weight.size(0), K = x.size(1);
+  Tensor out = new_matrix(x, M, N, out_fp32 ? at::kFloat : at::kBFloat16);
+  if (M == 0) return out;
+  check(coda_b200_gemm_e4m3(x.data_ptr(), x_scale.data_ptr<float>(), weight.data_ptr(), weight_scale.data_ptr<float>(), out.data_ptr(), N,
+                            out_fp32, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), status_ptr(status), stream_of(x)),
+        "gemm_e4m3");
+  return out;
+}
+
+// (loss, inv_count, lse); every matrix operand is dense, so its strides are its extents
+std::tuple<Tensor, Tensor, Tensor> ce_pieces_fwd(const Tensor& x, const Tensor& weight, const Tensor& target, int64_t ignore_index, bool mean,
+                                                 const Tensor& status) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t M = x.size(0), V = weight.size(0), K = x.size(1);
+  const int64_t tiles = coda_b200_lse_tiles(static_cast<int>(V));
+  const auto f32 = x.options().dtype(at::kFloat);
+  Tensor parts = at::empty({2 * M * tiles + 2 * M}, f32), lse = at::empty({M}, f32), loss = at::empty({}, f32), inv_count = at::empty({}, f32);
+  float* part = parts.data_ptr<float>();
+  check(coda_b200_ce_loss(x.data_ptr(), K, 1, weight.data_ptr(), 1, K, target.data_ptr<int32_t>(), static_cast<int>(ignore_index), mean, part,
+                          part + M * tiles, part + 2 * M * tiles, lse.data_ptr<float>(), part + 2 * M * tiles + M, loss.data_ptr<float>(),
+                          inv_count.data_ptr<float>(), static_cast<int>(M), static_cast<int>(V), static_cast<int>(K), status_ptr(status),
+                          stream_of(x)),
+        "ce_loss");
+  return {loss, inv_count, lse};
+}
+
+// Walks the vocabulary in pieces of `piece` columns with one [M, piece] buffer: the piece's softmax gradient, then its
+// rows of dweight, then its share of dx, summed over the pieces in fp32.
+OptPair ce_pieces_bwd(const Tensor& dloss, const Tensor& inv_count, const Tensor& lse, const Tensor& x, const Tensor& weight,
+                      const Tensor& target, int64_t ignore_index, int64_t piece, bool need_dx, bool need_dw, const Tensor& status) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t M = x.size(0), V = weight.size(0), K = x.size(1);
+  const Tensor xs = x.as_strided({M, K}, {K, 1}), ws = weight.as_strided({V, K}, {K, 1});
+  const OptTensor alpha = (dloss * inv_count).reshape({1}).to(at::kFloat);
+  const int64_t width = std::min(piece, V), ldg = (width + 7) / 8 * 8;
+  Tensor g = new_matrix(x, M, ldg, at::kBFloat16);
+  OptTensor dx, dw, dx32;
+  if (need_dx) dx = new_matrix(x, M, K, at::kBFloat16);
+  if (need_dw) dw = new_matrix(x, V, K, at::kBFloat16);
+  if (need_dx && width < V) dx32 = new_matrix(x, M, K, at::kFloat);
+  for (int64_t c0 = 0; c0 < V; c0 += width) {
+    const int64_t n = std::min(width, V - c0);
+    const Tensor w = ws.narrow(0, c0, n), gp = g.as_strided({M, n}, {ldg, 1});
+    check(coda_b200_gemm_softmax_grad(xs.data_ptr(), K, 1, w.data_ptr(), 1, K, lse.data_ptr<float>(), target.data_ptr<int32_t>(),
+                                      static_cast<int>(ignore_index), static_cast<int>(c0), gp.data_ptr(), ldg, static_cast<int>(M),
+                                      static_cast<int>(n), static_cast<int>(K), status_ptr(status), stream_of(x)),
+          "gemm_softmax_grad");
+    if (need_dw) {
+      Tensor out = dw->narrow(0, c0, n);
+      gemm_out(gp.t(), xs, out, alpha, c10::nullopt, status);
+    }
+    if (need_dx) {
+      Tensor out = c0 + n < V ? *dx32 : *dx;
+      gemm_out(gp, w, out, alpha, c0 > 0 ? dx32 : c10::nullopt, status);
+    }
+  }
+  return {dx, dw};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(coda_b200n, m) {
@@ -325,6 +486,17 @@ TORCH_LIBRARY(coda_b200n, m) {
   m.def("qknorm_rope_bwd(Tensor dq, Tensor dk, Tensor dv, Tensor x, Tensor weight, Tensor preact, Tensor mean_sq, Tensor gamma, "
         "Tensor positions, Tensor frequencies, int head_dim, int num_heads_q, int num_heads_k, float eps, bool need_dx, bool need_dw, "
         "Tensor status) -> (Tensor?, Tensor?, Tensor)");
+
+  m.def("dropout(Tensor x, float p, Tensor? rng, int stream_id) -> (Tensor, Tensor)");
+  m.def("add_rmsnorm_fwd(Tensor x, Tensor? residual, Tensor weight, float eps, float p, Tensor? rng, int stream_id) -> "
+        "(Tensor, Tensor?, Tensor, Tensor?)");
+  m.def("add_rmsnorm_bwd(Tensor dout, Tensor? dh, Tensor h, Tensor rstd, Tensor weight, float p, Tensor? rng, int stream_id, bool need_dx, "
+        "bool need_dres, bool need_dw) -> (Tensor?, Tensor?, Tensor?)");
+  m.def("rows_e4m3(Tensor x, Tensor? residual, Tensor? weight, float eps) -> (Tensor, Tensor, Tensor?)");
+  m.def("linear_e4m3(Tensor x, Tensor x_scale, Tensor weight, Tensor weight_scale, bool out_fp32, Tensor status) -> Tensor");
+  m.def("ce_pieces_fwd(Tensor x, Tensor weight, Tensor target, int ignore_index, bool mean, Tensor status) -> (Tensor, Tensor, Tensor)");
+  m.def("ce_pieces_bwd(Tensor dloss, Tensor inv_count, Tensor lse, Tensor x, Tensor weight, Tensor target, int ignore_index, int piece, "
+        "bool need_dx, bool need_dw, Tensor status) -> (Tensor?, Tensor?)");
 }
 
 TORCH_LIBRARY_IMPL(coda_b200n, CUDA, m) {
@@ -347,4 +519,11 @@ TORCH_LIBRARY_IMPL(coda_b200n, CUDA, m) {
   m.impl("cross_entropy_bwd", cross_entropy_bwd);
   m.impl("qknorm_rope_fwd", qknorm_rope_fwd);
   m.impl("qknorm_rope_bwd", qknorm_rope_bwd);
+  m.impl("dropout", dropout);
+  m.impl("add_rmsnorm_fwd", add_rmsnorm_fwd);
+  m.impl("add_rmsnorm_bwd", add_rmsnorm_bwd);
+  m.impl("rows_e4m3", rows_e4m3);
+  m.impl("linear_e4m3", linear_e4m3);
+  m.impl("ce_pieces_fwd", ce_pieces_fwd);
+  m.impl("ce_pieces_bwd", ce_pieces_bwd);
 }

@@ -1,0 +1,113 @@
+"""Cross entropy over a vocabulary walked in pieces, keeping no logits between forward and backward.
+
+It has no counterpart in the reference.  Same conventions as :mod:`coda_kernels_b200.ops`.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from . import ops
+from ._lib import check, lib
+from .ops import _noop_fake, _require, _require_cuda_bf16, _stream, gemm, lse_tiles, status_word
+
+
+@torch.library.custom_op("coda_b200::ce_loss_out", mutates_args=("parts", "lse", "loss", "inv_count"), device_types="cuda")
+def _ce_loss_out(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, mean: bool, parts: Tensor, lse: Tensor, loss: Tensor,
+                 inv_count: Tensor) -> None:
+    M, K = x.shape
+    V = weight.shape[0]
+    tiles = lse_tiles(V)
+    base = parts.data_ptr()
+    check(
+        lib.coda_b200_ce_loss(x.data_ptr(), K, 1, weight.data_ptr(), 1, K, target.data_ptr(), ignore_index, int(mean), base, base + 4 * M * tiles,
+                              base + 8 * M * tiles, lse.data_ptr(), base + 8 * M * tiles + 4 * M, loss.data_ptr(), inv_count.data_ptr(), M, V,
+                              K, status_word(x.device).data_ptr(), _stream(x)),
+        "ce_loss",
+    )
+
+
+@torch.library.custom_op("coda_b200::gemm_softmax_grad_out", mutates_args=("grad",), device_types="cuda")
+def _gemm_softmax_grad_out(x: Tensor, weight: Tensor, lse: Tensor, target: Tensor, ignore_index: int, col0: int, grad: Tensor) -> None:
+    M, K = x.shape
+    N = weight.shape[0]
+    check(
+        lib.coda_b200_gemm_softmax_grad(x.data_ptr(), K, 1, weight.data_ptr(), 1, K, lse.data_ptr(), target.data_ptr(), ignore_index, col0,
+                                        grad.data_ptr(), grad.shape[1], M, N, K, status_word(x.device).data_ptr(), _stream(x)),
+        "gemm_softmax_grad",
+    )
+
+
+for _op in (_ce_loss_out, _gemm_softmax_grad_out):
+    _op.register_fake(_noop_fake)
+
+
+# Default size of the [rows, piece] gradient buffer, in elements (512 MiB), and the narrowest piece it is cut down to for
+# very many rows: below it the fp32 sum of dx, read and written once a piece, would cost more than a few percent of the
+# piece's GEMMs.
+_PIECE_ELEMENTS = 1 << 28
+_PIECE_MIN = 8192
+
+
+def default_piece(rows: int, vocab: int) -> int:
+    """Columns per piece: pieces of one width, a multiple of the GEMM's column tile, as few as the buffer allows."""
+    widest = max(_PIECE_MIN, _PIECE_ELEMENTS // max(rows, 1))
+    pieces = -(-vocab // widest)
+    return min(vocab, -(-vocab // pieces // 256) * 256) if pieces > 1 else vocab
+
+
+def _require_ce(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int) -> None:
+    _require_cuda_bf16(x, weight)
+    _require(x.dim() == 2 and weight.dim() == 2 and x.shape[1] == weight.shape[1], "x [M, K] and weight [V, K] expected")
+    _require(weight.shape[0] > 0 and x.shape[1] > 0 and x.shape[1] % 8 == 0, "weight must have rows, and K must be a positive multiple of 8")
+    _require(target.device == x.device and weight.device == x.device, "x, weight and target must be on one device")
+    _require(tuple(target.shape) == (x.shape[0],), "target must have one label per row")
+    _require(-(2**31) <= ignore_index < 2**31, "ignore_index must fit int32")
+
+
+def ce_pieces_forward(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, mean: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """``(loss, inv_count, lse)``; nothing of size ``[M, V]`` is written."""
+    _require_ce(x, weight, target, ignore_index)
+    ops._debug_check_targets(target, weight.shape[0], ignore_index)
+    M = x.shape[0]
+    f32 = dict(dtype=torch.float32, device=x.device)
+    if M == 0:  # a sum over nothing, and 0 / 0
+        return torch.full((), float("nan") if mean else 0.0, **f32), torch.full((), float("inf") if mean else 1.0, **f32), torch.empty(0, **f32)
+    if ops._fast():
+        return ops._native.ce_pieces_fwd(x, weight, target, ignore_index, mean, status_word(x.device))
+    parts = torch.empty(2 * M * lse_tiles(weight.shape[0]) + 2 * M, **f32)
+    lse, loss, inv_count = torch.empty(M, **f32), torch.empty((), **f32), torch.empty((), **f32)
+    _ce_loss_out(x, weight, target, ignore_index, mean, parts, lse, loss, inv_count)
+    return loss, inv_count, lse
+
+
+def ce_pieces_backward(dloss: Tensor, inv_count: Tensor, lse: Tensor, x: Tensor, weight: Tensor, target: Tensor, ignore_index: int,
+                       piece: int, need_dx: bool, need_dw: bool) -> tuple[Optional[Tensor], Optional[Tensor]]:
+    """Gradients from one ``[M, piece]`` buffer: per piece of the vocabulary its softmax gradient ``g`` (the logits are
+    computed again), its rows of ``dweight = alpha g^T x``, and ``dx += alpha g @ weight`` in fp32."""
+    M, K = x.shape
+    V = weight.shape[0]
+    if M == 0:
+        return (torch.zeros_like(x) if need_dx else None), (torch.zeros_like(weight) if need_dw else None)
+    if ops._fast():
+        return ops._native.ce_pieces_bwd(dloss, inv_count, lse, x, weight, target, ignore_index, piece, need_dx, need_dw,
+                                         status_word(x.device))
+    alpha = (dloss * inv_count).reshape(1).to(dtype=torch.float32)
+    width = min(piece, V)
+    g = torch.empty(M, -(-width // 8) * 8, dtype=x.dtype, device=x.device)
+    dx = torch.empty_like(x) if need_dx else None
+    dw = torch.empty_like(weight) if need_dw else None
+    dx32 = torch.empty(M, K, dtype=torch.float32, device=x.device) if need_dx and width < V else None
+    for c0 in range(0, V, width):
+        n = min(width, V - c0)
+        w = weight[c0:c0 + n]
+        _gemm_softmax_grad_out(x, w, lse, target, ignore_index, c0, g)
+        gp = g[:, :n]
+        if need_dw:
+            gemm(gp.mT, x, out=dw[c0:c0 + n], alpha=alpha)
+        if need_dx:
+            gemm(gp, w, out=dx32 if c0 + n < V else dx, alpha=alpha, C=dx32 if c0 > 0 else None)
+    return dx, dw

@@ -1,0 +1,190 @@
+"""Row operators around the fused linears: dropout, residual + dropout + RMS norm, rows in e4m3, and the GEMM that reads them.
+
+They have no counterpart in the reference.  Same conventions as :mod:`coda_kernels_b200.ops`: mutating custom ops over
+the C ABI with wrappers that allocate, and one compiled entry point per direction that eager calls go through.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from . import ops
+from ._lib import check, lib
+from .ops import _aligned16, _noop_fake, _require, _stream, status_word
+
+_DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+E4M3 = torch.float8_e4m3fn
+
+
+def _ptr(t: Optional[Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+# ------------------------------------------------------------------------------------------------ custom ops
+@torch.library.custom_op("coda_b200::dropout_out", mutates_args=("out", "used"), device_types="cuda")
+def _dropout_out(x: Tensor, p: float, rng: Optional[Tensor], stream_id: int, out: Tensor, used: Tensor) -> None:
+    cols = x.shape[-1]
+    check(
+        lib.coda_b200_dropout(x.data_ptr(), out.data_ptr(), x.numel() // cols, cols, _DTYPE_CODES[x.dtype], float(p), _ptr(rng), stream_id,
+                              used.data_ptr(), _stream(x)),
+        "dropout",
+    )
+
+
+@torch.library.custom_op("coda_b200::add_rmsnorm_out", mutates_args=("h", "out", "rstd", "used"), device_types="cuda")
+def _add_rmsnorm_out(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float, p: float, rng: Optional[Tensor], stream_id: int,
+                     h: Optional[Tensor], out: Tensor, rstd: Tensor, used: Optional[Tensor]) -> None:
+    cols = x.shape[-1]
+    check(
+        lib.coda_b200_add_rmsnorm_fwd(x.data_ptr(), _ptr(residual), weight.data_ptr(), float(eps), float(p), _ptr(rng), stream_id, _ptr(used),
+                                      _ptr(h), out.data_ptr(), rstd.data_ptr(), x.numel() // cols, cols, _DTYPE_CODES[x.dtype], _stream(x)),
+        "add_rmsnorm",
+    )
+
+
+@torch.library.custom_op("coda_b200::add_rmsnorm_bwd_out", mutates_args=("dx", "dres", "dweight"), device_types="cuda")
+def _add_rmsnorm_bwd_out(dout: Tensor, dh: Optional[Tensor], h: Tensor, rstd: Tensor, weight: Tensor, p: float, rng: Optional[Tensor],
+                         stream_id: int, dx: Optional[Tensor], dres: Optional[Tensor], dweight: Optional[Tensor]) -> None:
+    cols = h.shape[-1]
+    rows = h.numel() // cols
+    scratch_bytes = int(lib.coda_b200_add_rmsnorm_bwd_scratch_bytes(rows, cols)) if dweight is not None else 0
+    scratch = torch.empty(scratch_bytes // 4, dtype=torch.float32, device=h.device) if dweight is not None else None
+    check(
+        lib.coda_b200_add_rmsnorm_bwd(dout.data_ptr(), _ptr(dh), h.data_ptr(), rstd.data_ptr(), weight.data_ptr(), float(p), _ptr(rng),
+                                      stream_id, _ptr(dx), _ptr(dres), _ptr(dweight), _ptr(scratch), scratch_bytes, rows, cols,
+                                      _DTYPE_CODES[h.dtype], _stream(h)),
+        "add_rmsnorm backward",
+    )
+
+
+@torch.library.custom_op("coda_b200::rows_e4m3_out", mutates_args=("h", "q", "scale"), device_types="cuda")
+def _rows_e4m3_out(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], eps: float, h: Optional[Tensor], q: Tensor,
+                   scale: Tensor) -> None:
+    cols = x.shape[-1]
+    check(
+        lib.coda_b200_rows_e4m3(x.data_ptr(), _ptr(residual), _ptr(weight), float(eps), _ptr(h), q.data_ptr(), scale.data_ptr(),
+                                x.numel() // cols, cols, _DTYPE_CODES[x.dtype], _stream(x)),
+        "rows_e4m3",
+    )
+
+
+@torch.library.custom_op("coda_b200::gemm_e4m3_out", mutates_args=("out",), device_types="cuda")
+def _gemm_e4m3_out(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor, out: Tensor) -> None:
+    M, K = x.shape
+    N = weight.shape[0]
+    check(
+        lib.coda_b200_gemm_e4m3(x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(), out.data_ptr(), N,
+                                int(out.dtype == torch.float32), M, N, K, status_word(x.device).data_ptr(), _stream(x)),
+        "gemm_e4m3",
+    )
+
+
+for _op in (_dropout_out, _add_rmsnorm_out, _add_rmsnorm_bwd_out, _rows_e4m3_out, _gemm_e4m3_out):
+    _op.register_fake(_noop_fake)
+
+
+# ------------------------------------------------------------------------------------------------ argument checks
+def _require_rows(x: Tensor) -> None:
+    if not x.is_cuda:
+        raise RuntimeError("coda_b200 operators run on CUDA tensors only; there is no CPU fallback")
+    if x.dtype not in _DTYPE_CODES:
+        raise NotImplementedError(f"coda_b200 row operators take bfloat16, float16 or float32, got {x.dtype}")
+    _require(x.dim() >= 1 and x.shape[-1] > 0, "x must have a last dimension of at least one element")
+
+
+def _require_like(t: Tensor, x: Tensor, name: str) -> None:
+    _require(t.shape == x.shape and t.dtype == x.dtype and t.device == x.device, f"{name} must match x in shape, dtype and device")
+
+
+def _require_weight(weight: Tensor, x: Tensor) -> None:
+    _require(weight.dim() == 1 and weight.shape[0] == x.shape[-1] and weight.dtype == x.dtype and weight.device == x.device,
+             "weight must hold one entry per column of x, in x's dtype, on x's device")
+
+
+def _require_dropout(x: Tensor, p: float, rng: Optional[Tensor], stream: int) -> None:
+    _require(0.0 <= p < 1.0, f"the dropout probability must be at least 0 and below 1, got {p}")
+    _require(0 <= stream < 2**32, "the dropout stream must be a 32-bit number")
+    _require(p == 0.0 or rng is not None, "dropout needs rng, an int64 CUDA tensor [seed, step]")
+    if rng is not None:
+        _require(rng.dtype == torch.int64 and rng.device == x.device and tuple(rng.shape) == (2,),
+                 "rng must be an int64 tensor [seed, step] on x's device")
+
+
+def _require_no_grad(name: str, *tensors: Optional[Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no backward: call it under torch.no_grad() or on detached tensors")
+
+
+# ------------------------------------------------------------------------------------------------ wrappers (dense tensors)
+def dropout_rows(x: Tensor, p: float, rng: Optional[Tensor], stream: int) -> tuple[Tensor, Tensor]:
+    """``(out, used)``: dropout of a dense tensor and the ``[seed, step]`` its mask was made from."""
+    if ops._fast():
+        return ops._native.dropout(x, p, rng, stream)
+    out = torch.empty_like(x)
+    used = torch.empty(2, dtype=torch.int64, device=x.device)
+    _dropout_out(x, p, rng, stream, out, used)
+    return out, used
+
+
+def add_rmsnorm_forward(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float, p: float, rng: Optional[Tensor], stream: int):
+    """``(out, h or None, rstd, used or None)``; ``h`` is ``None`` when it would be ``x`` itself."""
+    if ops._fast():
+        return ops._native.add_rmsnorm_fwd(x, residual, weight, eps, p, rng, stream)
+    out = torch.empty_like(x)
+    h = torch.empty_like(x) if residual is not None or p > 0.0 else None
+    rstd = torch.empty(x.numel() // x.shape[-1], dtype=torch.float32, device=x.device)
+    used = torch.empty(2, dtype=torch.int64, device=x.device) if p > 0.0 else None
+    _add_rmsnorm_out(x, residual, weight, eps, p, rng, stream, h, out, rstd, used)
+    return out, h, rstd, used
+
+
+def add_rmsnorm_backward(dout: Tensor, dh: Optional[Tensor], h: Tensor, rstd: Tensor, weight: Tensor, p: float, rng: Optional[Tensor],
+                         stream: int, need_dx: bool, need_dres: bool, need_dw: bool):
+    """``(dx, dresidual, dweight)``, ``None`` where not wanted."""
+    if ops._fast():
+        return ops._native.add_rmsnorm_bwd(dout, dh, h, rstd, weight, p, rng, stream, need_dx, need_dres, need_dw)
+    dx = torch.empty_like(h) if need_dx else None
+    dres = torch.empty_like(h) if need_dres else None
+    dw = None
+    if need_dw:
+        dw = torch.empty_like(weight) if h.numel() > 0 else torch.zeros_like(weight)
+    _add_rmsnorm_bwd_out(dout, dh, h, rstd, weight, p, rng, stream, dx, dres, dw)
+    return dx, dres, dw
+
+
+def rows_e4m3(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], eps: float):
+    """``(q, scale, h or None)``: rows of ``x`` (plus ``residual``, normalised with ``weight``) as e4m3 values and scales."""
+    if ops._fast():
+        return ops._native.rows_e4m3(x, residual, weight, eps)
+    h = torch.empty_like(x) if residual is not None else None
+    q = torch.empty(x.shape, dtype=E4M3, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    _rows_e4m3_out(x, residual, weight, eps, h, q, scale)
+    return q, scale, h
+
+
+def gemm_e4m3(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor, out_dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """``(x * x_scale[:, None]) @ (weight * weight_scale[:, None])^T`` for dense e4m3 ``x [M, K]`` and ``weight [N, K]``."""
+    for t in (x, x_scale, weight, weight_scale):
+        if not t.is_cuda:
+            raise RuntimeError("coda_b200 operators run on CUDA tensors only; there is no CPU fallback")
+        _require(t.device == x.device, "all operands must be on one device")
+    if x.dtype != E4M3 or weight.dtype != E4M3:
+        raise NotImplementedError(f"x and weight must be float8_e4m3fn, got {x.dtype} and {weight.dtype}")
+    _require(x.dim() == 2 and weight.dim() == 2 and x.shape[1] == weight.shape[1], "x [M, K] and weight [N, K] expected")
+    _require(x.shape[1] > 0 and x.shape[1] % 16 == 0, "K must be a positive multiple of 16")
+    _require(weight.shape[0] > 0 and weight.shape[0] % 8 == 0, "the number of weight rows must be a positive multiple of 8")
+    for name, s, n in (("x_scale", x_scale, x.shape[0]), ("weight_scale", weight_scale, weight.shape[0])):
+        _require(s.dtype == torch.float32 and tuple(s.shape) == (n,), f"{name} must be float32 with one entry per row")
+    _require(out_dtype in (torch.bfloat16, torch.float32), "out_dtype must be bfloat16 or float32")
+    x, x_scale, weight = _aligned16(x), x_scale.contiguous(), _aligned16(weight)
+    weight_scale = _aligned16(weight_scale)
+    if ops._fast():
+        return ops._native.linear_e4m3(x, x_scale, weight, weight_scale, out_dtype == torch.float32, status_word(x.device))
+    out = torch.empty(x.shape[0], weight.shape[0], dtype=out_dtype, device=x.device)
+    if x.shape[0] > 0:
+        _gemm_e4m3_out(x, x_scale, weight, weight_scale, out)
+    return out

@@ -348,6 +348,66 @@ int coda_b200_qknorm_rope_bwd_noalloc(const void* dq, int64_t ld_dq, const void*
                                       int head_dim, int hq, int hk, float eps, void* grad, int64_t ld_grad, float* dgamma,
                                       int M, void* stream);
 
+/* ---- around the fused linears (no counterpart in the reference) ----
+ *
+ * Row kernels: dense row-major [rows, cols] matrices (leading dimension cols) of
+ * `dtype` 0 = bf16, 1 = fp16, 2 = fp32, any cols >= 1 and any alignment of the
+ * element type; rows == 0 launches nothing and writes nothing.
+ *
+ * Dropout: element (r, c) stays if word c % 4 of Philox4x32-10 with key
+ * `seed` and counter (r * ceil(cols / 4) + c / 4 [64 bits], step, stream_id) is at
+ * least round(p * 2^32); it is then multiplied by 1 / (1 - p).  A dropped element
+ * is +0 whatever it held.  `rng` points to device int64 [seed, step] (step is
+ * taken modulo 2^32) and is read by the kernel; it may be NULL when p == 0.
+ * 0 <= p < 1, 0 <= stream_id < 2^32.  `rng_used` (NULL, or device int64 [2])
+ * receives the values the call used, for a backward that runs after `rng` moved on. */
+
+/* out = dropout(x).  The backward is the same call on the gradient with the forward's rng values. */
+int coda_b200_dropout(const void* x, void* out, int64_t rows, int64_t cols, int dtype, double p, const int64_t* rng,
+                      int64_t stream_id, int64_t* rng_used, void* stream);
+
+/* h = residual + dropout(x) (residual NULL: h = dropout(x)), rstd = rsqrt(mean(h^2) + eps) of the unrounded h (fp32 [rows]),
+ * out = h * rstd * weight from the unrounded h.  `h` may be NULL (not wanted). */
+int coda_b200_add_rmsnorm_fwd(const void* x, const void* residual, const void* weight, float eps, double p, const int64_t* rng,
+                              int64_t stream_id, int64_t* rng_used, void* h, void* out, float* rstd, int64_t rows,
+                              int64_t cols, int dtype, void* stream);
+
+/* Backward of the above from dout and dh (NULL: zero): with g = dout * weight and xh = h * rstd,
+ * dres = dh + rstd * (g - xh * mean(g * xh)), dx = dropout(dres), dweight = sum over rows of dout * xh (in `dtype`,
+ * summed in fp32 in a fixed order).  dx, dres and dweight may each be NULL; dweight needs
+ * coda_b200_add_rmsnorm_bwd_scratch_bytes of scratch.  With rows == 0 dweight is not written. */
+int64_t coda_b200_add_rmsnorm_bwd_scratch_bytes(int64_t rows, int64_t cols);
+int coda_b200_add_rmsnorm_bwd(const void* dout, const void* dh, const void* h, const float* rstd, const void* weight, double p,
+                              const int64_t* rng, int64_t stream_id, void* dx, void* dres, void* dweight, void* scratch,
+                              int64_t scratch_bytes, int64_t rows, int64_t cols, int dtype, void* stream);
+
+/* Rows as e4m3 values with one fp32 scale each: y = residual + x, normalised and weighted as above when weight != NULL
+ * (residual and h may be NULL; h receives residual + x); scale = max(max|y| / 448, 2^-126), q = y / scale rounded once.
+ * A row that holds NaN gets the scale NaN. */
+int coda_b200_rows_e4m3(const void* x, const void* residual, const void* weight, float eps, void* h, void* q, float* scale,
+                        int64_t rows, int64_t cols, int dtype, void* stream);
+
+/* D[m, n] = a_scale[m] * b_scale[n] * sum_k A[m, k] * B[n, k] for dense row-major e4m3 A [M, K] and B [N, K], fp32
+ * accumulation; D is bf16 or fp32 with leading dimension ldd.  K a multiple of 16, N and ldd multiples of 8; A, B, D and
+ * b_scale 16-byte aligned. */
+int coda_b200_gemm_e4m3(const void* A, const float* a_scale, const void* B, const float* b_scale, void* D, int64_t ldd,
+                        int d_is_fp32, int M, int N, int K, int* dev_status, void* stream);
+
+/* Cross entropy of the logits A @ B over all N columns (any N), storing none of them: lse fp32 [M], losses fp32 [M] (zero
+ * in ignored rows, NaN for a label outside [0, N)), and the scalars loss = inv_count * sum(losses) and inv_count
+ * (1 / rows that are not ignored with `mean`, else 1).  part_max / part_sum fp32 [M, coda_b200_lse_tiles(N)] and
+ * target_logit fp32 [M] are workspace. */
+int coda_b200_ce_loss(const void* A, int64_t a_stride_m, int64_t a_stride_k, const void* B, int64_t b_stride_k,
+                      int64_t b_stride_n, const int32_t* target, int ignore_index, int mean, float* part_max, float* part_sum,
+                      float* target_logit, float* lse, float* losses, float* loss, float* inv_count, int M, int N, int K,
+                      int* dev_status, void* stream);
+
+/* G[r, j] = exp(z_rj - lse[r]) - (col0 + j == target[r]) in bf16 for the logits z = A @ B of one piece of the vocabulary
+ * (N columns, the first of which is column col0 of the whole), zero in ignored rows.  ldg: a multiple of 8, >= N. */
+int coda_b200_gemm_softmax_grad(const void* A, int64_t a_stride_m, int64_t a_stride_k, const void* B, int64_t b_stride_k,
+                                int64_t b_stride_n, const float* lse, const int32_t* target, int ignore_index, int col0, void* G,
+                                int64_t ldg, int M, int N, int K, int* dev_status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
