@@ -86,12 +86,14 @@ __device__ __forceinline__ void store_chunk(T* p, const float* v, int n) {
   }
 }
 
-// v / s as e4m3, rounded once (the division is the correctly rounded one)
+// v * inv as e4m3.  inv is the row's 1 / scale: a division for every element made this kernel slower than its memory traffic
+// (8192 x 5120 bf16: 125 us a pass with, 72 us without); the product's extra rounding of 2^-24 moves a value only where it lies
+// that near to the middle of two e4m3 values.  Saturation turns 448 (1 + 2^-23) into 448.
 template <bool kVec>
-__device__ __forceinline__ void store_e4m3(__nv_fp8_e4m3* p, const float* v, float s, int n) {
+__device__ __forceinline__ void store_e4m3(__nv_fp8_e4m3* p, const float* v, float inv, int n) {
   uint32_t e[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) e[j] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * j] / s, v[2 * j + 1] / s), __NV_SATFINITE, __NV_E4M3);
+  for (int j = 0; j < 4; ++j) e[j] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * j] * inv, v[2 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
   if constexpr (kVec) {
     if (n > 0) *reinterpret_cast<uint2*>(p) = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
   } else {
@@ -285,6 +287,7 @@ norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T
     const float r = weight != nullptr ? rsqrtf(sq / static_cast<float>(cols) + eps) : 1.0f;
     float s = 1.0f;
     if (kE4M3) s = max_nan(top * r / 448.0f, 1.17549435e-38f);
+    const float inv = 1.0f / s;
     if (lane == 0) {
       if (kE4M3) scale[row] = s;
       else rstd[row] = r;
@@ -298,7 +301,7 @@ norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T
         for (int j = 0; j < 8; ++j) v[k][j] = v[k][j] * r * chunk_get(w, j);
       }
       if constexpr (kE4M3) {
-        store_e4m3<kVec>(q + base + c, v[k], s, n);
+        store_e4m3<kVec>(q + base + c, v[k], inv, n);
       } else {
         store_chunk<kVec>(out + base + c, v[k], n);
       }
@@ -445,6 +448,7 @@ norm_fwd_long_kernel(const T* __restrict__ x, const T* __restrict__ residual, co
     const float r = weight != nullptr ? rsqrtf(sq / static_cast<float>(cols) + eps) : 1.0f;
     float s = 1.0f;
     if (kE4M3) s = max_nan(top * r / 448.0f, 1.17549435e-38f);
+    const float inv = 1.0f / s;
     if (threadIdx.x == 0) {
       if (kE4M3) scale[row] = s;
       else rstd[row] = r;
@@ -456,7 +460,7 @@ norm_fwd_long_kernel(const T* __restrict__ x, const T* __restrict__ residual, co
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = v[j] * r * chunk_get(w, j);
       }
-      if constexpr (kE4M3) store_e4m3<kVec>(q + base + c, v, s, cols - c);
+      if constexpr (kE4M3) store_e4m3<kVec>(q + base + c, v, inv, cols - c);
       else store_chunk<kVec>(out + base + c, v, cols - c);
     }
   }

@@ -9,8 +9,12 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <climits>
+#include <cmath>
+#include <initializer_list>
 #include <tuple>
 
 #include "../../include/coda_b200.h"
@@ -292,123 +296,264 @@ std::tuple<OptTensor, OptTensor, Tensor> qknorm_rope_bwd(const Tensor& dq, const
 }
 
 // ---------------------------------------------------------------------------------------- around the fused linears
+// Operators whose kernels take microseconds: the whole call, autograd node and argument checks included, is C++.
+// Registered for the Autograd key, they run the forward directly when nothing needs a gradient.
 
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+inline void require_cuda(const Tensor& t) {
+  TORCH_CHECK(t.is_cuda(), "coda_b200 operators run on CUDA tensors only; there is no CPU fallback");
+}
+inline void require_rows(const Tensor& x) {
+  require_cuda(x);
+  const auto dt = x.scalar_type();
+  TORCH_CHECK_NOT_IMPLEMENTED(dt == at::kBFloat16 || dt == at::kHalf || dt == at::kFloat,
+                              "coda_b200 row operators take bfloat16, float16 or float32, got ", dt);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "x must have a last dimension of at least one element");
+}
+inline void require_like(const Tensor& t, const Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes(), name,
+                    " must match x in shape, dtype and device");
+}
+inline void require_weight(const Tensor& w, const Tensor& x) {
+  TORCH_CHECK_VALUE(w.device() == x.device() && w.scalar_type() == x.scalar_type() && w.dim() == 1 && w.size(0) == x.size(-1),
+                    "weight must hold one entry per column of x, in x's dtype, on x's device");
+}
+inline void require_dropout(const Tensor& x, double p, const OptTensor& rng, int64_t stream) {
+  TORCH_CHECK_VALUE(p >= 0.0 && p < 1.0, "the dropout probability must be at least 0 and below 1, got ", p);
+  TORCH_CHECK_VALUE(stream >= 0 && stream <= 0xffffffffLL, "the dropout stream must be a 32-bit number");
+  TORCH_CHECK_VALUE(p == 0.0 || rng.has_value(), "dropout needs rng, an int64 CUDA tensor [seed, step]");
+  if (rng.has_value())
+    TORCH_CHECK_VALUE(rng->device() == x.device() && rng->scalar_type() == at::kLong && rng->dim() == 1 && rng->size(0) == 2,
+                      "rng must be an int64 tensor [seed, step] on x's device");
+}
+inline void require_no_grad(const char* name, std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : tensors)
+    TORCH_CHECK(!t->defined() || !t->requires_grad(), name, " has no backward: call it under torch.no_grad() or on detached tensors");
+}
+inline void require_first_order(const char* name) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), name, " can be differentiated once only");
+}
+inline bool wants_grad(std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : tensors)
+    if (t->requires_grad()) return true;
+  return false;
+}
 inline int row_dtype(const Tensor& t) {
   return t.scalar_type() == at::kBFloat16 ? 0 : t.scalar_type() == at::kHalf ? 1 : 2;
 }
-// [rows, cols] of a tensor that is taken as dense rows along its last dimension
-inline std::tuple<int64_t, int64_t> row_extents(const Tensor& t) {
-  TORCH_CHECK(t.is_cuda() && t.is_contiguous() && t.dim() >= 1 && t.size(-1) > 0, "a contiguous CUDA tensor with a last dimension is expected");
-  const auto dt = t.scalar_type();
-  TORCH_CHECK(dt == at::kBFloat16 || dt == at::kHalf || dt == at::kFloat, "bfloat16, float16 or float32 expected");
-  return {t.numel() / t.size(-1), t.size(-1)};
-}
-inline void require_like(const Tensor& t, const Tensor& like, const char* name) {
-  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == like.scalar_type() && t.is_contiguous() && t.sizes() == like.sizes(), name,
-              " must be contiguous and match x in shape, dtype and device");
-}
-inline void require_weight(const Tensor& w, const Tensor& x) {
-  TORCH_CHECK(w.device() == x.device() && w.scalar_type() == x.scalar_type() && w.is_contiguous() && w.dim() == 1 && w.size(0) == x.size(-1),
-              "weight must hold one entry per column of x, in x's dtype, on x's device");
-}
-inline const int64_t* rng_ptr(const OptTensor& rng, const Tensor& x) {
-  if (!rng.has_value()) return nullptr;
-  TORCH_CHECK(rng->device() == x.device() && rng->scalar_type() == at::kLong && rng->numel() == 2 && rng->is_contiguous(),
-              "rng must be a contiguous int64 tensor [seed, step] on x's device");
-  return rng->data_ptr<int64_t>();
-}
+inline const int64_t* rng_ptr(const Tensor& rng) { return rng.defined() ? rng.data_ptr<int64_t>() : nullptr; }
+inline void* ptr_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+inline Tensor dense(const OptTensor& t) { return t.has_value() ? t->contiguous() : Tensor(); }
 
-// (out, the [seed, step] the mask was made from)
-std::tuple<Tensor, Tensor> dropout(const Tensor& x, double p, const OptTensor& rng, int64_t stream_id) {
+// dropout of dense x from rng; `used` (when wanted) receives the [seed, step] the mask was made from
+Tensor run_dropout(const Tensor& x, double p, const Tensor& rng, int64_t stream, Tensor* used) {
   const c10::cuda::CUDAGuard guard(x.device());
-  const auto [rows, cols] = row_extents(x);
-  Tensor out = at::empty_like(x), used = at::empty({2}, x.options().dtype(at::kLong));
-  check(coda_b200_dropout(x.data_ptr(), out.data_ptr(), rows, cols, row_dtype(x), p, rng_ptr(rng, x), stream_id, used.data_ptr<int64_t>(),
-                          stream_of(x)),
+  Tensor out = at::empty_like(x);
+  if (used != nullptr) *used = at::empty({2}, x.options().dtype(at::kLong));
+  check(coda_b200_dropout(x.data_ptr(), out.data_ptr(), x.numel() / x.size(-1), x.size(-1), row_dtype(x), p, rng_ptr(rng), stream,
+                          used != nullptr ? used->data_ptr<int64_t>() : nullptr, stream_of(x)),
         "dropout");
-  return {out, used};
+  return out;
 }
 
-// (out, h or nothing, rstd, the [seed, step] used or nothing); without a residual and dropout h is x itself
-std::tuple<Tensor, OptTensor, Tensor, OptTensor> add_rmsnorm_fwd(const Tensor& x, const OptTensor& residual, const Tensor& weight, double eps,
-                                                                 double p, const OptTensor& rng, int64_t stream_id) {
+class DropoutNode : public torch::autograd::Function<DropoutNode> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, double p, const OptTensor& rng, int64_t stream) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    Tensor used, out = run_dropout(x.contiguous(), p, dense(rng), stream, &used);
+    ctx->save_for_backward({used});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["stream"] = stream;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    require_first_order("dropout");
+    const Tensor used = ctx->get_saved_variables()[0];
+    return {run_dropout(grads[0].contiguous(), ctx->saved_data["p"].toDouble(), used, ctx->saved_data["stream"].toInt(), nullptr), Tensor(),
+            Tensor(), Tensor()};
+  }
+};
+
+Tensor dropout(const Tensor& x, double p, const OptTensor& rng, int64_t stream) {
+  require_rows(x);
+  require_dropout(x, p, rng, stream);
+  if (wants_grad({&x})) return DropoutNode::apply(x, p, rng, stream);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return run_dropout(x.contiguous(), p, dense(rng), stream, nullptr);
+}
+
+struct NormForward {
+  Tensor out, h, rstd, used;  // h only with a residual, used only with dropout
+};
+NormForward run_norm(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps, double p, const Tensor& rng, int64_t stream) {
   const c10::cuda::CUDAGuard guard(x.device());
-  const auto [rows, cols] = row_extents(x);
-  require_weight(weight, x);
-  if (residual.has_value()) require_like(*residual, x, "residual");
-  Tensor out = at::empty_like(x), rstd = at::empty({rows}, x.options().dtype(at::kFloat));
-  OptTensor h, used;
-  if (residual.has_value() || p > 0.0) h = at::empty_like(x);
-  if (p > 0.0) used = at::empty({2}, x.options().dtype(at::kLong));
-  check(coda_b200_add_rmsnorm_fwd(x.data_ptr(), ptr_or_null(residual), weight.data_ptr(), static_cast<float>(eps), p, rng_ptr(rng, x), stream_id,
-                                  used.has_value() ? used->data_ptr<int64_t>() : nullptr, h.has_value() ? h->data_ptr() : nullptr,
-                                  out.data_ptr(), rstd.data_ptr<float>(), rows, cols, row_dtype(x), stream_of(x)),
+  const int64_t cols = x.size(-1), rows = x.numel() / cols;
+  NormForward f;
+  f.out = at::empty_like(x);
+  f.rstd = at::empty({rows}, x.options().dtype(at::kFloat));
+  if (residual.defined()) f.h = at::empty_like(x);
+  if (p > 0.0) f.used = at::empty({2}, x.options().dtype(at::kLong));
+  check(coda_b200_add_rmsnorm_fwd(x.data_ptr(), ptr_or_null(residual), weight.data_ptr(), static_cast<float>(eps), p, rng_ptr(rng), stream,
+                                  f.used.defined() ? f.used.data_ptr<int64_t>() : nullptr, ptr_or_null(f.h), f.out.data_ptr(),
+                                  f.rstd.data_ptr<float>(), rows, cols, row_dtype(x), stream_of(x)),
         "add_rmsnorm");
-  return {out, h, rstd, used};
+  return f;
 }
-
-// (dx or nothing, dres or nothing, dweight or nothing)
-std::tuple<OptTensor, OptTensor, OptTensor> add_rmsnorm_bwd(const Tensor& dout, const OptTensor& dh, const Tensor& h, const Tensor& rstd,
-                                                            const Tensor& weight, double p, const OptTensor& rng, int64_t stream_id,
-                                                            bool need_dx, bool need_dres, bool need_dw) {
+// (dx, dres, dweight), undefined where not wanted
+variable_list run_norm_backward(const Tensor& dout, const Tensor& dh, const Tensor& h, const Tensor& rstd, const Tensor& weight, double p,
+                                const Tensor& rng, int64_t stream, bool need_dx, bool need_dres, bool need_dw) {
   const c10::cuda::CUDAGuard guard(h.device());
-  const auto [rows, cols] = row_extents(h);
-  require_like(dout, h, "dout");
-  if (dh.has_value()) require_like(*dh, h, "dh");
-  OptTensor dx, dres, dw;
+  const int64_t cols = h.size(-1), rows = h.numel() / cols;
+  Tensor dx, dres, dw, scratch;
   if (need_dx) dx = at::empty_like(h);
   if (need_dres) dres = at::empty_like(h);
-  Tensor scratch;
+  int64_t scratch_bytes = 0;
   if (need_dw) {
     dw = rows > 0 ? at::empty_like(weight) : at::zeros_like(weight);
-    scratch = at::empty({coda_b200_add_rmsnorm_bwd_scratch_bytes(rows, cols) / 4}, h.options().dtype(at::kFloat));
+    scratch_bytes = coda_b200_add_rmsnorm_bwd_scratch_bytes(rows, cols);
+    scratch = at::empty({scratch_bytes / 4}, h.options().dtype(at::kFloat));
   }
-  check(coda_b200_add_rmsnorm_bwd(dout.data_ptr(), ptr_or_null(dh), h.data_ptr(), rstd.data_ptr<float>(), weight.data_ptr(), p, rng_ptr(rng, h),
-                                  stream_id, need_dx ? dx->data_ptr() : nullptr, need_dres ? dres->data_ptr() : nullptr,
-                                  need_dw ? dw->data_ptr() : nullptr, need_dw ? scratch.data_ptr() : nullptr,
-                                  need_dw ? scratch.numel() * 4 : 0, rows, cols, row_dtype(h), stream_of(h)),
+  check(coda_b200_add_rmsnorm_bwd(dout.data_ptr(), ptr_or_null(dh), h.data_ptr(), rstd.data_ptr<float>(), weight.data_ptr(), p, rng_ptr(rng),
+                                  stream, ptr_or_null(dx), ptr_or_null(dres), ptr_or_null(dw), ptr_or_null(scratch), scratch_bytes, rows, cols,
+                                  row_dtype(h), stream_of(h)),
         "add_rmsnorm backward");
   return {dx, dres, dw};
 }
 
-// (q, scale, h or nothing)
-std::tuple<Tensor, Tensor, OptTensor> rows_e4m3(const Tensor& x, const OptTensor& residual, const OptTensor& weight, double eps) {
-  const c10::cuda::CUDAGuard guard(x.device());
-  const auto [rows, cols] = row_extents(x);
-  if (weight.has_value()) require_weight(*weight, x);
-  OptTensor h;
-  if (residual.has_value()) {
-    require_like(*residual, x, "residual");
-    h = at::empty_like(x);
+class RMSNormNode : public torch::autograd::Function<RMSNormNode> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, double eps) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor xc = x.contiguous(), w = weight.contiguous();
+    NormForward f = run_norm(xc, Tensor(), w, eps, 0.0, Tensor(), 0);
+    ctx->save_for_backward({xc, w, f.rstd});
+    return f.out;
   }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    require_first_order("rms_norm");
+    const auto saved = ctx->get_saved_variables();
+    auto g = run_norm_backward(grads[0].contiguous(), Tensor(), saved[0], saved[2], saved[1], 0.0, Tensor(), 0, false, ctx->needs_input_grad(0),
+                               ctx->needs_input_grad(1));
+    return {g[1], g[2], Tensor()};
+  }
+};
+
+class AddRMSNormNode : public torch::autograd::Function<AddRMSNormNode> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const Tensor& weight, double eps, double p,
+                               const OptTensor& rng, int64_t stream) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor w = weight.contiguous();
+    NormForward f = run_norm(x.contiguous(), residual.contiguous(), w, eps, p, dense(rng), stream);
+    ctx->save_for_backward({f.h, w, f.rstd, f.used});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["stream"] = stream;
+    ctx->set_materialize_grads(false);
+    return {f.out, f.h};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    require_first_order("add_rms_norm");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor& h = saved[0];
+    const Tensor dout = grads[0].defined() ? grads[0].contiguous() : at::zeros_like(h);  // undefined: only h was used
+    const Tensor dh = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    auto g = run_norm_backward(dout, dh, h, saved[2], saved[1], ctx->saved_data["p"].toDouble(), saved[3], ctx->saved_data["stream"].toInt(),
+                               ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2));
+    return {g[0], g[1], g[2], Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor rms_norm(const Tensor& x, const Tensor& weight, double eps) {
+  require_rows(x);
+  require_weight(weight, x);
+  if (wants_grad({&x, &weight})) return RMSNormNode::apply(x, weight, eps);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return run_norm(x.contiguous(), Tensor(), weight.contiguous(), eps, 0.0, Tensor(), 0).out;
+}
+
+std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps, double p,
+                                        const OptTensor& rng, int64_t stream) {
+  require_rows(x);
+  require_like(residual, x, "residual");
+  require_weight(weight, x);
+  require_dropout(x, p, rng, stream);
+  if (wants_grad({&x, &residual, &weight})) {
+    auto r = AddRMSNormNode::apply(x, residual, weight, eps, p, rng, stream);
+    return {r[0], r[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  NormForward f = run_norm(x.contiguous(), residual.contiguous(), weight.contiguous(), eps, p, dense(rng), stream);
+  return {f.out, f.h};
+}
+
+// (q, scale, h or nothing)
+std::tuple<Tensor, Tensor, OptTensor> rows_e4m3(const Tensor& x_in, const OptTensor& residual_in, const OptTensor& weight_in, double eps) {
+  require_rows(x_in);
+  require_no_grad("the e4m3 output", {&x_in});
+  if (residual_in.has_value()) {
+    require_like(*residual_in, x_in, "residual");
+    require_no_grad("the e4m3 output", {&*residual_in});
+  }
+  if (weight_in.has_value()) {
+    require_weight(*weight_in, x_in);
+    require_no_grad("the e4m3 output", {&*weight_in});
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::cuda::CUDAGuard guard(x_in.device());
+  const Tensor x = x_in.contiguous(), residual = dense(residual_in), weight = dense(weight_in);
   Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
   Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  OptTensor h;
+  if (residual.defined()) h = at::empty_like(x);
   check(coda_b200_rows_e4m3(x.data_ptr(), ptr_or_null(residual), ptr_or_null(weight), static_cast<float>(eps),
-                            h.has_value() ? h->data_ptr() : nullptr, q.data_ptr(), scale.data_ptr<float>(), rows, cols, row_dtype(x),
-                            stream_of(x)),
+                            h.has_value() ? h->data_ptr() : nullptr, q.data_ptr(), scale.data_ptr<float>(), x.numel() / x.size(-1), x.size(-1),
+                            row_dtype(x), stream_of(x)),
         "rows_e4m3");
   return {q, scale, h};
 }
 
-Tensor linear_e4m3(const Tensor& x, const Tensor& x_scale, const Tensor& weight, const Tensor& weight_scale, bool out_fp32,
+Tensor linear_e4m3(const Tensor& x_in, const Tensor& x_scale, const Tensor& weight_in, const Tensor& weight_scale, bool out_fp32,
                    const Tensor& status) {
-  const c10::cuda::CUDAGuard guard(x.device());
-  const int64_t M = x.size(0), N = weight.size(0), K = x.size(1);
+  for (const Tensor* t : {&x_in, &x_scale, &weight_in, &weight_scale}) {
+    require_cuda(*t);
+    TORCH_CHECK_VALUE(t->device() == x_in.device(), "all operands must be on one device");
+  }
+  TORCH_CHECK_NOT_IMPLEMENTED(x_in.scalar_type() == at::kFloat8_e4m3fn && weight_in.scalar_type() == at::kFloat8_e4m3fn,
+                              "x and weight must be float8_e4m3fn, got ", x_in.scalar_type(), " and ", weight_in.scalar_type());
+  TORCH_CHECK_VALUE(x_in.dim() == 2 && weight_in.dim() == 2 && x_in.size(1) == weight_in.size(1), "x [M, K] and weight [N, K] expected");
+  const int64_t M = x_in.size(0), N = weight_in.size(0), K = x_in.size(1);
+  TORCH_CHECK_VALUE(K > 0 && K % 16 == 0, "K must be a positive multiple of 16");
+  TORCH_CHECK_VALUE(N > 0 && N % 8 == 0, "the number of weight rows must be a positive multiple of 8");
+  TORCH_CHECK_VALUE(x_scale.scalar_type() == at::kFloat && x_scale.dim() == 1 && x_scale.size(0) == M,
+                    "x_scale must be float32 with one entry per row");
+  TORCH_CHECK_VALUE(weight_scale.scalar_type() == at::kFloat && weight_scale.dim() == 1 && weight_scale.size(0) == N,
+                    "weight_scale must be float32 with one entry per row");
+  TORCH_CHECK_VALUE(M <= INT_MAX && N <= INT_MAX && K <= INT_MAX, "extents must fit 31 bits");
+  require_no_grad("linear_e4m3", {&x_in, &x_scale, &weight_in, &weight_scale});
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::cuda::CUDAGuard guard(x_in.device());
+  const Tensor x = aligned16(x_in), xs = x_scale.contiguous(), weight = aligned16(weight_in), ws = aligned16(weight_scale);
   Tensor out = new_matrix(x, M, N, out_fp32 ? at::kFloat : at::kBFloat16);
   if (M == 0) return out;
-  check(coda_b200_gemm_e4m3(x.data_ptr(), x_scale.data_ptr<float>(), weight.data_ptr(), weight_scale.data_ptr<float>(), out.data_ptr(), N,
-                            out_fp32, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), status_ptr(status), stream_of(x)),
+  check(coda_b200_gemm_e4m3(x.data_ptr(), xs.data_ptr<float>(), weight.data_ptr(), ws.data_ptr<float>(), out.data_ptr(), N, out_fp32,
+                            static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), status_ptr(status), stream_of(x)),
         "gemm_e4m3");
   return out;
 }
 
 // (loss, inv_count, lse); every matrix operand is dense, so its strides are its extents
-std::tuple<Tensor, Tensor, Tensor> ce_pieces_fwd(const Tensor& x, const Tensor& weight, const Tensor& target, int64_t ignore_index, bool mean,
-                                                 const Tensor& status) {
+std::tuple<Tensor, Tensor, Tensor> run_ce(const Tensor& x, const Tensor& weight, const Tensor& target, int64_t ignore_index, bool mean,
+                                          const Tensor& status) {
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t M = x.size(0), V = weight.size(0), K = x.size(1);
-  const int64_t tiles = coda_b200_lse_tiles(static_cast<int>(V));
   const auto f32 = x.options().dtype(at::kFloat);
+  if (M == 0)  // a sum over nothing, and 0 / 0
+    return {at::full({}, mean ? NAN : 0.0, f32), at::full({}, mean ? INFINITY : 1.0, f32), at::empty({0}, f32)};
+  const int64_t tiles = coda_b200_lse_tiles(static_cast<int>(V));
   Tensor parts = at::empty({2 * M * tiles + 2 * M}, f32), lse = at::empty({M}, f32), loss = at::empty({}, f32), inv_count = at::empty({}, f32);
   float* part = parts.data_ptr<float>();
   check(coda_b200_ce_loss(x.data_ptr(), K, 1, weight.data_ptr(), 1, K, target.data_ptr<int32_t>(), static_cast<int>(ignore_index), mean, part,
@@ -421,15 +566,20 @@ std::tuple<Tensor, Tensor, Tensor> ce_pieces_fwd(const Tensor& x, const Tensor& 
 
 // Walks the vocabulary in pieces of `piece` columns with one [M, piece] buffer: the piece's softmax gradient, then its
 // rows of dweight, then its share of dx, summed over the pieces in fp32.
-OptPair ce_pieces_bwd(const Tensor& dloss, const Tensor& inv_count, const Tensor& lse, const Tensor& x, const Tensor& weight,
-                      const Tensor& target, int64_t ignore_index, int64_t piece, bool need_dx, bool need_dw, const Tensor& status) {
+OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tensor& lse, const Tensor& x, const Tensor& weight,
+                        const Tensor& target, int64_t ignore_index, int64_t piece, bool need_dx, bool need_dw, const Tensor& status) {
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t M = x.size(0), V = weight.size(0), K = x.size(1);
+  OptTensor dx, dw, dx32;
+  if (M == 0) {
+    if (need_dx) dx = at::zeros_like(x);
+    if (need_dw) dw = at::zeros_like(weight);
+    return {dx, dw};
+  }
   const Tensor xs = x.as_strided({M, K}, {K, 1}), ws = weight.as_strided({V, K}, {K, 1});
   const OptTensor alpha = (dloss * inv_count).reshape({1}).to(at::kFloat);
   const int64_t width = std::min(piece, V), ldg = (width + 7) / 8 * 8;
   Tensor g = new_matrix(x, M, ldg, at::kBFloat16);
-  OptTensor dx, dw, dx32;
   if (need_dx) dx = new_matrix(x, M, K, at::kBFloat16);
   if (need_dw) dw = new_matrix(x, V, K, at::kBFloat16);
   if (need_dx && width < V) dx32 = new_matrix(x, M, K, at::kFloat);
@@ -450,6 +600,46 @@ OptPair ce_pieces_bwd(const Tensor& dloss, const Tensor& inv_count, const Tensor
     }
   }
   return {dx, dw};
+}
+
+class CePiecesNode : public torch::autograd::Function<CePiecesNode> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& weight_in, const Tensor& target_in, int64_t ignore_index,
+                        bool mean, int64_t piece, const Tensor& status) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor x = x_in.contiguous(), weight = weight_in.contiguous(), target = target_in.contiguous();
+    auto [loss, inv_count, lse] = run_ce(x, weight, target, ignore_index, mean, status);
+    ctx->save_for_backward({x, weight, target, lse, inv_count});
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["piece"] = piece;
+    ctx->saved_data["status"] = status;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    require_first_order("linear_cross_entropy_pieces");
+    const auto s = ctx->get_saved_variables();
+    auto [dx, dw] = run_ce_backward(grads[0], s[4], s[3], s[0], s[1], s[2], ctx->saved_data["ignore_index"].toInt(),
+                                    ctx->saved_data["piece"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                                    ctx->saved_data["status"].toTensor());
+    return {dx.value_or(Tensor()), dw.value_or(Tensor()), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor linear_cross_entropy_pieces(const Tensor& x, const Tensor& weight, const Tensor& target, int64_t ignore_index, bool mean, int64_t piece,
+                                   const Tensor& status) {
+  for (const Tensor* t : {&x, &weight}) {
+    require_cuda(*t);
+    TORCH_CHECK_NOT_IMPLEMENTED(t->scalar_type() == at::kBFloat16, "coda_b200 operators take bfloat16 matrices, got ", t->scalar_type());
+  }
+  TORCH_CHECK_VALUE(x.dim() == 2 && weight.dim() == 2 && x.size(1) == weight.size(1), "x [M, K] and weight [V, K] expected");
+  TORCH_CHECK_VALUE(weight.size(0) > 0 && x.size(1) > 0 && x.size(1) % 8 == 0, "weight must have rows, and K must be a positive multiple of 8");
+  TORCH_CHECK_VALUE(target.device() == x.device() && weight.device() == x.device(), "x, weight and target must be on one device");
+  TORCH_CHECK_VALUE(target.dim() == 1 && target.size(0) == x.size(0) && target.scalar_type() == at::kInt, "target must have one label per row");
+  TORCH_CHECK_VALUE(ignore_index >= INT_MIN && ignore_index <= INT_MAX, "ignore_index must fit int32");
+  TORCH_CHECK_VALUE(x.size(0) <= INT_MAX && weight.size(0) <= INT_MAX - 256, "extents must fit 31 bits");
+  if (wants_grad({&x, &weight})) return CePiecesNode::apply(x, weight, target, ignore_index, mean, piece, status);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return std::get<0>(run_ce(x.contiguous(), weight.contiguous(), target.contiguous(), ignore_index, mean, status));
 }
 
 }  // namespace
@@ -487,16 +677,12 @@ TORCH_LIBRARY(coda_b200n, m) {
         "Tensor positions, Tensor frequencies, int head_dim, int num_heads_q, int num_heads_k, float eps, bool need_dx, bool need_dw, "
         "Tensor status) -> (Tensor?, Tensor?, Tensor)");
 
-  m.def("dropout(Tensor x, float p, Tensor? rng, int stream_id) -> (Tensor, Tensor)");
-  m.def("add_rmsnorm_fwd(Tensor x, Tensor? residual, Tensor weight, float eps, float p, Tensor? rng, int stream_id) -> "
-        "(Tensor, Tensor?, Tensor, Tensor?)");
-  m.def("add_rmsnorm_bwd(Tensor dout, Tensor? dh, Tensor h, Tensor rstd, Tensor weight, float p, Tensor? rng, int stream_id, bool need_dx, "
-        "bool need_dres, bool need_dw) -> (Tensor?, Tensor?, Tensor?)");
+  m.def("dropout(Tensor x, float p, Tensor? rng, int stream) -> Tensor");
+  m.def("rms_norm(Tensor x, Tensor weight, float eps) -> Tensor");
+  m.def("add_rms_norm(Tensor x, Tensor residual, Tensor weight, float eps, float p, Tensor? rng, int stream) -> (Tensor, Tensor)");
   m.def("rows_e4m3(Tensor x, Tensor? residual, Tensor? weight, float eps) -> (Tensor, Tensor, Tensor?)");
   m.def("linear_e4m3(Tensor x, Tensor x_scale, Tensor weight, Tensor weight_scale, bool out_fp32, Tensor status) -> Tensor");
-  m.def("ce_pieces_fwd(Tensor x, Tensor weight, Tensor target, int ignore_index, bool mean, Tensor status) -> (Tensor, Tensor, Tensor)");
-  m.def("ce_pieces_bwd(Tensor dloss, Tensor inv_count, Tensor lse, Tensor x, Tensor weight, Tensor target, int ignore_index, int piece, "
-        "bool need_dx, bool need_dw, Tensor status) -> (Tensor?, Tensor?)");
+  m.def("linear_cross_entropy_pieces(Tensor x, Tensor weight, Tensor target, int ignore_index, bool mean, int piece, Tensor status) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(coda_b200n, CUDA, m) {
@@ -519,11 +705,16 @@ TORCH_LIBRARY_IMPL(coda_b200n, CUDA, m) {
   m.impl("cross_entropy_bwd", cross_entropy_bwd);
   m.impl("qknorm_rope_fwd", qknorm_rope_fwd);
   m.impl("qknorm_rope_bwd", qknorm_rope_bwd);
-  m.impl("dropout", dropout);
-  m.impl("add_rmsnorm_fwd", add_rmsnorm_fwd);
-  m.impl("add_rmsnorm_bwd", add_rmsnorm_bwd);
-  m.impl("rows_e4m3", rows_e4m3);
-  m.impl("linear_e4m3", linear_e4m3);
-  m.impl("ce_pieces_fwd", ce_pieces_fwd);
-  m.impl("ce_pieces_bwd", ce_pieces_bwd);
 }
+
+// The operators that bring their own autograd node sit on the Autograd key, and on the CUDA key for calls that come in
+// below it (inference mode).
+#define CODA_WITH_AUTOGRAD(m)                                          \
+  m.impl("dropout", dropout);                                           \
+  m.impl("rms_norm", rms_norm);                                         \
+  m.impl("add_rms_norm", add_rms_norm);                                 \
+  m.impl("rows_e4m3", rows_e4m3);                                       \
+  m.impl("linear_e4m3", linear_e4m3);                                   \
+  m.impl("linear_cross_entropy_pieces", linear_cross_entropy_pieces)
+TORCH_LIBRARY_IMPL(coda_b200n, AutogradCUDA, m) { CODA_WITH_AUTOGRAD(m); }
+TORCH_LIBRARY_IMPL(coda_b200n, CUDA, m) { CODA_WITH_AUTOGRAD(m); }

@@ -14,8 +14,9 @@ from typing import Optional
 import torch
 
 from .._guards import autocast_custom_bwd, autocast_custom_fwd, input_guard
-from ..ops import _require
+from ..ops import _debug_check_targets, _fast, _require, lazy_status_check, status_word
 from ..ops_ce import ce_pieces_backward, ce_pieces_forward, default_piece
+from ..ops_rows import call_native
 
 
 class LinearCrossEntropyPieces(torch.autograd.Function):
@@ -58,4 +59,8 @@ def linear_cross_entropy_pieces(
     if piece is None:
         piece = default_piece(x.shape[0], weight.shape[0])
     _require(piece >= 1, "piece must be at least 1")
+    if _fast() and x.is_cuda:
+        lazy_status_check(x.device)
+        _debug_check_targets(target, weight.shape[0], ignore_index)
+        return call_native("linear_cross_entropy_pieces", x, weight, target, ignore_index, reduction == "mean", int(piece), status_word(x.device))
     return LinearCrossEntropyPieces.apply(x, weight, target, ignore_index, reduction, int(piece))

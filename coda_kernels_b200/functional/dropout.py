@@ -13,7 +13,8 @@ import torch
 from torch import Tensor
 
 from .._guards import autocast_custom_bwd, autocast_custom_fwd, input_guard
-from ..ops_rows import _require_dropout, _require_rows, dropout_rows
+from ..ops import _fast
+from ..ops_rows import _require_dropout, _require_rows, call_native, dropout_rows
 
 
 class Dropout(torch.autograd.Function):
@@ -44,4 +45,6 @@ def dropout(x: Tensor, p: float, rng: Optional[Tensor] = None, stream: int = 0) 
     ``rng`` is an int64 CUDA tensor ``[seed, step]`` (not needed for ``p = 0``); advance ``step`` (``rng[1] += 1``) once a
     training step, and give every place of the model its own ``stream`` number.  The mask depends on the rows and the
     last dimension of ``x``, not on its other dimensions."""
+    if _fast() and x.is_cuda:
+        return call_native("dropout", x, p, rng, stream)
     return Dropout.apply(x, float(p), rng, int(stream))

@@ -14,6 +14,7 @@ import torch
 from torch import Tensor
 
 from .._guards import autocast_custom_bwd, autocast_custom_fwd, input_guard
+from ..ops import _fast
 from ..ops_rows import (
     _require_dropout,
     _require_like,
@@ -22,6 +23,7 @@ from ..ops_rows import (
     _require_weight,
     add_rmsnorm_backward,
     add_rmsnorm_forward,
+    call_native,
     rows_e4m3,
 )
 
@@ -80,6 +82,8 @@ class AddRMSNorm(torch.autograd.Function):
 
 def rms_norm(x: Tensor, weight: Tensor, eps: float) -> Tensor:
     """``x * rsqrt(mean(x^2) + eps) * weight`` over the last dimension of ``x [..., N]`` (bf16, fp16 or fp32)."""
+    if _fast() and x.is_cuda:
+        return call_native("rms_norm", x, weight, eps)
     return RMSNorm.apply(x, weight, float(eps))
 
 
@@ -88,11 +92,20 @@ def add_rms_norm(x: Tensor, residual: Tensor, weight: Tensor, eps: float, p: flo
     """``(out, h)``: ``h = residual + dropout(x)`` and ``out = rms_norm(h, weight, eps)``, ``x`` and ``residual [..., N]``.
 
     ``p``, ``rng`` and ``stream`` are those of :func:`dropout`, and give the same mask."""
+    if _fast() and x.is_cuda:
+        return call_native("add_rms_norm", x, residual, weight, eps, p, rng, stream)
     return AddRMSNorm.apply(x, residual, weight, float(eps), float(p), rng, int(stream))
 
 
-@input_guard
 def _rows_e4m3(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], eps: float):
+    if _fast() and x.is_cuda:
+        return call_native("rows_e4m3", x, residual, weight, eps)
+    _require_no_grad("the e4m3 output", x, residual, weight)
+    return _rows_e4m3_composed(x, residual, weight, float(eps))
+
+
+@input_guard
+def _rows_e4m3_composed(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], eps: float):
     _require_rows(x)
     if residual is not None:
         _require_like(residual, x, "residual")
@@ -104,20 +117,17 @@ def _rows_e4m3(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], 
 def rms_norm_e4m3(x: Tensor, weight: Tensor, eps: float) -> tuple[Tensor, Tensor]:
     """``(q, scale)``: the rows of ``rms_norm(x, weight, eps)`` as ``float8_e4m3fn`` values and one fp32 scale each
     (``q * scale[..., None]`` is the row), for :func:`linear_e4m3`.  Inference only."""
-    _require_no_grad("rms_norm_e4m3", x, weight)
-    q, scale, _ = _rows_e4m3(x, None, weight, float(eps))
+    q, scale, _ = _rows_e4m3(x, None, weight, eps)
     return q, scale
 
 
 def add_rms_norm_e4m3(x: Tensor, residual: Tensor, weight: Tensor, eps: float) -> tuple[Tensor, Tensor, Tensor]:
     """``(q, scale, h)``: :func:`add_rms_norm` without dropout, its first output in 8 bits.  Inference only."""
-    _require_no_grad("add_rms_norm_e4m3", x, residual, weight)
-    return _rows_e4m3(x, residual, weight, float(eps))
+    return _rows_e4m3(x, residual, weight, eps)
 
 
 def quantize_e4m3(x: Tensor) -> tuple[Tensor, Tensor]:
     """``(q, scale)``: the rows of ``x [..., N]`` as ``float8_e4m3fn`` values and ``scale = max|row| / 448`` each: a
     weight, once, or activations that no norm precedes."""
-    _require_no_grad("quantize_e4m3", x)
     q, scale, _ = _rows_e4m3(x, None, None, 0.0)
     return q, scale

@@ -1,6 +1,7 @@
 """Cross entropy over a vocabulary walked in pieces, keeping no logits between forward and backward.
 
-It has no counterpart in the reference.  Same conventions as :mod:`coda_kernels_b200.ops`.
+It has no counterpart in the reference.  Eager calls run the compiled form of the same sequence (see
+:mod:`coda_kernels_b200.ops_rows`); what is here serves ``torch.compile`` and the other dispatch modes.
 """
 
 from __future__ import annotations
@@ -76,8 +77,6 @@ def ce_pieces_forward(x: Tensor, weight: Tensor, target: Tensor, ignore_index: i
     f32 = dict(dtype=torch.float32, device=x.device)
     if M == 0:  # a sum over nothing, and 0 / 0
         return torch.full((), float("nan") if mean else 0.0, **f32), torch.full((), float("inf") if mean else 1.0, **f32), torch.empty(0, **f32)
-    if ops._fast():
-        return ops._native.ce_pieces_fwd(x, weight, target, ignore_index, mean, status_word(x.device))
     parts = torch.empty(2 * M * lse_tiles(weight.shape[0]) + 2 * M, **f32)
     lse, loss, inv_count = torch.empty(M, **f32), torch.empty((), **f32), torch.empty((), **f32)
     _ce_loss_out(x, weight, target, ignore_index, mean, parts, lse, loss, inv_count)
@@ -92,9 +91,6 @@ def ce_pieces_backward(dloss: Tensor, inv_count: Tensor, lse: Tensor, x: Tensor,
     V = weight.shape[0]
     if M == 0:
         return (torch.zeros_like(x) if need_dx else None), (torch.zeros_like(weight) if need_dw else None)
-    if ops._fast():
-        return ops._native.ce_pieces_bwd(dloss, inv_count, lse, x, weight, target, ignore_index, piece, need_dx, need_dw,
-                                         status_word(x.device))
     alpha = (dloss * inv_count).reshape(1).to(dtype=torch.float32)
     width = min(piece, V)
     g = torch.empty(M, -(-width // 8) * 8, dtype=x.dtype, device=x.device)

@@ -1,7 +1,9 @@
 """Row operators around the fused linears: dropout, residual + dropout + RMS norm, rows in e4m3, and the GEMM that reads them.
 
-They have no counterpart in the reference.  Same conventions as :mod:`coda_kernels_b200.ops`: mutating custom ops over
-the C ABI with wrappers that allocate, and one compiled entry point per direction that eager calls go through.
+They have no counterpart in the reference.  Eager calls go through compiled operators that bring their own autograd node
+and argument checks (:func:`call_native`): their kernels take microseconds, and an ``autograd.Function`` in Python costs
+more than that.  While ``torch.compile`` traces, or with ``CODA_B200_DISPATCH`` other than ``native``, the functions of
+:mod:`coda_kernels_b200.functional` use the Python nodes over the custom ops below, with the same checks.
 """
 
 from __future__ import annotations
@@ -11,12 +13,27 @@ from typing import Optional
 import torch
 from torch import Tensor
 
-from . import ops
-from ._lib import check, lib
+from ._lib import CodaB200Error, check, lib
 from .ops import _aligned16, _noop_fake, _require, _stream, status_word
 
 _DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 E4M3 = torch.float8_e4m3fn
+
+
+_native_ops: dict = {}
+
+
+def call_native(name: str, *args):
+    """An operator of the compiled dispatch layer; what the library refuses is raised as the package's own exception."""
+    op = _native_ops.get(name)
+    if op is None:
+        op = _native_ops[name] = getattr(torch.ops.coda_b200n, name).default
+    try:
+        return op(*args)
+    except NotImplementedError:
+        raise
+    except RuntimeError as ex:
+        raise CodaB200Error(str(ex).split("\n")[0]) from None
 
 
 def _ptr(t: Optional[Tensor]):
@@ -121,8 +138,6 @@ def _require_no_grad(name: str, *tensors: Optional[Tensor]) -> None:
 # ------------------------------------------------------------------------------------------------ wrappers (dense tensors)
 def dropout_rows(x: Tensor, p: float, rng: Optional[Tensor], stream: int) -> tuple[Tensor, Tensor]:
     """``(out, used)``: dropout of a dense tensor and the ``[seed, step]`` its mask was made from."""
-    if ops._fast():
-        return ops._native.dropout(x, p, rng, stream)
     out = torch.empty_like(x)
     used = torch.empty(2, dtype=torch.int64, device=x.device)
     _dropout_out(x, p, rng, stream, out, used)
@@ -131,8 +146,6 @@ def dropout_rows(x: Tensor, p: float, rng: Optional[Tensor], stream: int) -> tup
 
 def add_rmsnorm_forward(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float, p: float, rng: Optional[Tensor], stream: int):
     """``(out, h or None, rstd, used or None)``; ``h`` is ``None`` when it would be ``x`` itself."""
-    if ops._fast():
-        return ops._native.add_rmsnorm_fwd(x, residual, weight, eps, p, rng, stream)
     out = torch.empty_like(x)
     h = torch.empty_like(x) if residual is not None or p > 0.0 else None
     rstd = torch.empty(x.numel() // x.shape[-1], dtype=torch.float32, device=x.device)
@@ -144,8 +157,6 @@ def add_rmsnorm_forward(x: Tensor, residual: Optional[Tensor], weight: Tensor, e
 def add_rmsnorm_backward(dout: Tensor, dh: Optional[Tensor], h: Tensor, rstd: Tensor, weight: Tensor, p: float, rng: Optional[Tensor],
                          stream: int, need_dx: bool, need_dres: bool, need_dw: bool):
     """``(dx, dresidual, dweight)``, ``None`` where not wanted."""
-    if ops._fast():
-        return ops._native.add_rmsnorm_bwd(dout, dh, h, rstd, weight, p, rng, stream, need_dx, need_dres, need_dw)
     dx = torch.empty_like(h) if need_dx else None
     dres = torch.empty_like(h) if need_dres else None
     dw = None
@@ -157,8 +168,6 @@ def add_rmsnorm_backward(dout: Tensor, dh: Optional[Tensor], h: Tensor, rstd: Te
 
 def rows_e4m3(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], eps: float):
     """``(q, scale, h or None)``: rows of ``x`` (plus ``residual``, normalised with ``weight``) as e4m3 values and scales."""
-    if ops._fast():
-        return ops._native.rows_e4m3(x, residual, weight, eps)
     h = torch.empty_like(x) if residual is not None else None
     q = torch.empty(x.shape, dtype=E4M3, device=x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
@@ -179,11 +188,8 @@ def gemm_e4m3(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor, 
     _require(weight.shape[0] > 0 and weight.shape[0] % 8 == 0, "the number of weight rows must be a positive multiple of 8")
     for name, s, n in (("x_scale", x_scale, x.shape[0]), ("weight_scale", weight_scale, weight.shape[0])):
         _require(s.dtype == torch.float32 and tuple(s.shape) == (n,), f"{name} must be float32 with one entry per row")
-    _require(out_dtype in (torch.bfloat16, torch.float32), "out_dtype must be bfloat16 or float32")
     x, x_scale, weight = _aligned16(x), x_scale.contiguous(), _aligned16(weight)
     weight_scale = _aligned16(weight_scale)
-    if ops._fast():
-        return ops._native.linear_e4m3(x, x_scale, weight, weight_scale, out_dtype == torch.float32, status_word(x.device))
     out = torch.empty(x.shape[0], weight.shape[0], dtype=out_dtype, device=x.device)
     if x.shape[0] > 0:
         _gemm_e4m3_out(x, x_scale, weight, weight_scale, out)

@@ -430,3 +430,67 @@ def test_row_operators_under_compile(ck):
         assert torch.equal(a, b)
     for a, b in zip(torch.autograd.grad(eager, leaves, douts), torch.autograd.grad(traced, leaves, douts)):
         assert torch.equal(a, b)
+
+
+def test_both_bindings_give_the_same_bits(ck):
+    """The compiled operators and the Python nodes over the custom ops (what torch.compile traces)."""
+    from importlib import import_module
+
+    norm, drop, ce = (import_module(f"coda_kernels_b200.functional.{m}") for m in ("rms_norm", "dropout", "cross_entropy_pieces"))
+    rows_ops = import_module("coda_kernels_b200.ops_rows")
+    x, res, w = randn(50, 264), randn(50, 264, seed=1), randn(264, seed=2)
+    dout, dh = randn(50, 264, seed=3), randn(50, 264, seed=4)
+
+    def grads(outs, leaves, gs):
+        outs = outs if isinstance(outs, tuple) else (outs,)
+        return [o.detach() for o in outs] + list(torch.autograd.grad(outs, leaves, gs[: len(outs)]))
+
+    for native, node, args, n in (
+        (ck.add_rms_norm, norm.AddRMSNorm, (x, res, w, EPS, 0.1, rng_state(), 3), 3),
+        (ck.rms_norm, norm.RMSNorm, (x, w, EPS), 2),
+        (ck.dropout, drop.Dropout, (x, 0.4, rng_state(), 1), 1),
+    ):
+        results = []
+        for fn in (native, node.apply):
+            leaves = [a.clone().requires_grad_(True) for a in args[:n]]
+            results.append(grads(fn(*leaves, *args[n:]), leaves, (dout, dh)))
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
+    t = torch.randint(0, 50, (50,), dtype=torch.int32, device=DEV)
+    results = []
+    for fn in (lambda a, b: ck.linear_cross_entropy_pieces(a, b, t, piece=24),
+               lambda a, b: ce.LinearCrossEntropyPieces.apply(a, b, t, -100, "mean", 24)):
+        leaves = [x.clone().requires_grad_(True), res.clone().requires_grad_(True)]
+        loss = fn(*leaves)
+        results.append([loss.detach(), *torch.autograd.grad(loss, leaves)])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    for a, b in zip(ck.add_rms_norm_e4m3(x, res, w, EPS), rows_ops.rows_e4m3(x, res, w, EPS)):
+        assert torch.equal(a.float(), b.float())
+    q, s = ck.quantize_e4m3(torch.randn(9, 64, device=DEV))
+    q2, s2 = ck.quantize_e4m3(torch.randn(16, 64, device=DEV))
+    assert torch.equal(ck.linear_e4m3(q, s, q2, s2), rows_ops.gemm_e4m3(q, s, q2, s2))
+
+
+def test_second_derivative_is_refused(ck):
+    x, w = randn(4, 64).requires_grad_(True), randn(64, seed=1).requires_grad_(True)
+    for out in (ck.rms_norm(x, w, EPS), ck.dropout(x, 0.5, rng_state()), ck.add_rms_norm(x, x.detach(), w, EPS)[0]):
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad(out.sum(), x, create_graph=True)
+
+
+def test_inference_mode_and_backward_accumulation(ck):
+    x, res, w = randn(20, 128), randn(20, 128, seed=1), randn(128, seed=2)
+    with torch.inference_mode():
+        a = ck.add_rms_norm(x, res, w, EPS)
+        q = ck.rms_norm_e4m3(x, w, EPS)
+    b = ck.add_rms_norm(x, res, w, EPS)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and q[0].shape == x.shape
+    # x used twice: both contributions arrive, through .backward() into .grad
+    leaf, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    out, h = ck.add_rms_norm(leaf, leaf, wl, EPS)
+    (out.float().sum() + h.float().sum()).backward()
+    l1, l2 = x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    out, h = ck.add_rms_norm(l1, l2, w, EPS)
+    g1, g2 = torch.autograd.grad((out, h), (l1, l2), (torch.ones_like(out), torch.ones_like(h)))
+    assert torch.equal(leaf.grad, g1 + g2)
