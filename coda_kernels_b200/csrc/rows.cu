@@ -5,6 +5,7 @@
 #include <cuda_fp8.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <type_traits>
 
 #include "../../include/coda_b200.h"
@@ -15,9 +16,10 @@ using namespace cb;
 namespace {
 
 // ------------------------------------------------------------------ chunks
-// A thread works on chunks of 8 consecutive elements of a row, held as loaded (2-byte types: 4 registers, fp32: 8).
-// kVec: every chunk is whole and 16-byte aligned, and moves in 16-byte accesses; otherwise `n` elements (which may be <= 0)
-// move one by one.  Elements that are not there read as zero.
+// A thread works on chunks of 8 consecutive elements, held as loaded (2-byte types: 4 registers, fp32: 8).  A chunk always
+// starts at a multiple of 8 elements of the whole (dense, 16-byte aligned) matrix, so it moves in 16-byte accesses whatever
+// the row's length.  With cols % 8 != 0 (kShift) a row therefore begins `off` = row * cols mod 8 elements into its first
+// chunk; elements of a chunk that belong to the neighbouring rows are read, masked to zero before use, and never written.
 template <typename T>
 struct Chunk {
   uint32_t w[2 * sizeof(T)];
@@ -44,62 +46,102 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 
-template <bool kVec, typename T>
-__device__ __forceinline__ Chunk<T> load_chunk(const T* p, int n) {
+// The elements of a chunk that a thread may touch: [lo, hi).  Without kShift a chunk is whole or not there at all.
+template <bool kShift>
+struct Span {
+  int c0;  // column of element 0 (kShift: may be negative)
+  int lo, hi;
+  __device__ Span(int first, int cols) : c0(first), lo(first < 0 ? -first : 0), hi(cols - first < 8 ? cols - first : 8) {}
+  __device__ bool any() const { return kShift ? hi > lo : hi > 0; }
+  __device__ bool whole() const { return kShift ? (lo == 0 && hi == 8) : hi > 0; }
+};
+
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_whole(const T* p) {
   Chunk<T> c;
-  if constexpr (kVec) {
 #pragma unroll
-    for (int k = 0; k < static_cast<int>(sizeof(T)) / 2; ++k) {
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      if (n > 0) u = *(reinterpret_cast<const uint4*>(p) + k);
-      c.w[4 * k] = u.x;
-      c.w[4 * k + 1] = u.y;
-      c.w[4 * k + 2] = u.z;
-      c.w[4 * k + 3] = u.w;
-    }
-  } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) c.w[j] = j < n ? __float_as_uint(p[j]) : 0u;
-  } else {
-    const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
-    unsigned short e[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = j < n ? q[j] : static_cast<unsigned short>(0);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c.w[j] = static_cast<uint32_t>(e[2 * j]) | (static_cast<uint32_t>(e[2 * j + 1]) << 16);
+  for (int k = 0; k < static_cast<int>(sizeof(T)) / 2; ++k) {
+    const uint4 u = *(reinterpret_cast<const uint4*>(p) + k);
+    c.w[4 * k] = u.x;
+    c.w[4 * k + 1] = u.y;
+    c.w[4 * k + 2] = u.z;
+    c.w[4 * k + 3] = u.w;
   }
   return c;
 }
-template <bool kVec, typename T>
-__device__ __forceinline__ void store_chunk(T* p, const float* v, int n) {
-  if constexpr (!kVec) {
+template <typename T>
+__device__ __forceinline__ Chunk<T> zero_chunk() {
+  Chunk<T> c;
+#pragma unroll
+  for (int k = 0; k < static_cast<int>(2 * sizeof(T)); ++k) c.w[k] = 0u;
+  return c;
+}
+// elements [lo, hi) one by one, zero elsewhere
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_some(const T* p, int lo, int hi) {
+  Chunk<T> c = zero_chunk<T>();
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j >= lo && j < hi) {
+      if constexpr (sizeof(T) == 4) c.w[j] = __float_as_uint(p[j]);
+      else c.w[j >> 1] |= static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(p)[j]) << (16 * (j & 1));
+    }
+  return c;
+}
+// The chunk at p as it is, neighbours' elements included; `left` = elements from p to the end of the matrix (a chunk that
+// reaches beyond it is read one by one).  mask_chunk takes the neighbours out, where the values are used: a load that is
+// masked at once is waited for at once, row by row in the warps at a row's ends (backward 16384 x 4095: 383 us that way, KTM us
+// so).
+template <bool kShift, typename T>
+__device__ __forceinline__ Chunk<T> load_chunk(const T* p, const Span<kShift>& s, long long left) {
+  if (!s.any()) return zero_chunk<T>();
+  if constexpr (kShift) {
+    if (left < 8) return load_some(p, 0, static_cast<int>(left));
+  }
+  return load_whole(p);
+}
+template <bool kShift, typename T>
+__device__ __forceinline__ void mask_chunk(Chunk<T>& c, const Span<kShift>& s) {
+  if constexpr (kShift) {
+    if (s.whole()) return;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = from_f32<T>(v[j]);
-  } else if (n > 0) {
+      if (j < s.lo || j >= s.hi) {
+        if constexpr (sizeof(T) == 4) c.w[j] = 0u;
+        else c.w[j >> 1] &= (j & 1) ? 0x0000ffffu : 0xffff0000u;
+      }
+  }
+}
+template <bool kShift, typename T>
+__device__ __forceinline__ void store_chunk(T* p, const float* v, const Span<kShift>& s) {
+  if (s.whole()) {
     if constexpr (sizeof(T) == 4) {
       reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
       reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
     } else {
       *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
     }
+  } else if constexpr (kShift) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j >= s.lo && j < s.hi) p[j] = from_f32<T>(v[j]);
   }
 }
 
 // v * inv as e4m3.  inv is the row's 1 / scale: a division for every element made this kernel slower than its memory traffic
 // (8192 x 5120 bf16: 125 us a pass with, 72 us without); the product's extra rounding of 2^-24 moves a value only where it lies
 // that near to the middle of two e4m3 values.  Saturation turns 448 (1 + 2^-23) into 448.
-template <bool kVec>
-__device__ __forceinline__ void store_e4m3(__nv_fp8_e4m3* p, const float* v, float inv, int n) {
+template <bool kShift>
+__device__ __forceinline__ void store_e4m3(__nv_fp8_e4m3* p, const float* v, float inv, const Span<kShift>& s) {
   uint32_t e[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) e[j] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * j] * inv, v[2 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-  if constexpr (kVec) {
-    if (n > 0) *reinterpret_cast<uint2*>(p) = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
-  } else {
+  if (s.whole()) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
+  } else if constexpr (kShift) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j < n) p[j].__x = static_cast<__nv_fp8_storage_t>(e[j / 2] >> (8 * (j & 1)));
+      if (j >= s.lo && j < s.hi) p[j].__x = static_cast<__nv_fp8_storage_t>(e[j / 2] >> (8 * (j & 1)));
   }
 }
 
@@ -114,49 +156,96 @@ struct Dropout {
 };
 
 struct Mask {
-  uint32_t key[20];  // the ten rounds' two key words
-  uint32_t step, stream, threshold;
+  uint32_t k0, k1, lo, first, second;  // seed; round 1 of the words that do not depend on the block (see words)
+  uint32_t threshold;
   float scale;
 
-  __device__ explicit Mask(const Dropout& d) : step(0), stream(d.stream), threshold(d.threshold), scale(d.scale) {
-    uint32_t k0 = 0, k1 = 0;
-    if (d.rng != nullptr) {
-      const unsigned long long seed = static_cast<unsigned long long>(__ldg(d.rng));
-      k0 = static_cast<uint32_t>(seed);
-      k1 = static_cast<uint32_t>(seed >> 32);
-      step = static_cast<uint32_t>(__ldg(d.rng + 1));
+  __device__ explicit Mask(const Dropout& d) : threshold(d.threshold), scale(d.scale) {
+    const unsigned long long seed = static_cast<unsigned long long>(__ldg(d.rng));
+    k0 = static_cast<uint32_t>(seed);
+    k1 = static_cast<uint32_t>(seed >> 32);
+    const unsigned long long p1 = static_cast<unsigned long long>(static_cast<uint32_t>(__ldg(d.rng + 1))) * 0xCD9E8D57u;
+    lo = static_cast<uint32_t>(p1);
+    first = static_cast<uint32_t>(p1 >> 32) ^ k0;
+    second = d.stream ^ k1;
+  }
+  // The words of kN blocks, in step: the key words advance once for all of them, which costs fewer instructions than a key
+  // schedule each and fewer registers than one that is kept (16384 x 14336 bf16: 266 us with it kept, KTD us so).
+  template <int kN>
+  __device__ __forceinline__ void words(const unsigned long long (&block)[kN], uint32_t* u) const {
+    uint32_t c0[kN], c1[kN], c2[kN], c3[kN], a = k0, b = k1;
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const unsigned long long p0 = static_cast<unsigned long long>(static_cast<uint32_t>(block[n])) * 0xD2511F53u;
+      c0[n] = first ^ static_cast<uint32_t>(block[n] >> 32);
+      c1[n] = lo;
+      c2[n] = static_cast<uint32_t>(p0 >> 32) ^ second;
+      c3[n] = static_cast<uint32_t>(p0);
     }
 #pragma unroll
-    for (int i = 0; i < 10; ++i) {
-      key[2 * i] = k0 + i * 0x9E3779B9u;
-      key[2 * i + 1] = k1 + i * 0xBB67AE85u;
+    for (int i = 1; i < 10; ++i) {
+      a += 0x9E3779B9u;
+      b += 0xBB67AE85u;
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        const unsigned long long p0 = static_cast<unsigned long long>(c0[n]) * 0xD2511F53u;
+        const unsigned long long p1 = static_cast<unsigned long long>(c2[n]) * 0xCD9E8D57u;
+        c0[n] = static_cast<uint32_t>(p1 >> 32) ^ c1[n] ^ a;
+        c1[n] = static_cast<uint32_t>(p1);
+        c2[n] = static_cast<uint32_t>(p0 >> 32) ^ c3[n] ^ b;
+        c3[n] = static_cast<uint32_t>(p0);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      u[4 * n] = c0[n];
+      u[4 * n + 1] = c1[n];
+      u[4 * n + 2] = c2[n];
+      u[4 * n + 3] = c3[n];
     }
   }
-  __device__ __forceinline__ uint4 words(unsigned long long block) const {
-    uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32), c2 = step, c3 = stream;
+  // the words of 8 elements that begin at word `phase` (0 .. 3) of `block`
+  template <bool kShift>
+  __device__ __forceinline__ void words8(unsigned long long block, int phase, uint32_t* u) const {
+    if constexpr (kShift) {
+      if (phase != 0) {
+        words<3>({block, block + 1, block + 2}, u);
+        if (phase & 1) {
 #pragma unroll
-    for (int i = 0; i < 10; ++i) {
-      const unsigned long long p0 = static_cast<unsigned long long>(c0) * 0xD2511F53u;
-      const unsigned long long p1 = static_cast<unsigned long long>(c2) * 0xCD9E8D57u;
-      c0 = static_cast<uint32_t>(p1 >> 32) ^ c1 ^ key[2 * i];
-      c1 = static_cast<uint32_t>(p1);
-      c2 = static_cast<uint32_t>(p0 >> 32) ^ c3 ^ key[2 * i + 1];
-      c3 = static_cast<uint32_t>(p0);
+          for (int j = 0; j < 11; ++j) u[j] = u[j + 1];
+        }
+        if (phase & 2) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) u[j] = u[j + 2];
+        }
+        return;
+      }
     }
-    return make_uint4(c0, c1, c2, c3);
+    words<2>({block, block + 1}, u);
   }
-  // the 8 values of a chunk whose first generator block is `block`, after dropout: a dropped value is +0 whatever it held
-  __device__ __forceinline__ void apply(float* v, unsigned long long block) const {
+  // a dropped value is +0 whatever it held
+  __device__ __forceinline__ float apply(float v, uint32_t u) const { return u >= threshold ? v * scale : 0.0f; }
+  // 8 values of `row` from column c0 on (kShift: c0 may be any, also below zero, where the values are not used)
+  template <bool kShift>
+  __device__ __forceinline__ void apply8(float* v, long long row, int blocks, int c0) const {
+    uint32_t u[12];
+    words8<kShift>(static_cast<unsigned long long>(row * blocks + (c0 >> 2)), kShift ? c0 & 3 : 0, u);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint4 u = words(block + k);
-      v[4 * k] = u.x >= threshold ? v[4 * k] * scale : 0.0f;
-      v[4 * k + 1] = u.y >= threshold ? v[4 * k + 1] * scale : 0.0f;
-      v[4 * k + 2] = u.z >= threshold ? v[4 * k + 2] * scale : 0.0f;
-      v[4 * k + 3] = u.w >= threshold ? v[4 * k + 3] * scale : 0.0f;
-    }
+    for (int j = 0; j < 8; ++j) v[j] = apply(v[j], u[j]);
   }
 };
+struct NoMask {
+  __device__ explicit NoMask(const Dropout&) {}
+  template <bool kShift>
+  __device__ __forceinline__ void apply8(float*, long long, int, int) const {}
+};
+template <bool kDrop>
+using MaskOf = typename std::conditional<kDrop, Mask, NoMask>::type;
+
+// The [seed, step] a forward used, for its backward.
+__device__ __forceinline__ void note_used(const Dropout& d, long long* used) {
+  if (used != nullptr && blockIdx.x == 0 && threadIdx.x < 2) used[threadIdx.x] = d.rng != nullptr ? d.rng[threadIdx.x] : 0;
+}
 
 // max that keeps NaN
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -164,65 +253,100 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// (sum of a, max of b) over the kGroup threads of a row: a warp, or the whole block
-template <int kGroup, bool kMax>
-__device__ __forceinline__ void row_reduce(float& a, float& b, float* red) {
+// (sum of a, max of b >= 0) over the threads of a row: a warp (kWarp), or the whole block of at most 32 warps.  `red` is
+// two buffers of 64 floats used in turn, `turn` counts the calls: a buffer is written again only after the synchronisation
+// of the call in between, so one is enough.
+template <bool kWarp, bool kMax>
+__device__ __forceinline__ void row_reduce(float& a, float& b, float* red, int& turn) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     a += __shfl_xor_sync(0xffffffffu, a, o);
     if (kMax) b = max_nan(b, __shfl_xor_sync(0xffffffffu, b, o));
   }
-  if constexpr (kGroup > 32) {
-    constexpr int kWarps = kGroup / 32;
-    __syncthreads();  // the previous use of red is over
-    if ((threadIdx.x & 31) == 0) {
-      red[threadIdx.x >> 5] = a;
-      if (kMax) red[kWarps + (threadIdx.x >> 5)] = b;
+  if constexpr (!kWarp) {
+    float* r = red + 64 * (turn++ & 1);
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) {
+      r[threadIdx.x >> 5] = a;
+      if (kMax) r[32 + (threadIdx.x >> 5)] = b;
     }
     __syncthreads();
-    a = red[0];
-    if (kMax) b = red[kWarps];
+    a = lane < warps ? r[lane] : 0.f;
+    if (kMax) b = lane < warps ? r[32 + lane] : 0.f;
 #pragma unroll
-    for (int i = 1; i < kWarps; ++i) {
-      a += red[i];
-      if (kMax) b = max_nan(b, red[kWarps + i]);
+    for (int o = 16; o > 0; o >>= 1) {
+      a += __shfl_xor_sync(0xffffffffu, a, o);
+      if (kMax) b = max_nan(b, __shfl_xor_sync(0xffffffffu, b, o));
     }
   }
 }
 
 // ------------------------------------------------------------------ dropout alone
-// A stream of chunks, kDropUnroll of them in flight a thread.  Rows whose length is a multiple of 4 are one long row (the
-// generator's blocks do not care), so `cols` may exceed 31 bits here.
-constexpr int kDropThreads = 256, kDropUnroll = 2;
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kDropThreads) dropout_kernel(const T* __restrict__ x, T* __restrict__ out, long long rows, long long cols,
-                                                               Dropout d, long long* __restrict__ used) {
-  const Mask mask(d);
-  if (used != nullptr && blockIdx.x == 0 && threadIdx.x < 2) used[threadIdx.x] = d.rng != nullptr ? d.rng[threadIdx.x] : 0;
-  const bool drop = d.rng != nullptr;
-  const long long per_row = (cols + 7) / 8, blocks = (cols + 3) / 4, total = rows * per_row;
+// A stream of chunks of the whole matrix, kDropUnroll of them in flight a thread.  Bound by HBM without the generator, by
+// issue slots and registers with it (ten rounds are 40 instructions for 4 elements, 20 key words stay in registers): the
+// grid is what fits the SMs at once.
+constexpr int kDropThreads = 256, kDropUnroll = 2, kDropBlocksPerSm = 5;
+template <typename T, bool kShift, bool kDrop>
+__global__ void __launch_bounds__(kDropThreads, kDropBlocksPerSm)
+dropout_kernel(const T* __restrict__ x, T* __restrict__ out, long long total, long long cols, Dropout d, long long* __restrict__ used) {
+  const MaskOf<kDrop> mask(d);
+  note_used(d, used);
+  const long long chunks = (total + 7) / 8, blocks = (cols + 3) / 4;
   const long long stride = static_cast<long long>(gridDim.x) * kDropThreads;
-  for (long long i0 = blockIdx.x * static_cast<long long>(kDropThreads) + threadIdx.x; i0 < total; i0 += stride * kDropUnroll) {
+  for (long long i0 = blockIdx.x * static_cast<long long>(kDropThreads) + threadIdx.x; i0 < chunks; i0 += stride * kDropUnroll) {
     Chunk<T> in[kDropUnroll];
-    long long at[kDropUnroll], block[kDropUnroll];
-    int n[kDropUnroll];
 #pragma unroll
     for (int k = 0; k < kDropUnroll; ++k) {
-      const long long i = i0 + k * stride;
-      const long long row = rows == 1 ? 0 : i / per_row, c = 8 * (i - row * per_row);
-      n[k] = i < total ? static_cast<int>(cols - c < 8 ? cols - c : 8) : 0;
-      at[k] = row * cols + c;
-      block[k] = row * blocks + c / 4;
-      in[k] = load_chunk<kVec>(x + at[k], n[k]);
+      const long long e = 8 * (i0 + k * stride);
+      if (e + 8 <= total) in[k] = load_whole(x + e);
+      else in[k] = load_some(x + e, 0, e < total ? static_cast<int>(total - e) : 0);
+    }
+    uint32_t all[kDropUnroll * 8];
+    if constexpr (kDrop && !kShift) {  // cols % 4 == 0: a row's blocks follow the previous row's
+      unsigned long long block[2 * kDropUnroll];
+#pragma unroll
+      for (int k = 0; k < 2 * kDropUnroll; ++k) block[k] = 2 * static_cast<unsigned long long>(i0 + k / 2 * stride) + (k & 1);
+      mask.template words<2 * kDropUnroll>(block, all);
     }
 #pragma unroll
     for (int k = 0; k < kDropUnroll; ++k) {
-      if (n[k] <= 0) break;
+      const long long e = 8 * (i0 + k * stride);
+      if (e >= total) break;
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = chunk_get(in[k], j);
-      if (drop) mask.apply(v, block[k]);
-      store_chunk<kVec>(out + at[k], v, n[k]);
+      if constexpr (kDrop) {
+        uint32_t u[12];
+        if constexpr (!kShift) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) u[j] = all[8 * k + j];
+        } else {
+          long long row = total <= 0xffffffffLL ? static_cast<uint32_t>(e) / static_cast<uint32_t>(cols) : e / cols;
+          long long c = e - row * cols;
+          mask.template words8<true>(static_cast<unsigned long long>(row * blocks + c / 4), static_cast<int>(c & 3), u);
+          if (c + 8 > cols) {  // the next row (or rows) begins inside the chunk
+            uint32_t t[4] = {0u, 0u, 0u, 0u};
+            bool next = false;
+#pragma unroll
+            for (int j = 0; j < 8; ++j, ++c) {
+              if (c == cols) {
+                c = 0;
+                ++row;
+                next = true;
+              }
+              if (next) {
+                const int q = static_cast<int>(c & 3);
+                if (q == 0) mask.template words<1>({static_cast<unsigned long long>(row * blocks + c / 4)}, t);
+                u[j] = q == 0 ? t[0] : q == 1 ? t[1] : q == 2 ? t[2] : t[3];
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = mask.apply(v[j], u[j]);
+      }
+      const long long left = total - e;
+      store_chunk<true>(out + e, v, Span<true>(0, left < 8 ? static_cast<int>(left) : 8));
     }
   }
 }
@@ -232,79 +356,103 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const T* __restri
 // h * rstd * w.  kE4M3: out leaves as e4m3 values q with scale = max(max|out| / 448, 2^-126), q = out / scale rounded
 // once; without a weight the rows are converted as they are.
 //
-// Bound by HBM.  kGroup threads own a row (a warp: kGroup = 32, several rows a block; else the block) and keep its h in
-// registers as kChunks chunks each, so every tensor is read or written once; row_reduce is the only synchronisation.
-template <typename T, bool kVec, int kGroup, int kChunks, bool kE4M3>
-__global__ void __launch_bounds__(kGroup < 256 ? 256 : kGroup)
+// Bound by HBM: every tensor is read or written once.  The block (kWarp: a warp) owns a row and keeps its h in registers,
+// kChunks chunks a thread; the grid is what fits the SMs at once, and a row's successor is loaded while the row is reduced
+// and written.  A thread stays on the same columns for all of its rows (kShift: the grid's row stride is a multiple of 8, so
+// `off` stays too), so the weights are loaded once.
+constexpr int kWarpBlock = 256, kMaxThreads = 512;
+// Registers a thread, and so threads an SM, of each kernel (kMaxThreads of 128 registers fill one): two chunks of a 2-byte type fit 64 in the forward; fp32 chunks
+// and the shift's masks take 80; four chunks a thread, and the backward with its sums and prefetch, take 128.  With the
+// shift the backward has 112: a row of 4095 columns needs one warp more than one of 4096, and two such blocks have to fit.
+constexpr int fwd_regs(int elem_bytes, bool shift, int chunks) { return chunks == 4 ? 128 : (elem_bytes == 4 || shift) ? 80 : 64; }
+constexpr int bwd_regs(bool shift, int chunks) { return shift && chunks == 2 ? 112 : 128; }
+constexpr int threads_per_sm(int regs) { return 65536 / regs / 32 * 32; }
+
+template <bool kWarp>
+struct RowLoop {
+  long long row, step;
+  int tid, width;  // this thread and the number of threads of the row
+  __device__ RowLoop()
+      : row(kWarp ? static_cast<long long>(blockIdx.x) * (kWarpBlock / 32) + threadIdx.x / 32 : blockIdx.x),
+        step(kWarp ? static_cast<long long>(gridDim.x) * (kWarpBlock / 32) : gridDim.x),
+        tid(kWarp ? threadIdx.x & 31 : threadIdx.x),
+        width(kWarp ? 32 : blockDim.x) {}
+  // elements of the row's first chunk that belong to the row before it (kShift)
+  __device__ int offset(int cols) const { return static_cast<int>((row * cols) & 7); }
+};
+
+template <typename T, bool kShift, bool kDrop, bool kWarp, int kChunks, bool kE4M3>
+__global__ void __maxnreg__(fwd_regs(sizeof(T), kShift, kChunks))
 norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T* __restrict__ weight, float eps, Dropout d,
                 long long* __restrict__ used, T* __restrict__ h, T* __restrict__ out, float* __restrict__ rstd,
                 __nv_fp8_e4m3* __restrict__ q, float* __restrict__ scale, long long rows, int cols) {
-  __shared__ float red[2 * 32];
-  const Mask mask(d);
-  if (used != nullptr && blockIdx.x == 0 && threadIdx.x < 2) used[threadIdx.x] = d.rng != nullptr ? d.rng[threadIdx.x] : 0;
-  const bool drop = d.rng != nullptr;
+  __shared__ float red[kWarp ? 1 : 128];
+  int turn = 0;
+  const MaskOf<kDrop> mask(d);
+  note_used(d, used);
   const int blocks = (cols + 3) / 4;
-  const int lane = kGroup == 32 ? (threadIdx.x & 31) : threadIdx.x;
-  const int per_block = kGroup == 32 ? blockDim.x / 32 : 1;
-  for (long long row = static_cast<long long>(blockIdx.x) * per_block + (kGroup == 32 ? threadIdx.x / 32 : 0); row < rows;
-       row += static_cast<long long>(gridDim.x) * per_block) {
-    const long long base = row * cols;
-    float v[kChunks][8];
-    Chunk<T> a[kChunks], b[kChunks];
+  const long long total = rows * cols;
+  RowLoop<kWarp> at;
+  if (at.row >= rows) return;  // all threads of the row leave together
+  const int off = kShift ? at.offset(cols) : 0;
+  auto span = [&](int k) { return Span<kShift>(8 * (at.tid + k * at.width) - off, cols); };
+  Chunk<T> w[kChunks], a[kChunks], b[kChunks];
+#pragma unroll
+  for (int k = 0; k < kChunks; ++k)
+    if (weight != nullptr) w[k] = kShift ? load_some(weight + span(k).c0, span(k).lo, span(k).hi) : load_chunk(weight + span(k).c0, span(k), 8);
+  auto load = [&](long long row) {
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
-      const int c = 8 * (lane + k * kGroup), n = cols - c;
-      a[k] = load_chunk<kVec>(x + base + c, n);
-      if (residual != nullptr) b[k] = load_chunk<kVec>(residual + base + c, n);
+      const Span<kShift> s = span(k);
+      const long long e = row * cols + s.c0;
+      a[k] = load_chunk(x + e, s, total - e);
+      if (residual != nullptr) b[k] = load_chunk(residual + e, s, total - e);
     }
-    float sq = 0.f, top = 0.f;
+  };
+  load(at.row);
+  for (; at.row < rows; at.row += at.step) {
+    const long long base = at.row * cols;
+    float v[kChunks][8], sq = 0.f, top = 0.f;
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
-      const int c = 8 * (lane + k * kGroup), n = cols - c;
+      const Span<kShift> s = span(k);
+      mask_chunk(a[k], s);
+      if (residual != nullptr) mask_chunk(b[k], s);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[k][j] = chunk_get(a[k], j);
-      if (drop && n > 0) mask.apply(v[k], static_cast<unsigned long long>(row) * blocks + c / 4);
+      if (kDrop && s.any()) mask.template apply8<kShift>(v[k], at.row, blocks, s.c0);
       if (residual != nullptr) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[k][j] += chunk_get(b[k], j);
       }
-      if (h != nullptr) store_chunk<kVec>(h + base + c, v[k], n);
-      // (elements past the row are zero: x reads as zero there and dropout keeps zeros)
+      // (elements outside the row are zero: they were masked, and dropout keeps zeros)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sq = fmaf(v[k][j], v[k][j], sq);
-      if (kE4M3) {
-        if (weight != nullptr) {
-          const Chunk<T> w = load_chunk<kVec>(weight + c, n);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(v[k][j] * chunk_get(w, j)));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(v[k][j]));
-        }
+      for (int j = 0; j < 8; ++j) {
+        sq = fmaf(v[k][j], v[k][j], sq);
+        if (kE4M3) top = max_nan(top, fabsf(weight != nullptr ? v[k][j] * chunk_get(w[k], j) : v[k][j]));
       }
     }
-    row_reduce<kGroup, kE4M3>(sq, top, red);
+    if (at.row + at.step < rows) load(at.row + at.step);
+    if (h != nullptr) {
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) store_chunk(h + base + span(k).c0, v[k], span(k));
+    }
+    row_reduce<kWarp, kE4M3>(sq, top, red, turn);
     const float r = weight != nullptr ? rsqrtf(sq / static_cast<float>(cols) + eps) : 1.0f;
-    float s = 1.0f;
-    if (kE4M3) s = max_nan(top * r / 448.0f, 1.17549435e-38f);
-    const float inv = 1.0f / s;
-    if (lane == 0) {
-      if (kE4M3) scale[row] = s;
-      else rstd[row] = r;
+    const float s8 = max_nan(top * r / 448.0f, 1.17549435e-38f), inv = 1.0f / s8;
+    if (at.tid == 0) {
+      if (kE4M3) scale[at.row] = s8;
+      else rstd[at.row] = r;
     }
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
-      const int c = 8 * (lane + k * kGroup), n = cols - c;
+      const Span<kShift> s = span(k);
       if (weight != nullptr) {
-        const Chunk<T> w = load_chunk<kVec>(weight + c, n);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[k][j] = v[k][j] * r * chunk_get(w, j);
+        for (int j = 0; j < 8; ++j) v[k][j] = v[k][j] * r * chunk_get(w[k], j);
       }
-      if constexpr (kE4M3) {
-        store_e4m3<kVec>(q + base + c, v[k], inv, n);
-      } else {
-        store_chunk<kVec>(out + base + c, v[k], n);
-      }
+      if constexpr (kE4M3) store_e4m3(q + base + s.c0, v[k], inv, s);
+      else store_chunk(out + base + s.c0, v[k], s);
     }
   }
 }
@@ -314,199 +462,243 @@ norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T
 // h is the stored one: in a 2-byte type dw and xh carry its half step.  (Forming h again from x and residual would read one
 // more tensor, ten instead of nine tensor passes a step.)
 //
-// Bound by HBM.  Rows are owned as in the forward; a persistent grid keeps each thread on the same columns, so dw is summed
-// in registers and leaves as one partial row a block, which fold_rows_kernel adds in a fixed order.
-template <typename T, bool kVec, int kGroup, int kChunks>
-__global__ void __launch_bounds__(kGroup < 256 ? 256 : kGroup)
+// Bound by HBM, and laid out as the forward; dw is summed in registers over a thread's rows and leaves as one partial row a
+// block, which fold_rows_kernel adds in a fixed order.
+template <typename T, bool kShift, bool kDrop, bool kWarp, int kChunks>
+__global__ void __maxnreg__(bwd_regs(kShift, kChunks))
 norm_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* __restrict__ h, const float* __restrict__ rstd,
                 const T* __restrict__ weight, Dropout d, T* __restrict__ dx, T* __restrict__ dres, float* __restrict__ partial,
                 long long rows, int cols) {
-  __shared__ float red[2 * 32];
-  __shared__ float fold[kGroup == 32 ? 32 * kChunks * 8 : 1];
-  const Mask mask(d);
-  const bool drop = d.rng != nullptr;
+  // the next row's loads need as many registers again: affordable for two chunks of a 2-byte type
+  constexpr bool kPrefetch = sizeof(T) == 2 && kChunks <= 2;
+  __shared__ float red[kWarp ? 1 : 128];
+  __shared__ float fold[kWarp ? 256 : 1];
+  int turn = 0;
+  const MaskOf<kDrop> mask(d);
   const int blocks = (cols + 3) / 4;
-  const int lane = kGroup == 32 ? (threadIdx.x & 31) : threadIdx.x;
-  const int per_block = kGroup == 32 ? blockDim.x / 32 : 1;
-  float acc[kChunks][8];
-#pragma unroll
-  for (int k = 0; k < kChunks; ++k)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[k][j] = 0.f;
-  for (long long row = static_cast<long long>(blockIdx.x) * per_block + (kGroup == 32 ? threadIdx.x / 32 : 0); row < rows;
-       row += static_cast<long long>(gridDim.x) * per_block) {
-    const long long base = row * cols;
-    const float r = rstd[row];
-    Chunk<T> o[kChunks], hh[kChunks], e[kChunks];
+  const long long total = rows * cols;
+  RowLoop<kWarp> at;
+  const int off = kShift ? at.offset(cols) : 0;
+  auto span = [&](int k) { return Span<kShift>(8 * (at.tid + k * at.width) - off, cols); };
+  struct Row {
+    Chunk<T> o[kChunks], h[kChunks], e[kChunks];
+    float r;
+  };
+  auto load = [&](long long row, Row& in) {
+    in.r = rstd[row];
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
-      const int c = 8 * (lane + k * kGroup), n = cols - c;
-      o[k] = load_chunk<kVec>(dout + base + c, n);
-      hh[k] = load_chunk<kVec>(h + base + c, n);
-      if (dh != nullptr) e[k] = load_chunk<kVec>(dh + base + c, n);
+      const Span<kShift> s = span(k);
+      const long long e = row * cols + s.c0;
+      in.o[k] = load_chunk(dout + e, s, total - e);
+      in.h[k] = load_chunk(h + e, s, total - e);
+      if (dh != nullptr) in.e[k] = load_chunk(dh + e, s, total - e);
     }
+  };
+  Chunk<T> w[kChunks];
+  float acc[kChunks][8];
+#pragma unroll
+  for (int k = 0; k < kChunks; ++k) {
+    w[k] = kShift ? load_some(weight + span(k).c0, span(k).lo, span(k).hi) : load_chunk(weight + span(k).c0, span(k), 8);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[k][j] = 0.f;
+  }
+  Row cur, nxt;
+  if (kPrefetch && at.row < rows) load(at.row, cur);
+  for (; at.row < rows; at.row += at.step) {
+    if constexpr (kPrefetch) {
+      if (at.row + at.step < rows) load(at.row + at.step, nxt);
+    } else {
+      load(at.row, cur);
+    }
+    const long long base = at.row * cols;
+    const float r = cur.r;
     float dot = 0.f, unused = 0.f;
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
-      const int c = 8 * (lane + k * kGroup), n = cols - c;
-      const Chunk<T> w = load_chunk<kVec>(weight + c, n);
+      mask_chunk(cur.o[k], span(k));
+      mask_chunk(cur.h[k], span(k));
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float t = chunk_get(o[k], j) * (chunk_get(hh[k], j) * r);
+        const float t = chunk_get(cur.o[k], j) * (chunk_get(cur.h[k], j) * r);
         acc[k][j] += t;
-        dot = fmaf(t, chunk_get(w, j), dot);
+        dot = fmaf(t, chunk_get(w[k], j), dot);
       }
     }
-    row_reduce<kGroup, false>(dot, unused, red);
+    row_reduce<kWarp, false>(dot, unused, red, turn);
     const float m = dot / static_cast<float>(cols);
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
-      const int c = 8 * (lane + k * kGroup), n = cols - c;
-      const Chunk<T> w = load_chunk<kVec>(weight + c, n);
+      const Span<kShift> s = span(k);
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[j] = r * (chunk_get(o[k], j) * chunk_get(w, j) - chunk_get(hh[k], j) * r * m);
-        if (dh != nullptr) v[j] += chunk_get(e[k], j);
+        v[j] = r * (chunk_get(cur.o[k], j) * chunk_get(w[k], j) - chunk_get(cur.h[k], j) * r * m);
+        if (dh != nullptr) v[j] += chunk_get(cur.e[k], j);
       }
-      if (dres != nullptr) store_chunk<kVec>(dres + base + c, v, n);
+      if (dres != nullptr) store_chunk(dres + base + s.c0, v, s);
       if (dx != nullptr) {
-        if (drop && n > 0) mask.apply(v, static_cast<unsigned long long>(row) * blocks + c / 4);
-        store_chunk<kVec>(dx + base + c, v, n);
+        if (kDrop && s.any()) mask.template apply8<kShift>(v, at.row, blocks, s.c0);
+        store_chunk(dx + base + s.c0, v, s);
       }
     }
+    if constexpr (kPrefetch) cur = nxt;
   }
   if (partial == nullptr) return;
   float* mine = partial + static_cast<long long>(blockIdx.x) * cols;
-  if constexpr (kGroup == 32) {
+  if constexpr (kWarp) {
     // the warps of a block add up in turn
-    for (int w = 0; w < static_cast<int>(blockDim.x) / 32; ++w) {
-      if (static_cast<int>(threadIdx.x) / 32 == w) {
+    for (int c = threadIdx.x; c < cols; c += kWarpBlock) fold[c] = 0.f;
+    __syncthreads();
+    for (int i = 0; i < kWarpBlock / 32; ++i) {
+      if (static_cast<int>(threadIdx.x) / 32 == i) {
 #pragma unroll
         for (int k = 0; k < kChunks; ++k)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float* f = fold + (k * 32 + lane) * 8 + j;
-            *f = w == 0 ? acc[k][j] : *f + acc[k][j];
-          }
+          for (int j = 0; j < 8; ++j)
+            if (j >= span(k).lo && j < span(k).hi) fold[span(k).c0 + j] += acc[k][j];
       }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < cols; c += blockDim.x) mine[c] = fold[c];
+    for (int c = threadIdx.x; c < cols; c += kWarpBlock) mine[c] = fold[c];
   } else {
 #pragma unroll
-    for (int k = 0; k < kChunks; ++k) {
-      const int c = 8 * (lane + k * kGroup);
+    for (int k = 0; k < kChunks; ++k)
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (c + j < cols) mine[c + j] = acc[k][j];
-    }
+        if (j >= span(k).lo && j < span(k).hi) mine[span(k).c0 + j] = acc[k][j];
   }
 }
 
 // ------------------------------------------------------------------ rows longer than registers hold
-// The same mathematics for rows of more than kMaxCols columns: one block a row, which reads its operands twice (the second
+// The same mathematics for rows of more than 4 * kMaxThreads chunks: one block a row, which reads its operands twice (the second
 // time mostly from L2) and keeps its dw sums in the partial row itself.
-constexpr int kMaxCols = 16384, kColsLimit = 1 << 30;
+constexpr int kColsLimit = 1 << 30;
 constexpr int kLongThreads = 1024;
-template <typename T, bool kVec, bool kE4M3>
+template <typename T, bool kShift, bool kDrop, bool kE4M3>
 __global__ void __launch_bounds__(kLongThreads)
 norm_fwd_long_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T* __restrict__ weight, float eps, Dropout d,
                      long long* __restrict__ used, T* __restrict__ h, T* __restrict__ out, float* __restrict__ rstd,
                      __nv_fp8_e4m3* __restrict__ q, float* __restrict__ scale, long long rows, int cols) {
-  __shared__ float red[2 * 32];
-  const Mask mask(d);
-  if (used != nullptr && blockIdx.x == 0 && threadIdx.x < 2) used[threadIdx.x] = d.rng != nullptr ? d.rng[threadIdx.x] : 0;
+  __shared__ float red[128];
+  int turn = 0;
+  const MaskOf<kDrop> mask(d);
+  note_used(d, used);
   const int blocks = (cols + 3) / 4;
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-    const long long base = row * cols;
-    auto value = [&](int c, float* v) {  // h of the chunk at c, unrounded
-      const Chunk<T> a = load_chunk<kVec>(x + base + c, cols - c);
+  const long long total = rows * cols;
+  for (RowLoop<false> at; at.row < rows; at.row += at.step) {
+    const long long base = at.row * cols;
+    const int first = 8 * at.tid - (kShift ? at.offset(cols) : 0);
+    auto value = [&](const Span<kShift>& s, float* v) {  // h of a chunk, unrounded
+      const long long e = base + s.c0;
+      Chunk<T> a = load_chunk(x + e, s, total - e);
+      mask_chunk(a, s);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = chunk_get(a, j);
-      if (d.rng != nullptr) mask.apply(v, static_cast<unsigned long long>(row) * blocks + c / 4);
+      if (kDrop) mask.template apply8<kShift>(v, at.row, blocks, s.c0);
       if (residual != nullptr) {
-        const Chunk<T> b = load_chunk<kVec>(residual + base + c, cols - c);
+        Chunk<T> b = load_chunk(residual + e, s, total - e);
+        mask_chunk(b, s);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += chunk_get(b, j);
       }
     };
+    auto weights = [&](const Span<kShift>& s) {
+      return kShift ? load_some(weight + s.c0, s.lo, s.hi) : load_chunk(weight + s.c0, s, 8);
+    };
     float sq = 0.f, top = 0.f, v[8];
-    for (int c = 8 * threadIdx.x; c < cols; c += 8 * kLongThreads) {
-      value(c, v);
-      if (h != nullptr) store_chunk<kVec>(h + base + c, v, cols - c);
+    for (int c = first; c < cols; c += 8 * kLongThreads) {
+      const Span<kShift> s(c, cols);
+      value(s, v);
+      if (h != nullptr) store_chunk(h + base + c, v, s);
 #pragma unroll
       for (int j = 0; j < 8; ++j) sq = fmaf(v[j], v[j], sq);
       if (kE4M3) {
-        Chunk<T> w;
-        if (weight != nullptr) w = load_chunk<kVec>(weight + c, cols - c);
+        if (weight != nullptr) {
+          const Chunk<T> w = weights(s);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(weight != nullptr ? v[j] * chunk_get(w, j) : v[j]));
+          for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(v[j] * chunk_get(w, j)));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(v[j]));
+        }
       }
     }
-    row_reduce<kLongThreads, kE4M3>(sq, top, red);
+    row_reduce<false, kE4M3>(sq, top, red, turn);
     const float r = weight != nullptr ? rsqrtf(sq / static_cast<float>(cols) + eps) : 1.0f;
-    float s = 1.0f;
-    if (kE4M3) s = max_nan(top * r / 448.0f, 1.17549435e-38f);
-    const float inv = 1.0f / s;
-    if (threadIdx.x == 0) {
-      if (kE4M3) scale[row] = s;
-      else rstd[row] = r;
+    const float s8 = max_nan(top * r / 448.0f, 1.17549435e-38f), inv = 1.0f / s8;
+    if (at.tid == 0) {
+      if (kE4M3) scale[at.row] = s8;
+      else rstd[at.row] = r;
     }
-    for (int c = 8 * threadIdx.x; c < cols; c += 8 * kLongThreads) {
-      value(c, v);
+    for (int c = first; c < cols; c += 8 * kLongThreads) {
+      const Span<kShift> s(c, cols);
+      value(s, v);
       if (weight != nullptr) {
-        const Chunk<T> w = load_chunk<kVec>(weight + c, cols - c);
+        const Chunk<T> w = weights(s);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = v[j] * r * chunk_get(w, j);
       }
-      if constexpr (kE4M3) store_e4m3<kVec>(q + base + c, v, inv, cols - c);
-      else store_chunk<kVec>(out + base + c, v, cols - c);
+      if constexpr (kE4M3) store_e4m3(q + base + c, v, inv, s);
+      else store_chunk(out + base + c, v, s);
     }
   }
 }
 
-template <typename T, bool kVec>
+template <typename T, bool kShift, bool kDrop>
 __global__ void __launch_bounds__(kLongThreads)
 norm_bwd_long_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* __restrict__ h, const float* __restrict__ rstd,
                      const T* __restrict__ weight, Dropout d, T* __restrict__ dx, T* __restrict__ dres, float* __restrict__ partial,
                      long long rows, int cols) {
-  __shared__ float red[2 * 32];
-  const Mask mask(d);
+  __shared__ float red[128];
+  int turn = 0;
+  const MaskOf<kDrop> mask(d);
   const int blocks = (cols + 3) / 4;
+  const long long total = rows * cols;
   float* mine = partial != nullptr ? partial + static_cast<long long>(blockIdx.x) * cols : nullptr;
-  bool first = true;
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x, first = false) {
-    const long long base = row * cols;
-    const float r = rstd[row];
+  bool first_row = true;
+  for (RowLoop<false> at; at.row < rows; at.row += at.step, first_row = false) {
+    const long long base = at.row * cols;
+    const int first = 8 * at.tid - (kShift ? at.offset(cols) : 0);
+    const float r = rstd[at.row];
+    auto operands = [&](const Span<kShift>& s, Chunk<T>& o, Chunk<T>& hh, Chunk<T>& w) {
+      const long long e = base + s.c0;
+      o = load_chunk(dout + e, s, total - e);
+      hh = load_chunk(h + e, s, total - e);
+      mask_chunk(o, s);
+      mask_chunk(hh, s);
+      w = kShift ? load_some(weight + s.c0, s.lo, s.hi) : load_chunk(weight + s.c0, s, 8);
+    };
     float dot = 0.f, unused = 0.f;
-    for (int c = 8 * threadIdx.x; c < cols; c += 8 * kLongThreads) {
-      const int n = cols - c;
-      const Chunk<T> o = load_chunk<kVec>(dout + base + c, n), hh = load_chunk<kVec>(h + base + c, n), w = load_chunk<kVec>(weight + c, n);
+    Chunk<T> o, hh, w;
+    // a column may pass from one thread to another between rows: row_reduce's synchronisation lies between the two
+    for (int c = first; c < cols; c += 8 * kLongThreads) {
+      const Span<kShift> s(c, cols);
+      operands(s, o, hh, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float t = chunk_get(o, j) * (chunk_get(hh, j) * r);
         dot = fmaf(t, chunk_get(w, j), dot);
-        if (mine != nullptr && j < n) mine[c + j] = first ? t : mine[c + j] + t;
+        if (mine != nullptr && j >= s.lo && j < s.hi) mine[c + j] = first_row ? t : mine[c + j] + t;
       }
     }
-    row_reduce<kLongThreads, false>(dot, unused, red);
+    row_reduce<false, false>(dot, unused, red, turn);
     const float m = dot / static_cast<float>(cols);
-    for (int c = 8 * threadIdx.x; c < cols; c += 8 * kLongThreads) {
-      const int n = cols - c;
-      const Chunk<T> o = load_chunk<kVec>(dout + base + c, n), hh = load_chunk<kVec>(h + base + c, n), w = load_chunk<kVec>(weight + c, n);
+    for (int c = first; c < cols; c += 8 * kLongThreads) {
+      const Span<kShift> s(c, cols);
+      operands(s, o, hh, w);
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = r * (chunk_get(o, j) * chunk_get(w, j) - chunk_get(hh, j) * r * m);
       if (dh != nullptr) {
-        const Chunk<T> e = load_chunk<kVec>(dh + base + c, n);
+        const Chunk<T> e = load_chunk(dh + base + c, s, total - base - c);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += chunk_get(e, j);
       }
-      if (dres != nullptr) store_chunk<kVec>(dres + base + c, v, n);
+      if (dres != nullptr) store_chunk(dres + base + c, v, s);
       if (dx != nullptr) {
-        if (d.rng != nullptr) mask.apply(v, static_cast<unsigned long long>(row) * blocks + c / 4);
-        store_chunk<kVec>(dx + base + c, v, n);
+        if (kDrop) mask.template apply8<kShift>(v, at.row, blocks, s.c0);
+        store_chunk(dx + base + c, v, s);
       }
     }
   }
@@ -546,6 +738,11 @@ inline int check_extents(int64_t rows, int64_t cols, int dtype) {
   return kOk;
 }
 
+inline int check_norm_extents(int64_t rows, int64_t cols, int dtype) {
+  if (cols > kColsLimit) return fail(kBadArgument, "cols must not exceed 2^30");
+  return check_extents(rows, cols, dtype);
+}
+
 inline int make_dropout(double p, const int64_t* rng, int64_t stream_id, Dropout* d) {
   if (!(p >= 0.0 && p < 1.0)) return fail(kBadArgument, "dropout probability must be at least 0 and below 1");
   if (stream_id < 0 || stream_id > 0xffffffffLL) return fail(kBadArgument, "dropout stream must fit 32 bits");
@@ -558,28 +755,32 @@ inline int make_dropout(double p, const int64_t* rng, int64_t stream_id, Dropout
   return kOk;
 }
 
-// Threads of a row and chunks a thread, by the row's length: a warp to 1024 columns, then blocks of two chunks a thread
-// (most bytes in flight for the registers), to 16384 columns.
-struct RowShape {
-  int group, chunks;
+// How a launch covers the rows: chunks a thread (1: a warp a row; 2 or 4: a block of `threads` a row; 0: the kernels for
+// long rows).  Two chunks a thread as far as they reach, in blocks of exactly as many warps as the row needs.
+struct RowPlan {
+  bool shift;
+  int chunks, threads;
+  int64_t grid;
 };
-inline RowShape row_shape(int64_t cols) {
-  const int64_t n = (cols + 7) / 8;
-  if (n <= 32) return {32, 1};
-  if (n <= 128) return {32, 4};
-  if (n <= 512) return {256, 2};
-  if (n <= 1024) return {512, 2};
-  return {1024, 2};  // the long kernels take over beyond kMaxCols
-}
-
-inline int64_t row_blocks(int64_t rows, int64_t cols) {
-  const RowShape s = row_shape(cols);
-  const int64_t per_block = s.group == 32 ? 8 : 1, need = (rows + per_block - 1) / per_block;
-  const int64_t cap = static_cast<int64_t>(sm_count()) * (2048 / (s.group < 256 ? 256 : s.group)) / 2;
-  return need < cap ? need : cap;
+inline RowPlan row_plan(int64_t rows, int64_t cols, int dtype, bool backward) {
+  RowPlan p;
+  p.shift = cols % 8 != 0;
+  const int64_t n = (cols + (p.shift ? 14 : 7)) / 8;  // chunks a row may touch
+  p.chunks = n <= 32 ? 1 : n <= 2 * kMaxThreads ? 2 : n <= 4 * kMaxThreads ? 4 : 0;
+  p.threads = p.chunks == 1 ? kWarpBlock : p.chunks == 0 ? kLongThreads : static_cast<int>((n + 32 * p.chunks - 1) / (32 * p.chunks) * 32);
+  const int64_t per_block = p.chunks == 1 ? kWarpBlock / 32 : 1, need = (rows + per_block - 1) / per_block;
+  const int fit = p.chunks == 0 ? 2 : threads_per_sm(backward ? bwd_regs(p.shift, p.chunks) : fwd_regs(dtype == 2 ? 4 : 2, p.shift, p.chunks)) / p.threads;
+  const int64_t cap = static_cast<int64_t>(sm_count()) * (fit < 1 ? 1 : fit > 32 ? 32 : fit) / 8 * 8;  // kShift: rows advance by multiples of 8
+  p.grid = need < cap ? need : cap;
+  return p;
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline int check_aligned(std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if (!aligned16(p)) return fail(kBadArgument, "matrices must be 16-byte aligned");
+  return kOk;
+}
 
 template <class F>
 int by_dtype(int dtype, F&& f) {
@@ -587,24 +788,42 @@ int by_dtype(int dtype, F&& f) {
   if (dtype == 1) return f(__half());
   return f(float());
 }
-template <int kGroup, int kChunks>
-struct Shape {
-  [[maybe_unused]] static constexpr int group = kGroup;
-  static constexpr int chunks = kChunks, threads = kGroup < 256 ? 256 : kGroup;
-};
-// chunks = 0: the kernel for long rows
 template <class F>
-int by_shape(int64_t cols, F&& f) {
-  const RowShape s = row_shape(cols);
-  if (cols > kMaxCols) return f(Shape<kLongThreads, 0>());
-  if (s.group == 32) return s.chunks == 1 ? f(Shape<32, 1>()) : f(Shape<32, 4>());
-  if (s.group == 256) return f(Shape<256, 2>());
-  if (s.group == 512) return f(Shape<512, 2>());
-  return f(Shape<1024, 2>());
+int by_flag(bool flag, F&& f) {
+  return flag ? f(std::true_type()) : f(std::false_type());
 }
 template <class F>
-int by_vec(bool vec, F&& f) {
-  return vec ? f(std::true_type()) : f(std::false_type());
+int by_chunks(int chunks, F&& f) {
+  if (chunks == 1) return f(std::integral_constant<int, 1>());
+  if (chunks == 2) return f(std::integral_constant<int, 2>());
+  if (chunks == 4) return f(std::integral_constant<int, 4>());
+  return f(std::integral_constant<int, 0>());
+}
+
+template <bool kE4M3>
+int launch_norm_fwd(const void* x, const void* residual, const void* weight, float eps, const Dropout& d, int64_t* used, void* h, void* out,
+                    float* rstd, void* q, float* scale, int64_t rows, int64_t cols, int dtype, void* stream) {
+  const RowPlan plan = row_plan(rows, cols, dtype, false);
+  return by_dtype(dtype, [&](auto t) {
+    return by_flag(plan.shift, [&](auto shift) {
+      return by_flag(!kE4M3 && d.rng != nullptr, [&](auto drop) {
+        return by_chunks(plan.chunks, [&](auto chunks) {
+          using T = decltype(t);
+          constexpr bool kShift = decltype(shift)::value, kDrop = !kE4M3 && decltype(drop)::value;
+          constexpr int kChunks = decltype(chunks)::value;
+          auto kern = [] {
+            if constexpr (kChunks == 0) return norm_fwd_long_kernel<T, kShift, kDrop, kE4M3>;
+            else return norm_fwd_kernel<T, kShift, kDrop, kChunks == 1, kChunks, kE4M3>;
+          }();
+          kern<<<static_cast<int>(plan.grid), plan.threads, 0, static_cast<cudaStream_t>(stream)>>>(
+              static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const T*>(weight), eps, d,
+              reinterpret_cast<long long*>(used), static_cast<T*>(h), static_cast<T*>(out), rstd, static_cast<__nv_fp8_e4m3*>(q), scale, rows,
+              static_cast<int>(cols));
+          return launch_check(kE4M3 ? "e4m3 rows launch" : "add_rmsnorm forward launch");
+        });
+      });
+    });
+  });
 }
 
 }  // namespace
@@ -618,19 +837,20 @@ extern "C" int coda_b200_dropout(const void* x, void* out, int64_t rows, int64_t
   if (rc != kOk) return rc;
   if (rows == 0) return kOk;
   if (!x || !out) return fail(kBadArgument, "NULL pointer");
-  if (cols % 4 == 0) {
-    cols *= rows;
-    rows = 1;
-  }
-  const long long need = (rows * ((cols + 7) / 8) + kDropThreads * kDropUnroll - 1) / (kDropThreads * kDropUnroll);
-  const long long cap = static_cast<long long>(sm_count()) * 8;
+  rc = check_aligned({x, out});
+  if (rc != kOk) return rc;
+  const long long total = rows * cols, need = ((total + 7) / 8 + kDropThreads * kDropUnroll - 1) / (kDropThreads * kDropUnroll);
+  const long long cap = static_cast<long long>(sm_count()) * kDropBlocksPerSm;
   const int grid = static_cast<int>(need < cap ? need : cap);
   return by_dtype(dtype, [&](auto t) {
-    using T = decltype(t);
-    return by_vec(rows == 1 && cols % 8 == 0 && aligned16(x) && aligned16(out), [&](auto vec) {
-      dropout_kernel<T, decltype(vec)::value><<<grid, kDropThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-          static_cast<const T*>(x), static_cast<T*>(out), rows, cols, d, reinterpret_cast<long long*>(rng_used));
-      return launch_check("dropout launch");
+    return by_flag(d.rng != nullptr, [&](auto drop) {
+      return by_flag(d.rng != nullptr && cols % 4 != 0, [&](auto shift) {
+        using T = decltype(t);
+        constexpr bool kDrop = decltype(drop)::value, kShift = kDrop && decltype(shift)::value;
+        dropout_kernel<T, kShift, kDrop><<<grid, kDropThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+            static_cast<const T*>(x), static_cast<T*>(out), total, cols, d, reinterpret_cast<long long*>(rng_used));
+        return launch_check("dropout launch");
+      });
     });
   });
 }
@@ -638,73 +858,38 @@ extern "C" int coda_b200_dropout(const void* x, void* out, int64_t rows, int64_t
 extern "C" int coda_b200_add_rmsnorm_fwd(const void* x, const void* residual, const void* weight, float eps, double p, const int64_t* rng,
                                          int64_t stream_id, int64_t* rng_used, void* h, void* out, float* rstd, int64_t rows,
                                          int64_t cols, int dtype, void* stream) {
-  int rc = check_extents(rows, cols, dtype);
-  if (rc == kOk && cols > kColsLimit) rc = fail(kBadArgument, "cols must not exceed 2^30");
+  int rc = check_norm_extents(rows, cols, dtype);
   if (rc != kOk) return rc;
   Dropout d;
   rc = make_dropout(p, rng, stream_id, &d);
   if (rc != kOk) return rc;
   if (rows == 0) return kOk;
   if (!x || !weight || !out || !rstd) return fail(kBadArgument, "NULL pointer");
-  const int grid = static_cast<int>(row_blocks(rows, cols));
-  const bool vec = cols % 8 == 0 && aligned16(x) && aligned16(residual) && aligned16(weight) && aligned16(h) && aligned16(out);
-  return by_dtype(dtype, [&](auto t) {
-    return by_shape(cols, [&](auto shape) {
-      return by_vec(vec, [&](auto v) {
-        using T = decltype(t);
-        using S = decltype(shape);
-        auto kern = [] {
-          if constexpr (S::chunks == 0) return norm_fwd_long_kernel<T, decltype(v)::value, false>;
-          else return norm_fwd_kernel<T, decltype(v)::value, S::group, S::chunks, false>;
-        }();
-        kern<<<grid, S::threads, 0, static_cast<cudaStream_t>(stream)>>>(
-            static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const T*>(weight), eps, d,
-            reinterpret_cast<long long*>(rng_used), static_cast<T*>(h), static_cast<T*>(out), rstd, nullptr, nullptr, rows,
-            static_cast<int>(cols));
-        return launch_check("add_rmsnorm forward launch");
-      });
-    });
-  });
+  rc = check_aligned({x, residual, weight, h, out});
+  if (rc != kOk) return rc;
+  return launch_norm_fwd<false>(x, residual, weight, eps, d, rng_used, h, out, rstd, nullptr, nullptr, rows, cols, dtype, stream);
 }
 
 extern "C" int coda_b200_rows_e4m3(const void* x, const void* residual, const void* weight, float eps, void* h, void* q, float* scale,
                                    int64_t rows, int64_t cols, int dtype, void* stream) {
-  int rc = check_extents(rows, cols, dtype);
-  if (rc == kOk && cols > kColsLimit) rc = fail(kBadArgument, "cols must not exceed 2^30");
+  int rc = check_norm_extents(rows, cols, dtype);
   if (rc != kOk) return rc;
   if (rows == 0) return kOk;
   if (!x || !q || !scale) return fail(kBadArgument, "NULL pointer");
+  rc = check_aligned({x, residual, weight, h, q});
+  if (rc != kOk) return rc;
   const Dropout d{nullptr, 0u, 0u, 1.0f};
-  const int grid = static_cast<int>(row_blocks(rows, cols));
-  const bool vec = cols % 8 == 0 && aligned16(x) && aligned16(residual) && aligned16(weight) && aligned16(h) &&
-                   (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
-  return by_dtype(dtype, [&](auto t) {
-    return by_shape(cols, [&](auto shape) {
-      return by_vec(vec, [&](auto v) {
-        using T = decltype(t);
-        using S = decltype(shape);
-        auto kern = [] {
-          if constexpr (S::chunks == 0) return norm_fwd_long_kernel<T, decltype(v)::value, true>;
-          else return norm_fwd_kernel<T, decltype(v)::value, S::group, S::chunks, true>;
-        }();
-        kern<<<grid, S::threads, 0, static_cast<cudaStream_t>(stream)>>>(
-            static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const T*>(weight), eps, d, nullptr, static_cast<T*>(h),
-            nullptr, nullptr, static_cast<__nv_fp8_e4m3*>(q), scale, rows, static_cast<int>(cols));
-        return launch_check("e4m3 rows launch");
-      });
-    });
-  });
+  return launch_norm_fwd<true>(x, residual, weight, eps, d, nullptr, h, nullptr, nullptr, q, scale, rows, cols, dtype, stream);
 }
 
 extern "C" int64_t coda_b200_add_rmsnorm_bwd_scratch_bytes(int64_t rows, int64_t cols) {
-  return rows <= 0 || cols <= 0 ? 0 : row_blocks(rows, cols) * cols * static_cast<int64_t>(sizeof(float));
+  return rows <= 0 || cols <= 0 ? 0 : row_plan(rows, cols, 0, true).grid * cols * static_cast<int64_t>(sizeof(float));
 }
 
 extern "C" int coda_b200_add_rmsnorm_bwd(const void* dout, const void* dh, const void* h, const float* rstd, const void* weight, double p,
                                          const int64_t* rng, int64_t stream_id, void* dx, void* dres, void* dweight, void* scratch,
                                          int64_t scratch_bytes, int64_t rows, int64_t cols, int dtype, void* stream) {
-  int rc = check_extents(rows, cols, dtype);
-  if (rc == kOk && cols > kColsLimit) rc = fail(kBadArgument, "cols must not exceed 2^30");
+  int rc = check_norm_extents(rows, cols, dtype);
   if (rc != kOk) return rc;
   Dropout d;
   rc = make_dropout(p, rng, stream_id, &d);
@@ -713,26 +898,32 @@ extern "C" int coda_b200_add_rmsnorm_bwd(const void* dout, const void* dh, const
   if (!dout || !h || !rstd || !weight) return fail(kBadArgument, "NULL pointer");
   if (dweight != nullptr && (scratch == nullptr || scratch_bytes < coda_b200_add_rmsnorm_bwd_scratch_bytes(rows, cols)))
     return fail(kBadArgument, "the weight gradient needs coda_b200_add_rmsnorm_bwd_scratch_bytes of scratch");
-  const int blocks = static_cast<int>(row_blocks(rows, cols)), n = static_cast<int>(cols);
-  const bool vec = cols % 8 == 0 && aligned16(dout) && aligned16(dh) && aligned16(h) && aligned16(weight) && aligned16(dx) && aligned16(dres);
+  rc = check_aligned({dout, dh, h, weight, dx, dres});
+  if (rc != kOk) return rc;
+  const RowPlan plan = row_plan(rows, cols, dtype, true);
+  const int n = static_cast<int>(cols);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    const int rc2 = by_shape(cols, [&](auto shape) {
-      return by_vec(vec, [&](auto v) {
-        using S = decltype(shape);
-        auto kern = [] {
-          if constexpr (S::chunks == 0) return norm_bwd_long_kernel<T, decltype(v)::value>;
-          else return norm_bwd_kernel<T, decltype(v)::value, S::group, S::chunks>;
-        }();
-        kern<<<blocks, S::threads, 0, st>>>(
-            static_cast<const T*>(dout), static_cast<const T*>(dh), static_cast<const T*>(h), rstd, static_cast<const T*>(weight), d,
-            static_cast<T*>(dx), static_cast<T*>(dres), dweight != nullptr ? static_cast<float*>(scratch) : nullptr, rows, n);
-        return launch_check("add_rmsnorm backward launch");
+    const int rc2 = by_flag(plan.shift, [&](auto shift) {
+      return by_flag(d.rng != nullptr, [&](auto drop) {
+        return by_chunks(plan.chunks, [&](auto chunks) {
+          constexpr bool kShift = decltype(shift)::value, kDrop = decltype(drop)::value;
+          constexpr int kChunks = decltype(chunks)::value;
+          auto kern = [] {
+            if constexpr (kChunks == 0) return norm_bwd_long_kernel<T, kShift, kDrop>;
+            else return norm_bwd_kernel<T, kShift, kDrop, kChunks == 1, kChunks>;
+          }();
+          kern<<<static_cast<int>(plan.grid), plan.threads, 0, st>>>(
+              static_cast<const T*>(dout), static_cast<const T*>(dh), static_cast<const T*>(h), rstd, static_cast<const T*>(weight), d,
+              static_cast<T*>(dx), static_cast<T*>(dres), dweight != nullptr ? static_cast<float*>(scratch) : nullptr, rows, n);
+          return launch_check("add_rmsnorm backward launch");
+        });
       });
     });
     if (rc2 != kOk || dweight == nullptr) return rc2;
-    fold_rows_kernel<T><<<(n + 31) / 32, 1024, 0, st>>>(static_cast<const float*>(scratch), blocks, n, static_cast<T*>(dweight));
+    fold_rows_kernel<T><<<(n + 31) / 32, 1024, 0, st>>>(static_cast<const float*>(scratch), static_cast<int>(plan.grid), n,
+                                                         static_cast<T*>(dweight));
     return launch_check("add_rmsnorm weight gradient launch");
   });
 }

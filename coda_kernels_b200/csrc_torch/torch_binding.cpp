@@ -347,7 +347,7 @@ inline int row_dtype(const Tensor& t) {
 }
 inline const int64_t* rng_ptr(const Tensor& rng) { return rng.defined() ? rng.data_ptr<int64_t>() : nullptr; }
 inline void* ptr_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-inline Tensor dense(const OptTensor& t) { return t.has_value() ? t->contiguous() : Tensor(); }
+inline Tensor dense(const OptTensor& t) { return t.has_value() ? aligned16(*t) : Tensor(); }
 
 // dropout of dense x from rng; `used` (when wanted) receives the [seed, step] the mask was made from
 Tensor run_dropout(const Tensor& x, double p, const Tensor& rng, int64_t stream, Tensor* used) {
@@ -364,7 +364,7 @@ class DropoutNode : public torch::autograd::Function<DropoutNode> {
  public:
   static Tensor forward(AutogradContext* ctx, const Tensor& x, double p, const OptTensor& rng, int64_t stream) {
     at::AutoDispatchBelowADInplaceOrView below;
-    Tensor used, out = run_dropout(x.contiguous(), p, dense(rng), stream, &used);
+    Tensor used, out = run_dropout(aligned16(x), p, dense(rng), stream, &used);
     ctx->save_for_backward({used});
     ctx->saved_data["p"] = p;
     ctx->saved_data["stream"] = stream;
@@ -373,7 +373,7 @@ class DropoutNode : public torch::autograd::Function<DropoutNode> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     require_first_order("dropout");
     const Tensor used = ctx->get_saved_variables()[0];
-    return {run_dropout(grads[0].contiguous(), ctx->saved_data["p"].toDouble(), used, ctx->saved_data["stream"].toInt(), nullptr), Tensor(),
+    return {run_dropout(aligned16(grads[0]), ctx->saved_data["p"].toDouble(), used, ctx->saved_data["stream"].toInt(), nullptr), Tensor(),
             Tensor(), Tensor()};
   }
 };
@@ -383,7 +383,7 @@ Tensor dropout(const Tensor& x, double p, const OptTensor& rng, int64_t stream) 
   require_dropout(x, p, rng, stream);
   if (wants_grad({&x})) return DropoutNode::apply(x, p, rng, stream);
   at::AutoDispatchBelowADInplaceOrView below;
-  return run_dropout(x.contiguous(), p, dense(rng), stream, nullptr);
+  return run_dropout(aligned16(x), p, dense(rng), stream, nullptr);
 }
 
 struct NormForward {
@@ -428,7 +428,7 @@ class RMSNormNode : public torch::autograd::Function<RMSNormNode> {
  public:
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, double eps) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor xc = x.contiguous(), w = weight.contiguous();
+    const Tensor xc = aligned16(x), w = aligned16(weight);
     NormForward f = run_norm(xc, Tensor(), w, eps, 0.0, Tensor(), 0);
     ctx->save_for_backward({xc, w, f.rstd});
     return f.out;
@@ -436,7 +436,7 @@ class RMSNormNode : public torch::autograd::Function<RMSNormNode> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     require_first_order("rms_norm");
     const auto saved = ctx->get_saved_variables();
-    auto g = run_norm_backward(grads[0].contiguous(), Tensor(), saved[0], saved[2], saved[1], 0.0, Tensor(), 0, false, ctx->needs_input_grad(0),
+    auto g = run_norm_backward(aligned16(grads[0]), Tensor(), saved[0], saved[2], saved[1], 0.0, Tensor(), 0, false, ctx->needs_input_grad(0),
                                ctx->needs_input_grad(1));
     return {g[1], g[2], Tensor()};
   }
@@ -447,8 +447,8 @@ class AddRMSNormNode : public torch::autograd::Function<AddRMSNormNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const Tensor& weight, double eps, double p,
                                const OptTensor& rng, int64_t stream) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor w = weight.contiguous();
-    NormForward f = run_norm(x.contiguous(), residual.contiguous(), w, eps, p, dense(rng), stream);
+    const Tensor w = aligned16(weight);
+    NormForward f = run_norm(aligned16(x), aligned16(residual), w, eps, p, dense(rng), stream);
     ctx->save_for_backward({f.h, w, f.rstd, f.used});
     ctx->saved_data["p"] = p;
     ctx->saved_data["stream"] = stream;
@@ -459,8 +459,8 @@ class AddRMSNormNode : public torch::autograd::Function<AddRMSNormNode> {
     require_first_order("add_rms_norm");
     const auto saved = ctx->get_saved_variables();
     const Tensor& h = saved[0];
-    const Tensor dout = grads[0].defined() ? grads[0].contiguous() : at::zeros_like(h);  // undefined: only h was used
-    const Tensor dh = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    const Tensor dout = grads[0].defined() ? aligned16(grads[0]) : at::zeros_like(h);  // undefined: only h was used
+    const Tensor dh = grads[1].defined() ? aligned16(grads[1]) : Tensor();
     auto g = run_norm_backward(dout, dh, h, saved[2], saved[1], ctx->saved_data["p"].toDouble(), saved[3], ctx->saved_data["stream"].toInt(),
                                ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2));
     return {g[0], g[1], g[2], Tensor(), Tensor(), Tensor(), Tensor()};
@@ -472,7 +472,7 @@ Tensor rms_norm(const Tensor& x, const Tensor& weight, double eps) {
   require_weight(weight, x);
   if (wants_grad({&x, &weight})) return RMSNormNode::apply(x, weight, eps);
   at::AutoDispatchBelowADInplaceOrView below;
-  return run_norm(x.contiguous(), Tensor(), weight.contiguous(), eps, 0.0, Tensor(), 0).out;
+  return run_norm(aligned16(x), Tensor(), aligned16(weight), eps, 0.0, Tensor(), 0).out;
 }
 
 std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps, double p,
@@ -486,7 +486,7 @@ std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& residual,
     return {r[0], r[1]};
   }
   at::AutoDispatchBelowADInplaceOrView below;
-  NormForward f = run_norm(x.contiguous(), residual.contiguous(), weight.contiguous(), eps, p, dense(rng), stream);
+  NormForward f = run_norm(aligned16(x), aligned16(residual), aligned16(weight), eps, p, dense(rng), stream);
   return {f.out, f.h};
 }
 
@@ -504,7 +504,7 @@ std::tuple<Tensor, Tensor, OptTensor> rows_e4m3(const Tensor& x_in, const OptTen
   }
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::cuda::CUDAGuard guard(x_in.device());
-  const Tensor x = x_in.contiguous(), residual = dense(residual_in), weight = dense(weight_in);
+  const Tensor x = aligned16(x_in), residual = dense(residual_in), weight = dense(weight_in);
   Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
   Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
   OptTensor h;
@@ -607,7 +607,7 @@ class CePiecesNode : public torch::autograd::Function<CePiecesNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& weight_in, const Tensor& target_in, int64_t ignore_index,
                         bool mean, int64_t piece, const Tensor& status) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor x = x_in.contiguous(), weight = weight_in.contiguous(), target = target_in.contiguous();
+    const Tensor x = aligned16(x_in), weight = aligned16(weight_in), target = target_in.contiguous();
     auto [loss, inv_count, lse] = run_ce(x, weight, target, ignore_index, mean, status);
     ctx->save_for_backward({x, weight, target, lse, inv_count});
     ctx->saved_data["ignore_index"] = ignore_index;
@@ -639,7 +639,7 @@ Tensor linear_cross_entropy_pieces(const Tensor& x, const Tensor& weight, const 
   TORCH_CHECK_VALUE(x.size(0) <= INT_MAX && weight.size(0) <= INT_MAX - 256, "extents must fit 31 bits");
   if (wants_grad({&x, &weight})) return CePiecesNode::apply(x, weight, target, ignore_index, mean, piece, status);
   at::AutoDispatchBelowADInplaceOrView below;
-  return std::get<0>(run_ce(x.contiguous(), weight.contiguous(), target.contiguous(), ignore_index, mean, status));
+  return std::get<0>(run_ce(aligned16(x), aligned16(weight), target.contiguous(), ignore_index, mean, status));
 }
 
 }  // namespace

@@ -40,9 +40,15 @@ def _ptr(t: Optional[Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _dense16(t: Optional[Tensor]) -> Optional[Tensor]:
+    """What the row kernels take: dense and 16-byte aligned (a view that starts elsewhere is copied)."""
+    return None if t is None else _aligned16(t)
+
+
 # ------------------------------------------------------------------------------------------------ custom ops
 @torch.library.custom_op("coda_b200::dropout_out", mutates_args=("out", "used"), device_types="cuda")
 def _dropout_out(x: Tensor, p: float, rng: Optional[Tensor], stream_id: int, out: Tensor, used: Tensor) -> None:
+    x = _dense16(x)
     cols = x.shape[-1]
     check(
         lib.coda_b200_dropout(x.data_ptr(), out.data_ptr(), x.numel() // cols, cols, _DTYPE_CODES[x.dtype], float(p), _ptr(rng), stream_id,
@@ -54,6 +60,7 @@ def _dropout_out(x: Tensor, p: float, rng: Optional[Tensor], stream_id: int, out
 @torch.library.custom_op("coda_b200::add_rmsnorm_out", mutates_args=("h", "out", "rstd", "used"), device_types="cuda")
 def _add_rmsnorm_out(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float, p: float, rng: Optional[Tensor], stream_id: int,
                      h: Optional[Tensor], out: Tensor, rstd: Tensor, used: Optional[Tensor]) -> None:
+    x, residual, weight = _dense16(x), _dense16(residual), _dense16(weight)
     cols = x.shape[-1]
     check(
         lib.coda_b200_add_rmsnorm_fwd(x.data_ptr(), _ptr(residual), weight.data_ptr(), float(eps), float(p), _ptr(rng), stream_id, _ptr(used),
@@ -65,6 +72,7 @@ def _add_rmsnorm_out(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps:
 @torch.library.custom_op("coda_b200::add_rmsnorm_bwd_out", mutates_args=("dx", "dres", "dweight"), device_types="cuda")
 def _add_rmsnorm_bwd_out(dout: Tensor, dh: Optional[Tensor], h: Tensor, rstd: Tensor, weight: Tensor, p: float, rng: Optional[Tensor],
                          stream_id: int, dx: Optional[Tensor], dres: Optional[Tensor], dweight: Optional[Tensor]) -> None:
+    dout, dh, h, weight = _dense16(dout), _dense16(dh), _dense16(h), _dense16(weight)
     cols = h.shape[-1]
     rows = h.numel() // cols
     scratch_bytes = int(lib.coda_b200_add_rmsnorm_bwd_scratch_bytes(rows, cols)) if dweight is not None else 0
@@ -80,6 +88,7 @@ def _add_rmsnorm_bwd_out(dout: Tensor, dh: Optional[Tensor], h: Tensor, rstd: Te
 @torch.library.custom_op("coda_b200::rows_e4m3_out", mutates_args=("h", "q", "scale"), device_types="cuda")
 def _rows_e4m3_out(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], eps: float, h: Optional[Tensor], q: Tensor,
                    scale: Tensor) -> None:
+    x, residual, weight = _dense16(x), _dense16(residual), _dense16(weight)
     cols = x.shape[-1]
     check(
         lib.coda_b200_rows_e4m3(x.data_ptr(), _ptr(residual), _ptr(weight), float(eps), _ptr(h), q.data_ptr(), scale.data_ptr(),

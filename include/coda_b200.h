@@ -351,8 +351,9 @@ int coda_b200_qknorm_rope_bwd_noalloc(const void* dq, int64_t ld_dq, const void*
 /* ---- around the fused linears (no counterpart in the reference) ----
  *
  * Row kernels: dense row-major [rows, cols] matrices (leading dimension cols) of
- * `dtype` 0 = bf16, 1 = fp16, 2 = fp32, any cols >= 1 and any alignment of the
- * element type; rows == 0 launches nothing and writes nothing.
+ * `dtype` 0 = bf16, 1 = fp16, 2 = fp32, any cols >= 1 (2^30 at most for the
+ * norms), 16-byte aligned; rows == 0 launches nothing and writes nothing.  They
+ * read whole 16-byte groups inside the matrices given, and write nothing outside.
  *
  * Dropout: element (r, c) stays if word c % 4 of Philox4x32-10 with key
  * `seed` and counter (r * ceil(cols / 4) + c / 4 [64 bits], step, stream_id) is at
