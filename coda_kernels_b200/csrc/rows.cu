@@ -90,7 +90,7 @@ __device__ __forceinline__ Chunk<T> load_some(const T* p, int lo, int hi) {
 }
 // The chunk at p as it is, neighbours' elements included; `left` = elements from p to the end of the matrix (a chunk that
 // reaches beyond it is read one by one).  mask_chunk takes the neighbours out, where the values are used: a load that is
-// masked at once is waited for at once, row by row in the warps at a row's ends (backward 16384 x 4095: 383 us that way, KTM us
+// masked at once is waited for at once, row by row in the warps at a row's ends (backward 16384 x 4095: 383 us that way, 223 us
 // so).
 template <bool kShift, typename T>
 __device__ __forceinline__ Chunk<T> load_chunk(const T* p, const Span<kShift>& s, long long left) {
@@ -155,6 +155,11 @@ struct Dropout {
   float scale;  // 1 / (1 - p)
 };
 
+// Both halves of a 32 x 32-bit product (written out: the 64-bit product of the language took 8 % longer here).
+__device__ __forceinline__ void mul_wide(uint32_t a, uint32_t b, uint32_t& hi, uint32_t& lo) {
+  asm("{\n\t.reg .b64 t;\n\tmul.wide.u32 t, %2, %3;\n\tmov.b64 {%1, %0}, t;\n\t}" : "=r"(hi), "=r"(lo) : "r"(a), "r"(b));
+}
+
 struct Mask {
   uint32_t k0, k1, lo, first, second;  // seed; round 1 of the words that do not depend on the block (see words)
   uint32_t threshold;
@@ -164,23 +169,23 @@ struct Mask {
     const unsigned long long seed = static_cast<unsigned long long>(__ldg(d.rng));
     k0 = static_cast<uint32_t>(seed);
     k1 = static_cast<uint32_t>(seed >> 32);
-    const unsigned long long p1 = static_cast<unsigned long long>(static_cast<uint32_t>(__ldg(d.rng + 1))) * 0xCD9E8D57u;
-    lo = static_cast<uint32_t>(p1);
-    first = static_cast<uint32_t>(p1 >> 32) ^ k0;
+    uint32_t hi;
+    mul_wide(static_cast<uint32_t>(__ldg(d.rng + 1)), 0xCD9E8D57u, hi, lo);
+    first = hi ^ k0;
     second = d.stream ^ k1;
   }
   // The words of kN blocks, in step: the key words advance once for all of them, which costs fewer instructions than a key
-  // schedule each and fewer registers than one that is kept (16384 x 14336 bf16: 266 us with it kept, KTD us so).
+  // schedule each and fewer registers than one that is kept (16384 x 4095 bf16: 137 us with it kept, 118 us so).
   template <int kN>
   __device__ __forceinline__ void words(const unsigned long long (&block)[kN], uint32_t* u) const {
     uint32_t c0[kN], c1[kN], c2[kN], c3[kN], a = k0, b = k1;
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
-      const unsigned long long p0 = static_cast<unsigned long long>(static_cast<uint32_t>(block[n])) * 0xD2511F53u;
+      uint32_t hi0;
+      mul_wide(static_cast<uint32_t>(block[n]), 0xD2511F53u, hi0, c3[n]);
       c0[n] = first ^ static_cast<uint32_t>(block[n] >> 32);
       c1[n] = lo;
-      c2[n] = static_cast<uint32_t>(p0 >> 32) ^ second;
-      c3[n] = static_cast<uint32_t>(p0);
+      c2[n] = hi0 ^ second;
     }
 #pragma unroll
     for (int i = 1; i < 10; ++i) {
@@ -188,12 +193,13 @@ struct Mask {
       b += 0xBB67AE85u;
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
-        const unsigned long long p0 = static_cast<unsigned long long>(c0[n]) * 0xD2511F53u;
-        const unsigned long long p1 = static_cast<unsigned long long>(c2[n]) * 0xCD9E8D57u;
-        c0[n] = static_cast<uint32_t>(p1 >> 32) ^ c1[n] ^ a;
-        c1[n] = static_cast<uint32_t>(p1);
-        c2[n] = static_cast<uint32_t>(p0 >> 32) ^ c3[n] ^ b;
-        c3[n] = static_cast<uint32_t>(p0);
+        uint32_t hi0, lo0, hi1, lo1;
+        mul_wide(c0[n], 0xD2511F53u, hi0, lo0);
+        mul_wide(c2[n], 0xCD9E8D57u, hi1, lo1);
+        c0[n] = hi1 ^ c1[n] ^ a;
+        c1[n] = lo1;
+        c2[n] = hi0 ^ c3[n] ^ b;
+        c3[n] = lo0;
       }
     }
 #pragma unroll
@@ -282,34 +288,37 @@ __device__ __forceinline__ void row_reduce(float& a, float& b, float* red, int& 
 }
 
 // ------------------------------------------------------------------ dropout alone
-// A stream of chunks of the whole matrix, kDropUnroll of them in flight a thread.  Bound by HBM without the generator, by
-// issue slots and registers with it (ten rounds are 40 instructions for 4 elements, 20 key words stay in registers): the
-// grid is what fits the SMs at once.
-constexpr int kDropThreads = 256, kDropUnroll = 2, kDropBlocksPerSm = 5;
+// A stream of chunks of the whole matrix, drop_unroll() of them in flight a thread, by four blocks an SM (eight: 158 instead of
+// 147 us for 16384 x 14336 bf16 without a mask; 32 bytes a thread suffice, a second fp32 chunk costs 52 instead of 43 us at 8192
+// x 4096).  Without the mask, and in fp32, bound by HBM (6.2 to 6.4 TB/s).  With it a 2-byte type is bound by the integer
+// multiplier, 19 wide products for 4 elements: 233 us, one element a nanosecond, whatever the occupancy.
+constexpr int kDropThreads = 256, kDropBlocksPerSm = 4;
+constexpr int drop_unroll(int elem_bytes) { return elem_bytes == 4 ? 1 : 2; }
 template <typename T, bool kShift, bool kDrop>
 __global__ void __launch_bounds__(kDropThreads, kDropBlocksPerSm)
 dropout_kernel(const T* __restrict__ x, T* __restrict__ out, long long total, long long cols, Dropout d, long long* __restrict__ used) {
+  constexpr int kUnroll = drop_unroll(sizeof(T));
   const MaskOf<kDrop> mask(d);
   note_used(d, used);
   const long long chunks = (total + 7) / 8, blocks = (cols + 3) / 4;
   const long long stride = static_cast<long long>(gridDim.x) * kDropThreads;
-  for (long long i0 = blockIdx.x * static_cast<long long>(kDropThreads) + threadIdx.x; i0 < chunks; i0 += stride * kDropUnroll) {
-    Chunk<T> in[kDropUnroll];
+  for (long long i0 = blockIdx.x * static_cast<long long>(kDropThreads) + threadIdx.x; i0 < chunks; i0 += stride * kUnroll) {
+    Chunk<T> in[kUnroll];
 #pragma unroll
-    for (int k = 0; k < kDropUnroll; ++k) {
+    for (int k = 0; k < kUnroll; ++k) {
       const long long e = 8 * (i0 + k * stride);
       if (e + 8 <= total) in[k] = load_whole(x + e);
       else in[k] = load_some(x + e, 0, e < total ? static_cast<int>(total - e) : 0);
     }
-    uint32_t all[kDropUnroll * 8];
+    uint32_t all[kUnroll * 8];
     if constexpr (kDrop && !kShift) {  // cols % 4 == 0: a row's blocks follow the previous row's
-      unsigned long long block[2 * kDropUnroll];
+      unsigned long long block[2 * kUnroll];
 #pragma unroll
-      for (int k = 0; k < 2 * kDropUnroll; ++k) block[k] = 2 * static_cast<unsigned long long>(i0 + k / 2 * stride) + (k & 1);
-      mask.template words<2 * kDropUnroll>(block, all);
+      for (int k = 0; k < 2 * kUnroll; ++k) block[k] = 2 * static_cast<unsigned long long>(i0 + k / 2 * stride) + (k & 1);
+      mask.template words<2 * kUnroll>(block, all);
     }
 #pragma unroll
-    for (int k = 0; k < kDropUnroll; ++k) {
+    for (int k = 0; k < kUnroll; ++k) {
       const long long e = 8 * (i0 + k * stride);
       if (e >= total) break;
       float v[8];
@@ -361,12 +370,13 @@ dropout_kernel(const T* __restrict__ x, T* __restrict__ out, long long total, lo
 // and written.  A thread stays on the same columns for all of its rows (kShift: the grid's row stride is a multiple of 8, so
 // `off` stays too), so the weights are loaded once.
 constexpr int kWarpBlock = 256, kMaxThreads = 512;
-// Registers a thread, and so threads an SM, of each kernel (kMaxThreads of 128 registers fill one): two chunks of a 2-byte type fit 64 in the forward; fp32 chunks
-// and the shift's masks take 80; four chunks a thread, and the backward with its sums and prefetch, take 128.  With the
-// shift the backward has 112: a row of 4095 columns needs one warp more than one of 4096, and two such blocks have to fit.
+// Registers a thread, and so threads an SM.  Forward: two chunks of a 2-byte type fit 64; fp32 chunks and the shift's masks
+// take 80, four chunks 128.  Backward: with sums and the next row's loads two chunks of a 2-byte type take 128 (16384 x
+// 4096 bf16: 96 us; 102 us with 80 registers and no loads ahead, 133 us with 96 registers and loads ahead); fp32, which loads
+// nothing ahead, takes 96 (16384 x 4096: 203 us, 128: 236 us), but 128 with dropout (8192 x 8192: 220 us, 96: 255 us).
 constexpr int fwd_regs(int elem_bytes, bool shift, int chunks) { return chunks == 4 ? 128 : (elem_bytes == 4 || shift) ? 80 : 64; }
-constexpr int bwd_regs(bool shift, int chunks) { return shift && chunks == 2 ? 112 : 128; }
-constexpr int threads_per_sm(int regs) { return 65536 / regs / 32 * 32; }
+constexpr int bwd_regs(int elem_bytes, bool shift, bool drop) { return shift ? 80 : elem_bytes == 4 && !drop ? 96 : 128; }
+constexpr int threads_per_sm(int regs) { return 512 / regs * 4 * 32; }  // whole warps in each quarter of the SM
 
 template <bool kWarp>
 struct RowLoop {
@@ -465,12 +475,12 @@ norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T
 // Bound by HBM, and laid out as the forward; dw is summed in registers over a thread's rows and leaves as one partial row a
 // block, which fold_rows_kernel adds in a fixed order.
 template <typename T, bool kShift, bool kDrop, bool kWarp, int kChunks>
-__global__ void __maxnreg__(bwd_regs(kShift, kChunks))
+__global__ void __maxnreg__(bwd_regs(sizeof(T), kShift, kDrop))
 norm_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* __restrict__ h, const float* __restrict__ rstd,
                 const T* __restrict__ weight, Dropout d, T* __restrict__ dx, T* __restrict__ dres, float* __restrict__ partial,
                 long long rows, int cols) {
-  // the next row's loads need as many registers again: affordable for two chunks of a 2-byte type
-  constexpr bool kPrefetch = sizeof(T) == 2 && kChunks <= 2;
+  // the next row's loads need as many registers again
+  constexpr bool kPrefetch = !kShift && sizeof(T) == 2;
   __shared__ float red[kWarp ? 1 : 128];
   __shared__ float fold[kWarp ? 256 : 1];
   int turn = 0;
@@ -571,9 +581,10 @@ norm_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* _
 }
 
 // ------------------------------------------------------------------ rows longer than registers hold
-// The same mathematics for rows of more than 4 * kMaxThreads chunks: one block a row, which reads its operands twice (the second
-// time mostly from L2) and keeps its dw sums in the partial row itself.
-constexpr int kColsLimit = 1 << 30;
+// The same mathematics for rows that do not fit the registers: one block a row, which reads its operands twice (the second
+// time mostly from L2: 4096 x 16384 bf16 backward 120 us; 165 us with four chunks a thread in registers, which spill).  The
+// backward keeps its dw sums in shared memory, or, for rows of more than kSharedCols columns, in the partial row itself.
+constexpr int kColsLimit = 1 << 30, kSharedCols = 51200;
 constexpr int kLongThreads = 1024;
 template <typename T, bool kShift, bool kDrop, bool kE4M3>
 __global__ void __launch_bounds__(kLongThreads)
@@ -645,8 +656,27 @@ norm_fwd_long_kernel(const T* __restrict__ x, const T* __restrict__ residual, co
   }
 }
 
+// sums[0 .. 8) += v, or = v for the block's first row
+template <bool kShift>
+__device__ __forceinline__ void add_sums(float* sums, const float* v, const Span<kShift>& s, bool first) {
+  if constexpr (!kShift) {  // 16-byte aligned
+    float4* p = reinterpret_cast<float4*>(sums);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    if (!first) {
+      a = p[0];
+      b = p[1];
+    }
+    p[0] = make_float4(a.x + v[0], a.y + v[1], a.z + v[2], a.w + v[3]);
+    p[1] = make_float4(b.x + v[4], b.y + v[5], b.z + v[6], b.w + v[7]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j >= s.lo && j < s.hi) sums[j] = first ? v[j] : sums[j] + v[j];
+  }
+}
+
 template <typename T, bool kShift, bool kDrop>
-__global__ void __launch_bounds__(kLongThreads)
+__global__ void __launch_bounds__(kLongThreads, 2)
 norm_bwd_long_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* __restrict__ h, const float* __restrict__ rstd,
                      const T* __restrict__ weight, Dropout d, T* __restrict__ dx, T* __restrict__ dres, float* __restrict__ partial,
                      long long rows, int cols) {
@@ -655,7 +685,8 @@ norm_bwd_long_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const
   const MaskOf<kDrop> mask(d);
   const int blocks = (cols + 3) / 4;
   const long long total = rows * cols;
-  float* mine = partial != nullptr ? partial + static_cast<long long>(blockIdx.x) * cols : nullptr;
+  extern __shared__ __align__(16) float shared_sums[];
+  float* out_row = partial != nullptr ? partial + static_cast<long long>(blockIdx.x) * cols : nullptr;
   bool first_row = true;
   for (RowLoop<false> at; at.row < rows; at.row += at.step, first_row = false) {
     const long long base = at.row * cols;
@@ -669,7 +700,7 @@ norm_bwd_long_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const
       mask_chunk(hh, s);
       w = kShift ? load_some(weight + s.c0, s.lo, s.hi) : load_chunk(weight + s.c0, s, 8);
     };
-    float dot = 0.f, unused = 0.f;
+    float dot = 0.f, unused = 0.f, v[8];
     Chunk<T> o, hh, w;
     // a column may pass from one thread to another between rows: row_reduce's synchronisation lies between the two
     for (int c = first; c < cols; c += 8 * kLongThreads) {
@@ -679,7 +710,11 @@ norm_bwd_long_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const
       for (int j = 0; j < 8; ++j) {
         const float t = chunk_get(o, j) * (chunk_get(hh, j) * r);
         dot = fmaf(t, chunk_get(w, j), dot);
-        if (mine != nullptr && j >= s.lo && j < s.hi) mine[c + j] = first_row ? t : mine[c + j] + t;
+        v[j] = t;
+      }
+      if (partial != nullptr) {
+        if (cols <= kSharedCols) add_sums(shared_sums + c, v, s, first_row);
+        else add_sums(out_row + c, v, s, first_row);
       }
     }
     row_reduce<false, false>(dot, unused, red, turn);
@@ -687,7 +722,6 @@ norm_bwd_long_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const
     for (int c = first; c < cols; c += 8 * kLongThreads) {
       const Span<kShift> s(c, cols);
       operands(s, o, hh, w);
-      float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = r * (chunk_get(o, j) * chunk_get(w, j) - chunk_get(hh, j) * r * m);
       if (dh != nullptr) {
@@ -702,6 +736,9 @@ norm_bwd_long_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const
       }
     }
   }
+  if (partial == nullptr || cols > kSharedCols) return;
+  __syncthreads();
+  for (int c = threadIdx.x; c < cols; c += kLongThreads) out_row[c] = shared_sums[c];
 }
 
 // Column sums of the partial rows, in a fixed order.
@@ -762,17 +799,23 @@ struct RowPlan {
   int chunks, threads;
   int64_t grid;
 };
-inline RowPlan row_plan(int64_t rows, int64_t cols, int dtype, bool backward) {
+inline RowPlan row_plan(int64_t rows, int64_t cols, int dtype, bool backward, bool drop) {
   RowPlan p;
   p.shift = cols % 8 != 0;
   const int64_t n = (cols + (p.shift ? 14 : 7)) / 8;  // chunks a row may touch
-  p.chunks = n <= 32 ? 1 : n <= 2 * kMaxThreads ? 2 : n <= 4 * kMaxThreads ? 4 : 0;
+  p.chunks = n <= 32 ? 1 : n <= 2 * kMaxThreads ? 2 : n <= 4 * kMaxThreads && !backward ? 4 : 0;
   p.threads = p.chunks == 1 ? kWarpBlock : p.chunks == 0 ? kLongThreads : static_cast<int>((n + 32 * p.chunks - 1) / (32 * p.chunks) * 32);
   const int64_t per_block = p.chunks == 1 ? kWarpBlock / 32 : 1, need = (rows + per_block - 1) / per_block;
-  const int fit = p.chunks == 0 ? 2 : threads_per_sm(backward ? bwd_regs(p.shift, p.chunks) : fwd_regs(dtype == 2 ? 4 : 2, p.shift, p.chunks)) / p.threads;
+  const int elem = dtype == 2 ? 4 : 2, regs = backward ? bwd_regs(elem, p.shift, drop) : fwd_regs(elem, p.shift, p.chunks);
+  const int fit = p.chunks == 0 ? (backward && cols > kSharedCols / 2 && cols <= kSharedCols ? 1 : 2) : threads_per_sm(regs) / p.threads;
   const int64_t cap = static_cast<int64_t>(sm_count()) * (fit < 1 ? 1 : fit > 32 ? 32 : fit) / 8 * 8;  // kShift: rows advance by multiples of 8
   p.grid = need < cap ? need : cap;
   return p;
+}
+// the widest backward grid of any type, with and without dropout
+inline int64_t most_partial_rows(int64_t rows, int64_t cols) {
+  const int64_t a = row_plan(rows, cols, 0, true, false).grid, b = row_plan(rows, cols, 2, true, false).grid;
+  return a > b ? a : b;
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -792,22 +835,24 @@ template <class F>
 int by_flag(bool flag, F&& f) {
   return flag ? f(std::true_type()) : f(std::false_type());
 }
-template <class F>
+template <bool kBackward, class F>
 int by_chunks(int chunks, F&& f) {
   if (chunks == 1) return f(std::integral_constant<int, 1>());
   if (chunks == 2) return f(std::integral_constant<int, 2>());
-  if (chunks == 4) return f(std::integral_constant<int, 4>());
+  if constexpr (!kBackward) {
+    if (chunks == 4) return f(std::integral_constant<int, 4>());
+  }
   return f(std::integral_constant<int, 0>());
 }
 
 template <bool kE4M3>
 int launch_norm_fwd(const void* x, const void* residual, const void* weight, float eps, const Dropout& d, int64_t* used, void* h, void* out,
                     float* rstd, void* q, float* scale, int64_t rows, int64_t cols, int dtype, void* stream) {
-  const RowPlan plan = row_plan(rows, cols, dtype, false);
+  const RowPlan plan = row_plan(rows, cols, dtype, false, d.rng != nullptr);
   return by_dtype(dtype, [&](auto t) {
     return by_flag(plan.shift, [&](auto shift) {
       return by_flag(!kE4M3 && d.rng != nullptr, [&](auto drop) {
-        return by_chunks(plan.chunks, [&](auto chunks) {
+        return by_chunks<false>(plan.chunks, [&](auto chunks) {
           using T = decltype(t);
           constexpr bool kShift = decltype(shift)::value, kDrop = !kE4M3 && decltype(drop)::value;
           constexpr int kChunks = decltype(chunks)::value;
@@ -839,7 +884,7 @@ extern "C" int coda_b200_dropout(const void* x, void* out, int64_t rows, int64_t
   if (!x || !out) return fail(kBadArgument, "NULL pointer");
   rc = check_aligned({x, out});
   if (rc != kOk) return rc;
-  const long long total = rows * cols, need = ((total + 7) / 8 + kDropThreads * kDropUnroll - 1) / (kDropThreads * kDropUnroll);
+  const long long total = rows * cols, per_block = 8LL * kDropThreads * drop_unroll(dtype == 2 ? 4 : 2), need = (total + per_block - 1) / per_block;
   const long long cap = static_cast<long long>(sm_count()) * kDropBlocksPerSm;
   const int grid = static_cast<int>(need < cap ? need : cap);
   return by_dtype(dtype, [&](auto t) {
@@ -883,7 +928,7 @@ extern "C" int coda_b200_rows_e4m3(const void* x, const void* residual, const vo
 }
 
 extern "C" int64_t coda_b200_add_rmsnorm_bwd_scratch_bytes(int64_t rows, int64_t cols) {
-  return rows <= 0 || cols <= 0 ? 0 : row_plan(rows, cols, 0, true).grid * cols * static_cast<int64_t>(sizeof(float));
+  return rows <= 0 || cols <= 0 ? 0 : most_partial_rows(rows, cols) * cols * static_cast<int64_t>(sizeof(float));
 }
 
 extern "C" int coda_b200_add_rmsnorm_bwd(const void* dout, const void* dh, const void* h, const float* rstd, const void* weight, double p,
@@ -898,23 +943,30 @@ extern "C" int coda_b200_add_rmsnorm_bwd(const void* dout, const void* dh, const
   if (!dout || !h || !rstd || !weight) return fail(kBadArgument, "NULL pointer");
   if (dweight != nullptr && (scratch == nullptr || scratch_bytes < coda_b200_add_rmsnorm_bwd_scratch_bytes(rows, cols)))
     return fail(kBadArgument, "the weight gradient needs coda_b200_add_rmsnorm_bwd_scratch_bytes of scratch");
-  rc = check_aligned({dout, dh, h, weight, dx, dres});
+  rc = check_aligned({dout, dh, h, weight, dx, dres, scratch});
   if (rc != kOk) return rc;
-  const RowPlan plan = row_plan(rows, cols, dtype, true);
+  const RowPlan plan = row_plan(rows, cols, dtype, true, d.rng != nullptr);
   const int n = static_cast<int>(cols);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     const int rc2 = by_flag(plan.shift, [&](auto shift) {
       return by_flag(d.rng != nullptr, [&](auto drop) {
-        return by_chunks(plan.chunks, [&](auto chunks) {
+        return by_chunks<true>(plan.chunks, [&](auto chunks) {
           constexpr bool kShift = decltype(shift)::value, kDrop = decltype(drop)::value;
           constexpr int kChunks = decltype(chunks)::value;
           auto kern = [] {
             if constexpr (kChunks == 0) return norm_bwd_long_kernel<T, kShift, kDrop>;
             else return norm_bwd_kernel<T, kShift, kDrop, kChunks == 1, kChunks>;
           }();
-          kern<<<static_cast<int>(plan.grid), plan.threads, 0, st>>>(
+          int shared = 0;
+          if (kChunks == 0 && dweight != nullptr && cols <= kSharedCols) {
+            shared = n * static_cast<int>(sizeof(float));
+            const cudaError_t e =
+                cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedCols * static_cast<int>(sizeof(float)));
+            if (e != cudaSuccess) return fail(kCudaError, std::string("cudaFuncSetAttribute(smem): ") + cudaGetErrorString(e));
+          }
+          kern<<<static_cast<int>(plan.grid), plan.threads, shared, st>>>(
               static_cast<const T*>(dout), static_cast<const T*>(dh), static_cast<const T*>(h), rstd, static_cast<const T*>(weight), d,
               static_cast<T*>(dx), static_cast<T*>(dres), dweight != nullptr ? static_cast<float*>(scratch) : nullptr, rows, n);
           return launch_check("add_rmsnorm backward launch");

@@ -158,7 +158,7 @@ def test_add_rms_norm(ck, dtype, rows, cols, p):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,cols", [(1, 8), (65, 513), (300, 4096), (4, 16384), (2, 40000)])
+@pytest.mark.parametrize("rows,cols", [(1, 8), (65, 513), (300, 4096), (4, 16384), (2, 40000), (2, 60001), (2000, 257), (3000, 250), (700, 8190), (1300, 4095)])
 def test_rms_norm(ck, dtype, rows, cols):
     check_norm(dtype, 0.0, *norm_case(ck, dtype, rows, cols, 0.0, residual=False))
 
