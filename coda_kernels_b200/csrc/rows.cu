@@ -155,8 +155,16 @@ struct Dropout {
   float scale;  // 1 / (1 - p)
 };
 
-// Both halves of a 32 x 32-bit product (written out: the 64-bit product of the language took 8 % longer here).
+// Both halves of a 32 x 32-bit product.  Written out as one instruction (kAsm) it makes the dropout kernel, four blocks at
+// once, 8 % faster; in the norm kernels, two at once, it cost registers (backward 16384 x 4096 bf16 142 instead of 123 us).
+template <bool kAsm>
 __device__ __forceinline__ void mul_wide(uint32_t a, uint32_t b, uint32_t& hi, uint32_t& lo) {
+  if constexpr (!kAsm) {
+    const unsigned long long t = static_cast<unsigned long long>(a) * b;
+    hi = static_cast<uint32_t>(t >> 32);
+    lo = static_cast<uint32_t>(t);
+    return;
+  }
   asm("{\n\t.reg .b64 t;\n\tmul.wide.u32 t, %2, %3;\n\tmov.b64 {%1, %0}, t;\n\t}" : "=r"(hi), "=r"(lo) : "r"(a), "r"(b));
 }
 
@@ -170,7 +178,7 @@ struct Mask {
     k0 = static_cast<uint32_t>(seed);
     k1 = static_cast<uint32_t>(seed >> 32);
     uint32_t hi;
-    mul_wide(static_cast<uint32_t>(__ldg(d.rng + 1)), 0xCD9E8D57u, hi, lo);
+    mul_wide<false>(static_cast<uint32_t>(__ldg(d.rng + 1)), 0xCD9E8D57u, hi, lo);
     first = hi ^ k0;
     second = d.stream ^ k1;
   }
@@ -182,7 +190,7 @@ struct Mask {
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       uint32_t hi0;
-      mul_wide(static_cast<uint32_t>(block[n]), 0xD2511F53u, hi0, c3[n]);
+      mul_wide<(kN > 3)>(static_cast<uint32_t>(block[n]), 0xD2511F53u, hi0, c3[n]);
       c0[n] = first ^ static_cast<uint32_t>(block[n] >> 32);
       c1[n] = lo;
       c2[n] = hi0 ^ second;
@@ -194,8 +202,8 @@ struct Mask {
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
         uint32_t hi0, lo0, hi1, lo1;
-        mul_wide(c0[n], 0xD2511F53u, hi0, lo0);
-        mul_wide(c2[n], 0xCD9E8D57u, hi1, lo1);
+        mul_wide<(kN > 3)>(c0[n], 0xD2511F53u, hi0, lo0);
+        mul_wide<(kN > 3)>(c2[n], 0xCD9E8D57u, hi1, lo1);
         c0[n] = hi1 ^ c1[n] ^ a;
         c1[n] = lo1;
         c2[n] = hi0 ^ c3[n] ^ b;
