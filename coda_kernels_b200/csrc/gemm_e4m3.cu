@@ -8,15 +8,16 @@ namespace {
 
 // ------------------------------------------------------------------ few rows
 // The product for a handful of rows of x is a stream of the weight through the SMs, bound by HBM: a tile of the GEMM core
-// would keep 16 to 48 CTA pairs busy and fill most of its A operand with zeros.  Here a block owns 16 weight rows and its
-// 8 warps share out the contraction in steps of 64, several steps in flight; the warps' sums are added in shared memory
-// in a fixed order.
+// would keep 16 to 48 CTA pairs busy and fill most of its A operand with zeros.  Here a block owns 16 * kBands weight rows
+// and its 8 warps share out the contraction in steps of 64; the warps' sums are added in shared memory in a fixed order.
 //
 // The product itself is mma.sync m16n8k32 with the weight rows as M and the rows of x as N (kTiles tiles of 8).  A thread
 // holds, for weight rows g and g + 8 (g = lane / 4), 16 consecutive bytes at 16 (lane % 4) of the step, and the same 16
 // bytes of row g of x.  The instruction wants bytes 4 t .. 4 t + 3 and 16 + 4 t .. of a 32-byte slice from thread t; a
 // contraction may be taken in any order, so each thread's four words simply serve as (low, high) of two such slices, the
 // same for both operands, and every load is one 16-byte access.
+//
+// Every block reads all of x, mostly from L2, so beyond 16 rows it takes two bands of weight rows (kBands).
 constexpr int kRowsWarps = 8;
 
 __device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -26,79 +27,115 @@ __device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int kTiles, typename OutT>
-__global__ void __launch_bounds__(kRowsWarps * 32)
+template <int kTiles, int kBands, int kUnroll, typename OutT>
+__global__ void __launch_bounds__(kRowsWarps * 32, kTiles == 1 ? 4 : 1)
 few_rows_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x_scale, const uint8_t* __restrict__ w,
                 const float* __restrict__ w_scale, OutT* __restrict__ out, long long ldd, int M, int N, int K) {
-  constexpr int kUnroll = kTiles <= 2 ? 4 : 2;
-  __shared__ float part[kRowsWarps][kTiles * 8][17];
+  constexpr int kCols = 16 * kBands;
+  __shared__ float part[kRowsWarps / 2][kTiles * 8][kCols + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.x * 16;
-  const bool ok0 = n0 + g < N, ok1 = n0 + g + 8 < N;
-  const uint8_t* w0 = w + static_cast<long long>(n0 + g) * K;
-  const uint8_t* w1 = w0 + 8LL * K;
+  const int n0 = blockIdx.x * kCols;
+  const uint8_t* wr = w + static_cast<long long>(n0 + g) * K;
   const uint8_t* xr = x + static_cast<long long>(g) * K;
-  float acc[kTiles][4];
+  float acc[kBands][kTiles][4];
 #pragma unroll
-  for (int i = 0; i < kTiles; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+  for (int r = 0; r < kBands; ++r)
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) acc[r][i][0] = acc[r][i][1] = acc[r][i][2] = acc[r][i][3] = 0.f;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   for (int k0 = warp * 64 + t * 16; k0 - t * 16 < K; k0 += kRowsWarps * 64 * kUnroll) {
-    uint4 a0[kUnroll], a1[kUnroll], b[kUnroll][kTiles];
+    uint4 a[kUnroll][2 * kBands], b[kUnroll][kTiles];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int k = k0 + u * kRowsWarps * 64;
       const bool in = k < K;  // K is a multiple of 16: a 16-byte piece is all in or all out
-      a0[u] = in && ok0 ? __ldcs(reinterpret_cast<const uint4*>(w0 + k)) : zero;
-      a1[u] = in && ok1 ? __ldcs(reinterpret_cast<const uint4*>(w1 + k)) : zero;
+#pragma unroll
+      for (int r = 0; r < 2 * kBands; ++r)
+        a[u][r] = in && n0 + g + 8 * r < N ? __ldcs(reinterpret_cast<const uint4*>(wr + 8LL * r * K + k)) : zero;
 #pragma unroll
       for (int i = 0; i < kTiles; ++i)
         b[u][i] = in && g + 8 * i < M ? __ldg(reinterpret_cast<const uint4*>(xr + 8LL * i * K + k)) : zero;
     }
+    // all loads before the first product: left alone the compiler keeps fewer in flight (one row, 6144 x 4096: 9.3 instead of
+    // 7.6 us); with four tiles it is the other way round (22 instead of 15 us)
+    if constexpr (kTiles <= 2) asm volatile("" ::: "memory");
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) {
-        mma_e4m3(acc[i], a0[u].x, a1[u].x, a0[u].y, a1[u].y, b[u][i].x, b[u][i].y);
-        mma_e4m3(acc[i], a0[u].z, a1[u].z, a0[u].w, a1[u].w, b[u][i].z, b[u][i].w);
-      }
-  }
+      for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-  for (int i = 0; i < kTiles; ++i) {  // accumulator: weight rows g, g + 8 x rows 2 t, 2 t + 1 of x
-    part[warp][8 * i + 2 * t][g] = acc[i][0];
-    part[warp][8 * i + 2 * t + 1][g] = acc[i][1];
-    part[warp][8 * i + 2 * t][g + 8] = acc[i][2];
-    part[warp][8 * i + 2 * t + 1][g + 8] = acc[i][3];
+        for (int r = 0; r < kBands; ++r) {
+          mma_e4m3(acc[r][i], a[u][2 * r].x, a[u][2 * r + 1].x, a[u][2 * r].y, a[u][2 * r + 1].y, b[u][i].x, b[u][i].y);
+          mma_e4m3(acc[r][i], a[u][2 * r].z, a[u][2 * r + 1].z, a[u][2 * r].w, a[u][2 * r + 1].w, b[u][i].z, b[u][i].w);
+        }
+  }
+  // accumulator: weight rows g, g + 8 x rows 2 t, 2 t + 1 of x.  The upper half of the warps hands its sums to the lower
+  // half until one is left.
+#pragma unroll
+  for (int half = kRowsWarps / 2; half > 0; half /= 2) {
+    if (warp >= half && warp < 2 * half) {
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+        for (int r = 0; r < kBands; ++r)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) part[warp - half][8 * i + 2 * t + (j & 1)][16 * r + g + 8 * (j >> 1)] = acc[r][i][j];
+    }
+    __syncthreads();
+    if (warp < half) {
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+        for (int r = 0; r < kBands; ++r)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[r][i][j] += part[warp][8 * i + 2 * t + (j & 1)][16 * r + g + 8 * (j >> 1)];
+    }
+    __syncthreads();
+  }
+  if (warp == 0) {
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+      for (int r = 0; r < kBands; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) part[0][8 * i + 2 * t + (j & 1)][16 * r + g + 8 * (j >> 1)] = acc[r][i][j];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < kTiles * 8 * 16; i += kRowsWarps * 32) {
-    const int m = i / 16, n = i % 16;
+  for (int i = threadIdx.x; i < kTiles * 8 * kCols; i += kRowsWarps * 32) {
+    const int m = i / kCols, n = i % kCols;
     if (m >= M || n0 + n >= N) continue;
-    float s = part[0][m][n];
-#pragma unroll
-    for (int j = 1; j < kRowsWarps; ++j) s += part[j][m][n];
-    s *= x_scale[m] * w_scale[n0 + n];
+    const float s = part[0][m][n] * (x_scale[m] * w_scale[n0 + n]);
     if constexpr (sizeof(OutT) == 4) out[m * ldd + n0 + n] = s;
     else out[m * ldd + n0 + n] = __float2bfloat16_rn(s);
   }
 }
 
-constexpr int kFewRows = 32;
+// Against the GEMM core's tiles, weights from HBM: 28672 x 4096 takes 25 us to 8 rows and 33 us to 16, where the tiles take 37 us
+// for any count to 128; 6144 x 4096 7.6 and 11 us, the tiles 19 us.  From 17 rows on the blocks' reads of x weigh as much as
+// the weight: 4096 x 4096 to 32 rows 12 us, the tiles 18 us; but 6144 x 4096, whose blocks no longer run at once, 22 us.
+inline bool few_rows(int M, int N) { return M <= 16 || (M <= 32 && (N + 31) / 32 <= sm_count()); }
 
-template <typename OutT>
-int run_few_rows(const void* A, const float* a_scale, const void* B, const float* b_scale, void* D, int64_t ldd, int M, int N, int K,
-                 cudaStream_t stream) {
-  auto kern = M <= 8 ? few_rows_kernel<1, OutT> : M <= 16 ? few_rows_kernel<2, OutT> : few_rows_kernel<4, OutT>;
-  kern<<<(N + 15) / 16, kRowsWarps * 32, 0, stream>>>(static_cast<const uint8_t*>(A), a_scale, static_cast<const uint8_t*>(B), b_scale,
-                                                       static_cast<OutT*>(D), ldd, M, N, K);
+template <int kTiles, int kBands, int kUnroll, typename OutT>
+int launch_few_rows(const void* A, const float* a_scale, const void* B, const float* b_scale, void* D, int64_t ldd, int M, int N, int K,
+                    cudaStream_t stream) {
+  few_rows_kernel<kTiles, kBands, kUnroll, OutT><<<(N + 16 * kBands - 1) / (16 * kBands), kRowsWarps * 32, 0, stream>>>(
+      static_cast<const uint8_t*>(A), a_scale, static_cast<const uint8_t*>(B), b_scale, static_cast<OutT*>(D), ldd, M, N, K);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(kCudaError, std::string("e4m3 few-rows launch failed: ") + cudaGetErrorString(e));
   return kOk;
+}
+template <typename OutT>
+int run_few_rows(const void* A, const float* a_scale, const void* B, const float* b_scale, void* D, int64_t ldd, int M, int N, int K,
+                 cudaStream_t stream) {
+  if (M <= 8) return launch_few_rows<1, 1, 4, OutT>(A, a_scale, B, b_scale, D, ldd, M, N, K, stream);
+  if (M <= 16) return launch_few_rows<2, 1, 4, OutT>(A, a_scale, B, b_scale, D, ldd, M, N, K, stream);
+  return launch_few_rows<4, 2, 1, OutT>(A, a_scale, B, b_scale, D, ldd, M, N, K, stream);
 }
 
 template <typename OutT>
 int run_scaled(const void* A, const float* a_scale, const void* B, const float* b_scale, void* D, int64_t ldd, int M, int N, int K,
                int* dev_status, cudaStream_t stream) {
-  if (M <= kFewRows) return run_few_rows<OutT>(A, a_scale, B, b_scale, D, ldd, M, N, K, stream);
+  if (few_rows(M, N)) return run_few_rows<OutT>(A, a_scale, B, b_scale, D, ldd, M, N, K, stream);
   using Epi = EpiScaled<OutT>;
   const LaunchOptions opt = launch_options();
   if (opt.cta_group != 2) return fail(kBadArgument, "the e4m3 GEMM is built for CTA pairs only (cta_group = 2)");

@@ -295,7 +295,7 @@ def test_e4m3_edges(ck):
 
 # ------------------------------------------------------------------------------------------------ e4m3 projection
 @pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("M,N,K", [(1, 8, 16), (1, 4096, 1024), (2, 136, 48), (7, 64, 4096), (8, 1000, 528), (9, 1000, 528), (16, 264, 2064), (17, 512, 512), (130, 264, 1552),
+@pytest.mark.parametrize("M,N,K", [(1, 8, 16), (1, 4096, 1024), (2, 136, 48), (7, 64, 4096), (8, 1000, 528), (9, 1000, 528), (16, 264, 2064), (17, 512, 512), (32, 72, 1040), (20, 8200, 64), (33, 72, 64), (130, 264, 1552),
                                    (256, 256, 256), (333, 2056, 784), (1000, 520, 128)])
 def test_linear_e4m3(ck, M, N, K, out_dtype):
     """e4m3 products are exact in fp32; accumulating K of them, 32 an instruction, is off by at most (K / 32 + 1) * 2^-22
