@@ -816,8 +816,8 @@ inline RowPlan row_plan(int64_t rows, int64_t cols, int dtype, bool backward, bo
   const int64_t per_block = p.chunks == 1 ? kWarpBlock / 32 : 1, need = (rows + per_block - 1) / per_block;
   const int elem = dtype == 2 ? 4 : 2, regs = backward ? bwd_regs(elem, p.shift, drop) : fwd_regs(elem, p.shift, p.chunks);
   const int fit = p.chunks == 0 ? (backward && cols > kSharedCols / 2 && cols <= kSharedCols ? 1 : 2) : threads_per_sm(regs) / p.threads;
-  const int64_t cap = static_cast<int64_t>(sm_count()) * (fit < 1 ? 1 : fit > 32 ? 32 : fit) / 8 * 8;  // kShift: rows advance by multiples of 8
-  p.grid = need < cap ? need : cap;
+  const int64_t cap = std::max(static_cast<int64_t>(sm_count()) * std::min(std::max(fit, 1), 32) / 8, int64_t{1}) * 8;  // kShift: rows advance by multiples of 8
+  p.grid = std::min(need, cap);
   return p;
 }
 // the widest backward grid of any type, with and without dropout

@@ -16,7 +16,7 @@ import torch
 from .._guards import autocast_custom_bwd, autocast_custom_fwd, input_guard
 from ..ops import _debug_check_targets, _fast, _require, lazy_status_check, status_word
 from ..ops_ce import ce_pieces_backward, ce_pieces_forward, default_piece
-from ..ops_rows import call_native
+from ..ops_rows import _require_first_order, call_native
 
 
 class LinearCrossEntropyPieces(torch.autograd.Function):
@@ -35,6 +35,7 @@ class LinearCrossEntropyPieces(torch.autograd.Function):
     @input_guard
     @autocast_custom_bwd
     def backward(ctx, dloss: torch.Tensor):
+        _require_first_order("linear_cross_entropy_pieces")
         x, weight, target, lse, inv_count = ctx.saved_tensors
         need_dx, need_dw = ctx.needs_input_grad[:2]
         return (*ce_pieces_backward(dloss, inv_count, lse, x, weight, target, ctx.ignore_index, ctx.piece, need_dx, need_dw),

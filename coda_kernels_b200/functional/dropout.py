@@ -14,7 +14,7 @@ from torch import Tensor
 
 from .._guards import autocast_custom_bwd, autocast_custom_fwd, input_guard
 from ..ops import _fast
-from ..ops_rows import _require_dropout, _require_rows, call_native, dropout_rows
+from ..ops_rows import _require_dropout, _require_first_order, _require_rows, call_native, dropout_rows
 
 
 class Dropout(torch.autograd.Function):
@@ -35,6 +35,7 @@ class Dropout(torch.autograd.Function):
     @input_guard
     @autocast_custom_bwd
     def backward(ctx, dout: Tensor):
+        _require_first_order("dropout")
         (used,) = ctx.saved_tensors
         return dropout_rows(dout, ctx.p, used, ctx.stream)[0], None, None, None
 

@@ -14,9 +14,10 @@ import torch
 from torch import Tensor
 
 from .._guards import autocast_custom_bwd, autocast_custom_fwd, input_guard
-from ..ops import _fast
+from ..ops import _fast, _require
 from ..ops_rows import (
     _require_dropout,
+    _require_first_order,
     _require_like,
     _require_no_grad,
     _require_rows,
@@ -45,6 +46,7 @@ class RMSNorm(torch.autograd.Function):
     @input_guard
     @autocast_custom_bwd
     def backward(ctx, dout: Tensor):
+        _require_first_order("rms_norm")
         x, weight, rstd = ctx.saved_tensors
         need_dx, need_dw = ctx.needs_input_grad[:2]
         _, dx, dw = add_rmsnorm_backward(dout, None, x, rstd, weight, 0.0, None, 0, False, need_dx, need_dw)
@@ -72,6 +74,7 @@ class AddRMSNorm(torch.autograd.Function):
     @input_guard
     @autocast_custom_bwd
     def backward(ctx, dout: Optional[Tensor], dh: Optional[Tensor]):
+        _require_first_order("add_rms_norm")
         h, weight, rstd, used = ctx.saved_tensors
         need_dx, need_dres, need_dw = ctx.needs_input_grad[:3]
         if dout is None:  # only h was used
@@ -117,12 +120,14 @@ def _rows_e4m3_composed(x: Tensor, residual: Optional[Tensor], weight: Optional[
 def rms_norm_e4m3(x: Tensor, weight: Tensor, eps: float) -> tuple[Tensor, Tensor]:
     """``(q, scale)``: the rows of ``rms_norm(x, weight, eps)`` as ``float8_e4m3fn`` values and one fp32 scale each
     (``q * scale[..., None]`` is the row), for :func:`linear_e4m3`.  Inference only."""
+    _require(weight is not None, "rms_norm_e4m3 needs a weight (quantize_e4m3 takes rows as they are)")
     q, scale, _ = _rows_e4m3(x, None, weight, eps)
     return q, scale
 
 
 def add_rms_norm_e4m3(x: Tensor, residual: Tensor, weight: Tensor, eps: float) -> tuple[Tensor, Tensor, Tensor]:
     """``(q, scale, h)``: :func:`add_rms_norm` without dropout, its first output in 8 bits.  Inference only."""
+    _require(residual is not None and weight is not None, "add_rms_norm_e4m3 needs a residual and a weight")
     return _rows_e4m3(x, residual, weight, eps)
 
 

@@ -139,6 +139,12 @@ def _require_dropout(x: Tensor, p: float, rng: Optional[Tensor], stream: int) ->
                  "rng must be an int64 tensor [seed, step] on x's device")
 
 
+def _require_first_order(name: str) -> None:
+    """Called by the backwards: autograd runs them with gradients enabled only to differentiate them in turn."""
+    if not torch.compiler.is_compiling() and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} can be differentiated once only")
+
+
 def _require_no_grad(name: str, *tensors: Optional[Tensor]) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no backward: call it under torch.no_grad() or on detached tensors")

@@ -216,3 +216,23 @@ def test_under_compile(ck):
     loss = torch.compile(f, fullgraph=True, dynamic=False)(x, w, t)
     dx, dw = torch.autograd.grad(loss, (x, w))
     check(x, w, t, loss, dx, dw, "mean")
+
+
+@pytest.mark.parametrize("option,value,default", [("epi_tma", 0, 1), ("cta_group", 1, 2), ("split_tail", 0, 1)])
+def test_library_options_leave_the_result(ck, option, value, default):
+    """Whatever the stores, the grouping and the schedule, the definition decides."""
+    x, w, t = make(300, 136, 1003)
+    ck.set_option(option, value)
+    try:
+        loss = ck.linear_cross_entropy_pieces(x, w, t, piece=300)
+        dx, dw = torch.autograd.grad(loss, (x, w))
+        torch.cuda.synchronize()
+    finally:
+        ck.set_option(option, default)
+    check(x, w, t, loss, dx, dw, "mean")
+
+
+def test_second_derivative_is_refused(ck):
+    x, w, t = make(20, 64, 300)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(ck.linear_cross_entropy_pieces(x, w, t), x, create_graph=True)

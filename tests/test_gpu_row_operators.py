@@ -494,3 +494,60 @@ def test_inference_mode_and_backward_accumulation(ck):
     out, h = ck.add_rms_norm(l1, l2, w, EPS)
     g1, g2 = torch.autograd.grad((out, h), (l1, l2), (torch.ones_like(out), torch.ones_like(h)))
     assert torch.equal(leaf.grad, g1 + g2)
+
+
+def test_norm_beyond_31_bits(ck):
+    """The last rows of a matrix of more than 2^31 elements come out as they do alone."""
+    cols = 4096
+    rows = 2**31 // cols + 6
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=DEV)
+    for i in range(0, rows, 65536):
+        x[i:i + 65536].normal_()
+    w = randn(cols, seed=2, std=0.2, mean=1.0)
+    tail = x[-9:].clone()
+    out, h = ck.add_rms_norm(x, x, w, EPS)
+    o, hh = ck.add_rms_norm(tail, tail, w, EPS)
+    assert torch.equal(out[-9:], o) and torch.equal(h[-9:], hh)
+    del out, h
+    q, s = ck.quantize_e4m3(x)
+    qq, ss = ck.quantize_e4m3(tail)
+    assert torch.equal(q[-9:].float(), qq.float()) and torch.equal(s[-9:], ss)
+    del q
+    leaf = x.requires_grad_(True)
+    (dx,) = torch.autograd.grad(ck.rms_norm(leaf, w, EPS), leaf, x.detach())
+    lt = tail.requires_grad_(True)
+    (dt,) = torch.autograd.grad(ck.rms_norm(lt, w, EPS), lt, tail.detach())
+    assert torch.equal(dx[-9:], dt)
+
+
+def test_e4m3_projection_stores_and_groupings(ck):
+    """Per-thread stores give what TMA stores give; one CTA a tile is refused, as it is not built."""
+    x8, xs = ck.quantize_e4m3(randn(100, 128))
+    w8, ws = ck.quantize_e4m3(randn(328, 128, seed=1))
+    for out_dtype in (torch.bfloat16, torch.float32):
+        base = ck.linear_e4m3(x8, xs, w8, ws, out_dtype)
+        for name, value, default in (("epi_tma", 0, 1), ("tile_n", 64, 0), ("tile_n", 256, 0)):
+            ck.set_option(name, value)
+            try:
+                assert torch.equal(base, ck.linear_e4m3(x8, xs, w8, ws, out_dtype))
+            finally:
+                ck.set_option(name, default)
+    ck.set_option("cta_group", 1)
+    try:
+        with pytest.raises(ck.CodaB200Error, match="CTA pairs"):
+            ck.linear_e4m3(x8, xs, w8, ws)
+    finally:
+        ck.set_option("cta_group", 2)
+
+
+def test_inference_operators_under_compile(ck):
+    def f(x, res, w, w8, ws):
+        q, s, h = ck.add_rms_norm_e4m3(x, res, w, EPS)
+        return ck.linear_e4m3(q, s, w8, ws), h, *ck.quantize_e4m3(h)
+
+    x, res, w = randn(20, 128), randn(20, 128, seed=1), randn(128, seed=2)
+    w8, ws = ck.quantize_e4m3(randn(72, 128, seed=3))
+    with torch.no_grad():
+        traced = torch.compile(f, fullgraph=True, dynamic=False)(x, res, w, w8, ws)
+        for a, b in zip(f(x, res, w, w8, ws), traced):
+            assert torch.equal(a.float(), b.float())
