@@ -82,7 +82,8 @@ SIGNATURES = {
     "coda_b200_add_rmsnorm_bwd_scratch_bytes": (_L, [_L, _L]),
     "coda_b200_add_rmsnorm_bwd": (_I, [_P, _P, _P, _P, _P, _D, _P, _L, _P, _P, _P, _P, _L, _L, _L, _I, _P]),
     "coda_b200_rows_e4m3": (_I, [_P, _P, _P, _F, _P, _P, _P, _L, _L, _I, _P]),
-    "coda_b200_gemm_e4m3": (_I, [_P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P, _P]),
+    "coda_b200_gemm_e4m3_workspace_bytes": (_L, [_I, _I, _I]),
+    "coda_b200_gemm_e4m3": (_I, [_P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P, _L, _P, _P]),
     "coda_b200_ce_loss": (_I, [_P, _L, _L, _P, _L, _L, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P]),
     "coda_b200_gemm_softmax_grad": (_I, [_P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _P, _L, _I, _I, _I, _P, _P]),
 }

@@ -511,6 +511,50 @@ struct EpiScaled {
   }
 };
 
+// The same product with the roles of the operands exchanged: the accumulator's rows are weight rows, its columns rows of x, and
+// D[col, row] = acc * row_scale[row] * col_scale[col].  A thread holds one column of D; the lanes of a warp hold 32 of them
+// side by side, so each store of the warp is one run of 32 elements.
+template <typename OutT>
+struct EpiScaledT {
+  static constexpr uint32_t kLoadRingBytes = 0;
+  static constexpr bool kSplitTail = true;
+  struct Params {
+    alignas(64) CUtensorMap tm_ws;  // tail-split workspace as [slabs * tile rows, kBN] fp32, box 32 x 32 (unused otherwise)
+    OutT* D;                        // [columns of the accumulator, rows of the accumulator]
+    long long ldd;
+    const float* row_scale;
+    const float* col_scale;
+    float* ws = nullptr;
+    long long ws_bytes = 0;
+  };
+
+  template <int kBN>
+  __device__ static void run(const Params& p, EpiCtx& c) {
+    if (c.part_row0 >= 0) {  // one part of a tail tile: the raw accumulator goes to its slab
+      for_chunks(c.taddr, kBN / 32, [&](int ch, float* v) {
+        const uint32_t tile = ring_acquire(c);
+        stage_row_f32(tile, c.lane, v);
+        ring_publish();
+        if (c.lane == 0) tma_store_2d(&p.tm_ws, tile, ch * 32, c.part_row0);
+        ring_commit(c);
+      });
+      return;
+    }
+    const bool row_ok = c.row < c.M;
+    const float rs = row_ok ? __ldg(p.row_scale + c.row) : 0.f;
+    for_chunks(c.taddr, valid_chunks<kBN>(c.n0, c.N), [&](int ch, float* v) {
+      const int col = c.n0 + ch * 32;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (row_ok && col + j < c.N) {
+          const float t = v[j] * (rs * __ldg(p.col_scale + col + j));
+          if constexpr (sizeof(OutT) == 4) p.D[(col + j) * p.ldd + c.row] = t;
+          else p.D[(col + j) * p.ldd + c.row] = __float2bfloat16_rn(t);
+        }
+    });
+  }
+};
+
 // ------------------------------------------------------------------ per-head RMSNorm + RoPE on q,k; plain store for v
 // Columns are [q heads | k heads | v heads], each head kHD wide.  For q and k:
 //   ms = mean(acc^2) over the head (fp32, unrounded acc), r = rsqrt(ms + eps)

@@ -235,6 +235,18 @@ __global__ void __launch_bounds__(256) split_finalize_kernel(const float* __rest
   }
 }
 
+// The follow-up launch of a split launch, by epilogue.
+template <class Epi>
+struct SplitFinalize;
+template <typename OutT, Act kAct>
+struct SplitFinalize<EpiStore<OutT, kAct>> {
+  static void launch(const typename EpiStore<OutT, kAct>::Params& ep, const GemmShape& shape, int first_tail_tile, int tile_m, int bn,
+                     cudaStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(shape.sk_tail), static_cast<unsigned>(tile_m / kFinalizeRows), 1);
+    split_finalize_kernel<<<grid, 256, 0, stream>>>(ep.ws, ep.D, ep.ldd, shape, first_tail_tile, tile_m, bn, ep.alpha);
+  }
+};
+
 // With a prologue policy (`Pro`, see gemm_core.cuh) `a_ptr` is the raw matrix that TMA loads into the A slot and the
 // transform warps rewrite in place; `pp` carries what else they need.
 template <int kCtaGroup, int kBN, bool kAMn, bool kBMn, class Epi, class Pro = ProNone>
@@ -272,7 +284,7 @@ int launch_gemm_cfg(const void* a_ptr, long long lda, const void* b_ptr, long lo
   shape.sk_tail = 0;
   shape.sk_split = 1;
   typename Epi::Params ep_sk = ep;  // what the kernel receives (gains the workspace map if the tail is split)
-  if constexpr (has_split_tail<Epi>::value && std::is_same<Pro, ProNone>::value) {
+  if constexpr (has_split_tail<Epi>::value && Pro::kWarps == 0) {
     const int all = full_clusters(opt, kCtaGroup);
     if (opt.split_tail != 0 && ep.ws != nullptr && ep.ws_bytes >= split_workspace_bytes(all, tile_m, kBN)) {
       shape.sk_split = plan_tail_split(num_tiles, num_kb, all, &shape.sk_tail);
@@ -320,11 +332,9 @@ int launch_gemm_cfg(const void* a_ptr, long long lda, const void* b_ptr, long lo
   }
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tb, shape, ep_sk, status, pp);
   if (e != cudaSuccess) return fail(kCudaError, std::string("GEMM launch failed: ") + cudaGetErrorString(e));
-  if constexpr (has_split_tail<Epi>::value && std::is_same<Pro, ProNone>::value) {
+  if constexpr (has_split_tail<Epi>::value && Pro::kWarps == 0) {
     if (shape.sk_split > 1) {
-      const dim3 grid(static_cast<unsigned>(shape.sk_tail), static_cast<unsigned>(tile_m / kFinalizeRows), 1);
-      split_finalize_kernel<<<grid, 256, 0, stream>>>(ep.ws, ep.D, ep.ldd, shape, static_cast<int>(num_tiles) - shape.sk_tail, tile_m, kBN,
-                                                       ep.alpha);
+      SplitFinalize<Epi>::launch(ep, shape, static_cast<int>(num_tiles) - shape.sk_tail, tile_m, kBN, stream);
       e = cudaGetLastError();
       if (e != cudaSuccess) return fail(kCudaError, std::string("tail-split follow-up launch failed: ") + cudaGetErrorString(e));
     }

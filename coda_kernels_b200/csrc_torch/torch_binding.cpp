@@ -539,8 +539,12 @@ Tensor linear_e4m3(const Tensor& x_in, const Tensor& x_scale, const Tensor& weig
   const Tensor x = aligned16(x_in), xs = x_scale.contiguous(), weight = aligned16(weight_in), ws = aligned16(weight_scale);
   Tensor out = new_matrix(x, M, N, out_fp32 ? at::kFloat : at::kBFloat16);
   if (M == 0) return out;
+  const int64_t parts_bytes = coda_b200_gemm_e4m3_workspace_bytes(static_cast<int>(M), static_cast<int>(N), static_cast<int>(K));
+  Tensor parts;
+  if (parts_bytes > 0) parts = at::empty({parts_bytes / 4}, x.options().dtype(at::kFloat));
   check(coda_b200_gemm_e4m3(x.data_ptr(), xs.data_ptr<float>(), weight.data_ptr(), ws.data_ptr<float>(), out.data_ptr(), N, out_fp32,
-                            static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), status_ptr(status), stream_of(x)),
+                            static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), ptr_or_null(parts), parts_bytes, status_ptr(status),
+                            stream_of(x)),
         "gemm_e4m3");
   return out;
 }

@@ -101,9 +101,11 @@ def _rows_e4m3_out(x: Tensor, residual: Optional[Tensor], weight: Optional[Tenso
 def _gemm_e4m3_out(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor, out: Tensor) -> None:
     M, K = x.shape
     N = weight.shape[0]
+    ws_bytes = int(lib.coda_b200_gemm_e4m3_workspace_bytes(M, N, K))
+    ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device) if ws_bytes > 0 else None
     check(
         lib.coda_b200_gemm_e4m3(x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(), out.data_ptr(), N,
-                                int(out.dtype == torch.float32), M, N, K, status_word(x.device).data_ptr(), _stream(x)),
+                                int(out.dtype == torch.float32), M, N, K, _ptr(ws), ws_bytes, status_word(x.device).data_ptr(), _stream(x)),
         "gemm_e4m3",
     )
 

@@ -390,9 +390,13 @@ int coda_b200_rows_e4m3(const void* x, const void* residual, const void* weight,
 
 /* D[m, n] = a_scale[m] * b_scale[n] * sum_k A[m, k] * B[n, k] for dense row-major e4m3 A [M, K] and B [N, K], fp32
  * accumulation; D is bf16 or fp32 with leading dimension ldd.  K a multiple of 16, N and ldd multiples of 8; A, B, D and
- * b_scale 16-byte aligned. */
+ * b_scale 16-byte aligned.  `workspace` (16-byte aligned, may be NULL) of coda_b200_gemm_e4m3_workspace_bytes lets the
+ * contraction of a product with few tiles be cut into parts; its contents need not be kept or cleared.  The sums are
+ * added in a fixed order either way. */
+int64_t coda_b200_gemm_e4m3_workspace_bytes(int M, int N, int K);
 int coda_b200_gemm_e4m3(const void* A, const float* a_scale, const void* B, const float* b_scale, void* D, int64_t ldd,
-                        int d_is_fp32, int M, int N, int K, int* dev_status, void* stream);
+                        int d_is_fp32, int M, int N, int K, void* workspace, int64_t workspace_bytes, int* dev_status,
+                        void* stream);
 
 /* Cross entropy of the logits A @ B over all N columns (any N), storing none of them: lse fp32 [M], losses fp32 [M] (zero
  * in ignored rows, NaN for a label outside [0, N)), and the scalars loss = inv_count * sum(losses) and inv_count

@@ -295,7 +295,7 @@ def test_e4m3_edges(ck):
 
 # ------------------------------------------------------------------------------------------------ e4m3 projection
 @pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("M,N,K", [(1, 8, 16), (1, 4096, 1024), (2, 136, 48), (7, 64, 4096), (8, 1000, 528), (9, 1000, 528), (16, 264, 2064), (17, 512, 512), (32, 72, 1040), (20, 8200, 64), (33, 72, 64), (130, 264, 1552),
+@pytest.mark.parametrize("M,N,K", [(1, 8, 16), (1, 4096, 1024), (2, 136, 48), (7, 64, 4096), (8, 1000, 528), (9, 1000, 528), (16, 264, 2064), (17, 512, 512), (32, 72, 1040), (20, 8200, 64), (33, 72, 64), (64, 520, 4096), (40, 6144, 2048), (65, 1032, 8208), (100, 24, 1040), (128, 20000, 512), (129, 512, 2048), (130, 264, 1552),
                                    (256, 256, 256), (333, 2056, 784), (1000, 520, 128)])
 def test_linear_e4m3(ck, M, N, K, out_dtype):
     """e4m3 products are exact in fp32; accumulating K of them, 32 an instruction, is off by at most (K / 32 + 1) * 2^-22
@@ -522,7 +522,7 @@ def test_norm_beyond_31_bits(ck):
 
 def test_e4m3_projection_stores_and_groupings(ck):
     """Per-thread stores give what TMA stores give; one CTA a tile is refused, as it is not built."""
-    x8, xs = ck.quantize_e4m3(randn(100, 128))
+    x8, xs = ck.quantize_e4m3(randn(200, 128))
     w8, ws = ck.quantize_e4m3(randn(328, 128, seed=1))
     for out_dtype in (torch.bfloat16, torch.float32):
         base = ck.linear_e4m3(x8, xs, w8, ws, out_dtype)

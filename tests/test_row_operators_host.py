@@ -41,10 +41,12 @@ def test_c_entries_refuse_on_the_host():
     need = lib.coda_b200_add_rmsnorm_bwd_scratch_bytes(1000, 64)
     assert need > 0 and lib.coda_b200_add_rmsnorm_bwd_scratch_bytes(0, 64) == 0
     refused(lib.coda_b200_add_rmsnorm_bwd(p, p, p, p, p, 0.0, None, 0, p, p, p, p, need - 4, 1000, 64, 0, None), b"scratch")
-    refused(lib.coda_b200_gemm_e4m3(p, p, p, p, p, 16, 0, 4, 16, 40, p, None), b"multiple of 16")
-    refused(lib.coda_b200_gemm_e4m3(p, p, p, p, p, 12, 0, 4, 12, 32, p, None), b"multiples of 8")
-    refused(lib.coda_b200_gemm_e4m3(p + 8, p, p, p, p, 16, 0, 4, 16, 32, p, None), b"16-byte")
-    refused(lib.coda_b200_gemm_e4m3(p, p, p, p, p, 16, 0, 0, 16, 32, p, None), b"positive")
+    refused(lib.coda_b200_gemm_e4m3(p, p, p, p, p, 16, 0, 4, 16, 40, None, 0, p, None), b"multiple of 16")
+    refused(lib.coda_b200_gemm_e4m3(p, p, p, p, p, 12, 0, 4, 12, 32, None, 0, p, None), b"multiples of 8")
+    refused(lib.coda_b200_gemm_e4m3(p + 8, p, p, p, p, 16, 0, 4, 16, 32, None, 0, p, None), b"16-byte")
+    refused(lib.coda_b200_gemm_e4m3(p, p, p, p, p, 16, 0, 0, 16, 32, None, 0, p, None), b"positive")
+    refused(lib.coda_b200_gemm_e4m3(p, p, p, p, p, 16, 0, 4, 16, 32, p + 4, 64, p, None), b"16-byte")
+    assert lib.coda_b200_gemm_e4m3_workspace_bytes(100, 6144, 4096) > 0 == lib.coda_b200_gemm_e4m3_workspace_bytes(1, 6144, 4096)
     refused(lib.coda_b200_gemm_softmax_grad(p, 64, 1, p, 1, 64, p, p, -100, 0, p, 12, 4, 12, 64, p, None), b"ldg")
     refused(lib.coda_b200_gemm_softmax_grad(p, 64, 1, p, 1, 64, p, p, -100, -1, p, 16, 4, 12, 64, p, None), b"col0")
     refused(lib.coda_b200_ce_loss(p, 60, 1, p, 1, 60, p, -100, 1, p, p, p, p, p, p, p, 4, 12, 60, p, None), b"K must")
