@@ -128,14 +128,36 @@ __device__ __forceinline__ void store_chunk(T* p, const float* v, const Span<kSh
   }
 }
 
-// v * inv as e4m3.  inv is the row's 1 / scale: a division for every element made this kernel slower than its memory traffic
-// (8192 x 5120 bf16: 125 us a pass with, 72 us without); the product's extra rounding of 2^-24 moves a value only where it lies
-// that near to the middle of two e4m3 values.  Saturation turns 448 (1 + 2^-23) into 448.
+// max that keeps NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// The scale of a row of e4m3 values, and what divides by it.  The quotient has to be the correctly rounded one: values of
+// a 2-byte type lie exactly between two e4m3 values all the time (with max|y| = 21 / 8, say, where y / scale = 512 y / 3),
+// and a quotient one step off moves them all to the same side.  A division for every element made the kernel slower than its
+// memory traffic, though.  So: with inv = 1 / s rounded correctly and q = v inv, the residual v - q s is exact in an fma, and
+// q + residual * inv is v / s rounded correctly (Markstein, "Computation of elementary functions on the IBM RISC System/6000
+// processor", 1990; quantize 16384 x 4096 bf16: 44 us, 41 us with q alone).  Where the residual falls below the smallest fp32,
+// |v| < 2^-100, the last bit may be lost.
+struct RowScale {
+  float scale, inv, s;  // s: the scale, or 0 if that is infinite, so that finite values over it come out as 0
+  __device__ explicit RowScale(float top)
+      : scale(max_nan(top * (1.0f / 448.0f), 1.17549435e-38f)), inv(1.0f / scale), s(isinf(scale) ? 0.0f : scale) {}
+  __device__ float over(float v) const {
+    const float q = v * inv;
+    return fmaf(fmaf(-q, s, v), inv, q);
+  }
+};
+
+// Values over their row's scale as e4m3, rounded once more; saturation keeps 448 (1 + 2^-23) at 448.
 template <bool kShift>
-__device__ __forceinline__ void store_e4m3(__nv_fp8_e4m3* p, const float* v, float inv, const Span<kShift>& s) {
+__device__ __forceinline__ void store_e4m3(__nv_fp8_e4m3* p, const float* v, const RowScale& by, const Span<kShift>& s) {
   uint32_t e[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) e[j] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * j] * inv, v[2 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+  for (int j = 0; j < 4; ++j) e[j] = __nv_cvt_float2_to_fp8x2(make_float2(by.over(v[2 * j]), by.over(v[2 * j + 1])), __NV_SATFINITE, __NV_E4M3);
   if (s.whole()) {
     *reinterpret_cast<uint2*>(p) = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
   } else if constexpr (kShift) {
@@ -261,12 +283,6 @@ __device__ __forceinline__ void note_used(const Dropout& d, long long* used) {
   if (used != nullptr && blockIdx.x == 0 && threadIdx.x < 2) used[threadIdx.x] = d.rng != nullptr ? d.rng[threadIdx.x] : 0;
 }
 
-// max that keeps NaN
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 // (sum of a, max of b >= 0) over the threads of a row: a warp (kWarp), or the whole block of at most 32 warps.  `red` is
 // two buffers of 64 floats used in turn, `turn` counts the calls: a buffer is written again only after the synchronisation
 // of the call in between, so one is enough.
@@ -371,7 +387,7 @@ dropout_kernel(const T* __restrict__ x, T* __restrict__ out, long long total, lo
 // ------------------------------------------------------------------ residual + dropout(x), RMS norm
 // h = residual + dropout(x) (x alone without a residual); rstd = rsqrt(mean(h^2) + eps), taken of the unrounded h; out =
 // h * rstd * w.  kE4M3: out leaves as e4m3 values q with scale = max(max|out| / 448, 2^-126), q = out / scale rounded
-// once; without a weight the rows are converted as they are.
+// to e4m3; without a weight the rows are converted as they are.
 //
 // Bound by HBM: every tensor is read or written once.  The block (kWarp: a warp) owns a row and keeps its h in registers,
 // kChunks chunks a thread; the grid is what fits the SMs at once, and a row's successor is loaded while the row is reduced
@@ -457,9 +473,9 @@ norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T
     }
     row_reduce<kWarp, kE4M3>(sq, top, red, turn);
     const float r = weight != nullptr ? rsqrtf(sq / static_cast<float>(cols) + eps) : 1.0f;
-    const float s8 = max_nan(top * r / 448.0f, 1.17549435e-38f), inv = 1.0f / s8;
+    const RowScale by(top * r);
     if (at.tid == 0) {
-      if (kE4M3) scale[at.row] = s8;
+      if (kE4M3) scale[at.row] = by.scale;
       else rstd[at.row] = r;
     }
 #pragma unroll
@@ -469,7 +485,7 @@ norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[k][j] = v[k][j] * r * chunk_get(w[k], j);
       }
-      if constexpr (kE4M3) store_e4m3(q + base + s.c0, v[k], inv, s);
+      if constexpr (kE4M3) store_e4m3(q + base + s.c0, v[k], by, s);
       else store_chunk(out + base + s.c0, v[k], s);
     }
   }
@@ -645,9 +661,9 @@ norm_fwd_long_kernel(const T* __restrict__ x, const T* __restrict__ residual, co
     }
     row_reduce<false, kE4M3>(sq, top, red, turn);
     const float r = weight != nullptr ? rsqrtf(sq / static_cast<float>(cols) + eps) : 1.0f;
-    const float s8 = max_nan(top * r / 448.0f, 1.17549435e-38f), inv = 1.0f / s8;
+    const RowScale by(top * r);
     if (at.tid == 0) {
-      if (kE4M3) scale[at.row] = s8;
+      if (kE4M3) scale[at.row] = by.scale;
       else rstd[at.row] = r;
     }
     for (int c = first; c < cols; c += 8 * kLongThreads) {
@@ -658,7 +674,7 @@ norm_fwd_long_kernel(const T* __restrict__ x, const T* __restrict__ residual, co
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = v[j] * r * chunk_get(w, j);
       }
-      if constexpr (kE4M3) store_e4m3(q + base + c, v, inv, s);
+      if constexpr (kE4M3) store_e4m3(q + base + c, v, by, s);
       else store_chunk(out + base + c, v, s);
     }
   }

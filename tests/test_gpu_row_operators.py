@@ -272,6 +272,19 @@ def test_rows_in_e4m3(ck, dtype, rows, cols):
     check_e4m3(*ck.quantize_e4m3(x), x.double())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_e4m3_ties_follow_the_rounded_quotient(ck, dtype):
+    """Values of a 2-byte type lie on the middle between two e4m3 values all the time; they go to the even one, as the
+    correctly rounded fp32 quotient does."""
+    for i, top in enumerate((3.5, 2.625, 21.0, 1.0, 0.7, 5.25, 448.0, 1.3125 * 2.0**-20)):
+        x = (randn(64, 2048, dtype=torch.float32, seed=i).clamp(-3.9, 3.9) / 4 * top).to(dtype)
+        x[:, 5] = top
+        q, scale = ck.quantize_e4m3(x)
+        assert bool((scale == scale[0]).all())
+        want = (x.float() / scale[:, None]).to(torch.float8_e4m3fn)
+        assert torch.equal(q.float(), want.float()), top  # (a zero's sign is no value)
+
+
 def test_e4m3_edges(ck):
     x = randn(8, 96, dtype=torch.float32)
     x[1] = 0.0
