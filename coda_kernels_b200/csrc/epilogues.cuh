@@ -477,7 +477,7 @@ struct EpiScaled {
     OutT* D;
     long long ldd;
     const float* row_scale;  // [M]
-    const float* col_scale;  // [N], 16-byte aligned
+    const float* col_scale;  // [N]
     int use_tma;
   };
 
@@ -486,18 +486,16 @@ struct EpiScaled {
     const bool row_ok = c.row < c.M;
     const float rs = row_ok ? __ldg(p.row_scale + c.row) : 0.f;
     OutT* drow = p.D + static_cast<long long>(c.row) * p.ldd + c.n0;
+    // A lane holds the scale of one column of the chunk and hands it round; the next chunk's is on its way meanwhile (each
+    // chunk loading its own 32 scales cost a trip to L2 a chunk, 333 x 2056 x 1552: 3.2 of 12 us).
+    auto scale_of = [&](int ch) { return c.n0 + ch * 32 + c.lane < c.N ? __ldg(p.col_scale + c.n0 + ch * 32 + c.lane) : 0.f; };
+    float next = scale_of(0);
     for_chunks(c.taddr, valid_chunks<kBN>(c.n0, c.N), [&](int ch, float* v) {
       const int col = c.n0 + ch * 32;
+      const float mine = next;
+      next = scale_of(ch + 1);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (col + 4 * j < c.N) {  // N is a multiple of 8: a group of 4 is all in or all out
-          const float4 s = __ldg(reinterpret_cast<const float4*>(p.col_scale + col) + j);
-          v[4 * j] *= rs * s.x;
-          v[4 * j + 1] *= rs * s.y;
-          v[4 * j + 2] *= rs * s.z;
-          v[4 * j + 3] *= rs * s.w;
-        }
-      }
+      for (int j = 0; j < 32; ++j) v[j] *= rs * __shfl_sync(0xffffffffu, mine, j);
       if (p.use_tma) {
         const uint32_t tile = ring_acquire(c);
         stage_row(tile, c.lane, v, static_cast<OutT*>(nullptr));
@@ -542,15 +540,20 @@ struct EpiScaledT {
     }
     const bool row_ok = c.row < c.M;
     const float rs = row_ok ? __ldg(p.row_scale + c.row) : 0.f;
+    auto scale_of = [&](int ch) { return c.n0 + ch * 32 + c.lane < c.N ? __ldg(p.col_scale + c.n0 + ch * 32 + c.lane) : 0.f; };
+    float next = scale_of(0);
     for_chunks(c.taddr, valid_chunks<kBN>(c.n0, c.N), [&](int ch, float* v) {
       const int col = c.n0 + ch * 32;
+      const float mine = next;
+      next = scale_of(ch + 1);
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
+      for (int j = 0; j < 32; ++j) {
+        const float t = v[j] * (rs * __shfl_sync(0xffffffffu, mine, j));
         if (row_ok && col + j < c.N) {
-          const float t = v[j] * (rs * __ldg(p.col_scale + col + j));
           if constexpr (sizeof(OutT) == 4) p.D[(col + j) * p.ldd + c.row] = t;
           else p.D[(col + j) * p.ldd + c.row] = __float2bfloat16_rn(t);
         }
+      }
     });
   }
 };

@@ -100,8 +100,8 @@ few_rows_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x_scale
 }
 
 // Against the swapped tiles below, weights from HBM: to 8 rows 6144 x 4096 takes 7.6 us, 28672 x 4096 25 us and 4096 x 14336
-// 17 us (tiles, 17 rows: 14, 29 and 21 us); to 16 rows 11, 33 and 17 us.  Beyond, the blocks' reads of x weigh as much as the
-// weight (32 rows: 15, 51 and 34 us in the best form tried).
+// 17 us (swapped tiles, 17 rows: 14.5, 29 and 21 us); to 16 rows 11, 33 and 17 us.  Beyond, the blocks' reads of x weigh as much
+// as the weight (32 rows: 15, 51 and 34 us in the best form tried).
 constexpr int kFewRows = 16;
 
 template <typename OutT>
@@ -118,9 +118,11 @@ int run_few_rows(const void* A, const float* a_scale, const void* B, const float
 // ------------------------------------------------------------------ up to kSwapRows rows
 // With so few rows of x the GEMM core's 256-row tile would load mostly padding, and there would be too few column tiles for
 // the SMs.  So the weight takes the rows' place (256 of them a tile, whole) and x the columns', in the narrowest tile that
-// holds it; the tiles of the last round, which here is often the only one, are cut along K.  Weights from HBM, 32, 64 and 128
-// rows: 6144 x 4096 14.5, 15.5 and 19.3 us (not swapped 18.8), 28672 x 4096 29, 32 and 36 us (37), 4096 x 14336 21, 22 and 26 us (42).
+// holds it; the tiles of the last round, which here is often the only one, are cut along K.  Weights from HBM, 32 and 64 rows:
+// 6144 x 4096 14.6 and 15.4 us (not swapped 17.8), 28672 x 4096 29 and 30 us (35), 4096 x 14336 21 and 22 us (39).  To 128 rows the
+// parts cost as much as they save unless the contraction is long: 4096 x 4096 18.5 us (16.1), 4096 x 14336 26 us (39).
 constexpr int kSwapRows = 128;
+inline bool swapped(int M, int K) { return M > kFewRows && (M <= 64 || (M <= kSwapRows && K >= 8192)); }
 
 // Adds the parts of the cut tiles in order, scales them, and writes the transposed tile: block (t, b) has 32 accumulator rows
 // of tail tile t, which it turns through shared memory.
@@ -198,6 +200,15 @@ struct SplitFinalize<EpiScaledT<OutT>> {
 
 namespace {
 
+// The narrowest tile whose tiles all run at once, so that as many SMs as possible share the work; otherwise as for the other
+// GEMMs (333 x 2056 x 1552: 9.7 us with 64 columns, 10.7 with 128, 13.8 with 256).
+inline int tile_n(int M, int N, const LaunchOptions& opt) {
+  const long long tiles_m = (M + 2 * kBlockM - 1) / (2 * kBlockM), clusters = full_clusters(opt, 2);
+  for (int bn = 64; bn < 256 && opt.tile_n == 0; bn *= 2)
+    if (tiles_m * ((N + bn - 1) / bn) <= clusters) return bn;
+  return choose_tile_n(M, N, opt, true);
+}
+
 template <typename OutT>
 int run_scaled(const void* A, const float* a_scale, const void* B, const float* b_scale, void* D, int64_t ldd, int M, int N, int K,
                void* workspace, int64_t workspace_bytes, int* dev_status, cudaStream_t stream) {
@@ -205,7 +216,7 @@ int run_scaled(const void* A, const float* a_scale, const void* B, const float* 
   using Epi = EpiScaled<OutT>;
   const LaunchOptions opt = launch_options();
   if (opt.cta_group != 2) return fail(kBadArgument, "the e4m3 GEMM is built for CTA pairs only (cta_group = 2)");
-  if (M <= kSwapRows) return run_swapped<OutT>(A, a_scale, B, b_scale, D, ldd, M, N, K, workspace, workspace_bytes, dev_status, stream, opt);
+  if (swapped(M, K)) return run_swapped<OutT>(A, a_scale, B, b_scale, D, ldd, M, N, K, workspace, workspace_bytes, dev_status, stream, opt);
   typename Epi::Params ep;
   ep.D = static_cast<OutT*>(D);
   ep.ldd = ldd;
@@ -215,7 +226,7 @@ int run_scaled(const void* A, const float* a_scale, const void* B, const float* 
   const int rc = make_tmap_out(&ep.tm_d, ep.D, N, M, ldd);
   if (rc != kOk) return rc;
   const int K2 = K / 2;  // two e4m3 elements per two-byte unit
-  switch (choose_tile_n(M, N, opt, true)) {
+  switch (tile_n(M, N, opt)) {
     case 64: return launch_gemm_cfg<2, 64, false, false, Epi, ProE4M3>(A, K2, B, K2, M, N, K2, ep, dev_status, stream, opt);
     case 128: return launch_gemm_cfg<2, 128, false, false, Epi, ProE4M3>(A, K2, B, K2, M, N, K2, ep, dev_status, stream, opt);
     default: return launch_gemm_cfg<2, 256, false, false, Epi, ProE4M3>(A, K2, B, K2, M, N, K2, ep, dev_status, stream, opt);
@@ -224,7 +235,7 @@ int run_scaled(const void* A, const float* a_scale, const void* B, const float* 
 }  // namespace
 
 extern "C" int64_t coda_b200_gemm_e4m3_workspace_bytes(int M, int N, int K) {
-  if (M <= 0 || N <= 0 || K <= 0 || M > kSwapRows || M <= kFewRows) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || !swapped(M, K)) return 0;
   const LaunchOptions opt = launch_options();
   if (opt.split_tail == 0 || opt.cta_group != 2) return 0;
   const int clusters = full_clusters(opt, 2);
@@ -243,9 +254,8 @@ extern "C" int coda_b200_gemm_e4m3(const void* A, const float* a_scale, const vo
   if (K % 16 != 0) return fail(kBadArgument, "K must be a multiple of 16");
   if (N % 8 != 0 || ldd % 8 != 0 || ldd < N) return fail(kBadArgument, "N and ldd must be multiples of 8 with ldd >= N");
   if (workspace_bytes < 0) return fail(kBadArgument, "workspace_bytes must not be negative");
-  for (const void* p : {A, B, static_cast<const void*>(b_scale), static_cast<const void*>(D), static_cast<const void*>(workspace)})
-    if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0)
-      return fail(kBadArgument, "operands, output, column scales and workspace must be 16-byte aligned");
+  for (const void* p : {A, B, static_cast<const void*>(D), static_cast<const void*>(workspace)})
+    if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0) return fail(kBadArgument, "operands, output and workspace must be 16-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (d_is_fp32) return run_scaled<float>(A, a_scale, B, b_scale, D, ldd, M, N, K, workspace, workspace_bytes, dev_status, st);
   return run_scaled<__nv_bfloat16>(A, a_scale, B, b_scale, D, ldd, M, N, K, workspace, workspace_bytes, dev_status, st);

@@ -536,7 +536,7 @@ Tensor linear_e4m3(const Tensor& x_in, const Tensor& x_scale, const Tensor& weig
   require_no_grad("linear_e4m3", {&x_in, &x_scale, &weight_in, &weight_scale});
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::cuda::CUDAGuard guard(x_in.device());
-  const Tensor x = aligned16(x_in), xs = x_scale.contiguous(), weight = aligned16(weight_in), ws = aligned16(weight_scale);
+  const Tensor x = aligned16(x_in), xs = x_scale.contiguous(), weight = aligned16(weight_in), ws = weight_scale.contiguous();
   Tensor out = new_matrix(x, M, N, out_fp32 ? at::kFloat : at::kBFloat16);
   if (M == 0) return out;
   const int64_t parts_bytes = coda_b200_gemm_e4m3_workspace_bytes(static_cast<int>(M), static_cast<int>(N), static_cast<int>(K));

@@ -205,8 +205,7 @@ def gemm_e4m3(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor, 
     _require(weight.shape[0] > 0 and weight.shape[0] % 8 == 0, "the number of weight rows must be a positive multiple of 8")
     for name, s, n in (("x_scale", x_scale, x.shape[0]), ("weight_scale", weight_scale, weight.shape[0])):
         _require(s.dtype == torch.float32 and tuple(s.shape) == (n,), f"{name} must be float32 with one entry per row")
-    x, x_scale, weight = _aligned16(x), x_scale.contiguous(), _aligned16(weight)
-    weight_scale = _aligned16(weight_scale)
+    x, x_scale, weight, weight_scale = _aligned16(x), x_scale.contiguous(), _aligned16(weight), weight_scale.contiguous()
     out = torch.empty(x.shape[0], weight.shape[0], dtype=out_dtype, device=x.device)
     if x.shape[0] > 0:
         _gemm_e4m3_out(x, x_scale, weight, weight_scale, out)

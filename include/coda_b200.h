@@ -390,8 +390,8 @@ int coda_b200_rows_e4m3(const void* x, const void* residual, const void* weight,
                         int64_t rows, int64_t cols, int dtype, void* stream);
 
 /* D[m, n] = a_scale[m] * b_scale[n] * sum_k A[m, k] * B[n, k] for dense row-major e4m3 A [M, K] and B [N, K], fp32
- * accumulation; D is bf16 or fp32 with leading dimension ldd.  K a multiple of 16, N and ldd multiples of 8; A, B, D and
- * b_scale 16-byte aligned.  `workspace` (16-byte aligned, may be NULL) of coda_b200_gemm_e4m3_workspace_bytes lets the
+ * accumulation; D is bf16 or fp32 with leading dimension ldd.  K a multiple of 16, N and ldd multiples of 8; A, B and D
+ * 16-byte aligned.  `workspace` (16-byte aligned, may be NULL) of coda_b200_gemm_e4m3_workspace_bytes lets the
  * contraction of a product with few tiles be cut into parts; its contents need not be kept or cleared.  The sums are
  * added in a fixed order either way. */
 int64_t coda_b200_gemm_e4m3_workspace_bytes(int M, int N, int K);

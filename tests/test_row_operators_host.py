@@ -46,7 +46,7 @@ def test_c_entries_refuse_on_the_host():
     refused(lib.coda_b200_gemm_e4m3(p + 8, p, p, p, p, 16, 0, 4, 16, 32, None, 0, p, None), b"16-byte")
     refused(lib.coda_b200_gemm_e4m3(p, p, p, p, p, 16, 0, 0, 16, 32, None, 0, p, None), b"positive")
     refused(lib.coda_b200_gemm_e4m3(p, p, p, p, p, 16, 0, 4, 16, 32, p + 4, 64, p, None), b"16-byte")
-    assert lib.coda_b200_gemm_e4m3_workspace_bytes(100, 6144, 4096) > 0 == lib.coda_b200_gemm_e4m3_workspace_bytes(1, 6144, 4096)
+    assert lib.coda_b200_gemm_e4m3_workspace_bytes(50, 6144, 4096) > 0 == lib.coda_b200_gemm_e4m3_workspace_bytes(1, 6144, 4096)
     refused(lib.coda_b200_gemm_softmax_grad(p, 64, 1, p, 1, 64, p, p, -100, 0, p, 12, 4, 12, 64, p, None), b"ldg")
     refused(lib.coda_b200_gemm_softmax_grad(p, 64, 1, p, 1, 64, p, p, -100, -1, p, 16, 4, 12, 64, p, None), b"col0")
     refused(lib.coda_b200_ce_loss(p, 60, 1, p, 1, 60, p, -100, 1, p, p, p, p, p, p, p, 4, 12, 60, p, None), b"K must")
