@@ -283,17 +283,20 @@ __device__ __forceinline__ void note_used(const Dropout& d, long long* used) {
   if (used != nullptr && blockIdx.x == 0 && threadIdx.x < 2) used[threadIdx.x] = d.rng != nullptr ? d.rng[threadIdx.x] : 0;
 }
 
-// (sum of a, max of b >= 0) over the threads of a row: a warp (kWarp), or the whole block of at most 32 warps.  `red` is
-// two buffers of 64 floats used in turn, `turn` counts the calls: a buffer is written again only after the synchronisation
-// of the call in between, so one is enough.
-template <bool kWarp, bool kMax>
+// (sum of a, max of b >= 0) over the threads of a row: kLanes neighbouring lanes of a warp, or (0) the whole block of at
+// most 32 warps.  `red` is two buffers of 64 floats used in turn, `turn` counts the calls: a buffer is written again only
+// after the synchronisation of the call in between, so one is enough.
+template <int kLanes, bool kMax>
 __device__ __forceinline__ void row_reduce(float& a, float& b, float* red, int& turn) {
+  // the lanes of a row run together; those of the warp's other rows may have left the loop
+  constexpr uint32_t kOnes = kLanes == 0 || kLanes == 32 ? 0xffffffffu : (1u << (kLanes & 31)) - 1u;
+  const uint32_t lanes = kLanes == 0 || kLanes == 32 ? kOnes : kOnes << (threadIdx.x & 31 & ~(kLanes - 1));
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    if (kMax) b = max_nan(b, __shfl_xor_sync(0xffffffffu, b, o));
+  for (int o = kLanes == 0 ? 16 : kLanes / 2; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(lanes, a, o);
+    if (kMax) b = max_nan(b, __shfl_xor_sync(lanes, b, o));
   }
-  if constexpr (!kWarp) {
+  if constexpr (kLanes == 0) {
     float* r = red + 64 * (turn++ & 1);
     const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
     if (lane == 0) {
@@ -389,8 +392,8 @@ dropout_kernel(const T* __restrict__ x, T* __restrict__ out, long long total, lo
 // h * rstd * w.  kE4M3: out leaves as e4m3 values q with scale = max(max|out| / 448, 2^-126), q = out / scale rounded
 // to e4m3; without a weight the rows are converted as they are.
 //
-// Bound by HBM: every tensor is read or written once.  The block (kWarp: a warp) owns a row and keeps its h in registers,
-// kChunks chunks a thread; the grid is what fits the SMs at once, and a row's successor is loaded while the row is reduced
+// Bound by HBM: every tensor is read or written once.  The block (or kLanes lanes of a warp) owns a row and keeps its h in
+// registers, kChunks chunks a thread; the grid is what fits the SMs at once, and a row's successor is loaded while the row is reduced
 // and written.  A thread stays on the same columns for all of its rows (kShift: the grid's row stride is a multiple of 8, so
 // `off` stays too), so the weights are loaded once.
 constexpr int kWarpBlock = 256, kMaxThreads = 512;
@@ -402,31 +405,32 @@ constexpr int fwd_regs(int elem_bytes, bool shift, int chunks) { return chunks =
 constexpr int bwd_regs(int elem_bytes, bool shift, bool drop) { return shift ? 80 : elem_bytes == 4 && !drop ? 96 : 128; }
 constexpr int threads_per_sm(int regs) { return 512 / regs * 4 * 32; }  // whole warps in each quarter of the SM
 
-template <bool kWarp>
+template <int kLanes>
 struct RowLoop {
+  static constexpr int kPerBlock = kLanes == 0 ? 1 : kWarpBlock / (kLanes == 0 ? 1 : kLanes);  // rows of a block
   long long row, step;
   int tid, width;  // this thread and the number of threads of the row
   __device__ RowLoop()
-      : row(kWarp ? static_cast<long long>(blockIdx.x) * (kWarpBlock / 32) + threadIdx.x / 32 : blockIdx.x),
-        step(kWarp ? static_cast<long long>(gridDim.x) * (kWarpBlock / 32) : gridDim.x),
-        tid(kWarp ? threadIdx.x & 31 : threadIdx.x),
-        width(kWarp ? 32 : blockDim.x) {}
+      : row(kLanes == 0 ? blockIdx.x : static_cast<long long>(blockIdx.x) * kPerBlock + threadIdx.x / (kLanes == 0 ? 1 : kLanes)),
+        step(static_cast<long long>(gridDim.x) * kPerBlock),
+        tid(kLanes == 0 ? threadIdx.x : threadIdx.x & (kLanes - 1)),
+        width(kLanes == 0 ? blockDim.x : kLanes) {}
   // elements of the row's first chunk that belong to the row before it (kShift)
   __device__ int offset(int cols) const { return static_cast<int>((row * cols) & 7); }
 };
 
-template <typename T, bool kShift, bool kDrop, bool kWarp, int kChunks, bool kE4M3>
+template <typename T, bool kShift, bool kDrop, int kLanes, int kChunks, bool kE4M3>
 __global__ void __maxnreg__(fwd_regs(sizeof(T), kShift, kChunks))
 norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T* __restrict__ weight, float eps, Dropout d,
                 long long* __restrict__ used, T* __restrict__ h, T* __restrict__ out, float* __restrict__ rstd,
                 __nv_fp8_e4m3* __restrict__ q, float* __restrict__ scale, long long rows, int cols) {
-  __shared__ float red[kWarp ? 1 : 128];
+  __shared__ float red[kLanes != 0 ? 1 : 128];
   int turn = 0;
   const MaskOf<kDrop> mask(d);
   note_used(d, used);
   const int blocks = (cols + 3) / 4;
   const long long total = rows * cols;
-  RowLoop<kWarp> at;
+  RowLoop<kLanes> at;
   if (at.row >= rows) return;  // all threads of the row leave together
   const int off = kShift ? at.offset(cols) : 0;
   auto span = [&](int k) { return Span<kShift>(8 * (at.tid + k * at.width) - off, cols); };
@@ -471,7 +475,7 @@ norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T
 #pragma unroll
       for (int k = 0; k < kChunks; ++k) store_chunk(h + base + span(k).c0, v[k], span(k));
     }
-    row_reduce<kWarp, kE4M3>(sq, top, red, turn);
+    row_reduce<kLanes, kE4M3>(sq, top, red, turn);
     const float r = weight != nullptr ? rsqrtf(sq / static_cast<float>(cols) + eps) : 1.0f;
     const RowScale by(top * r);
     if (at.tid == 0) {
@@ -498,20 +502,20 @@ norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T
 //
 // Bound by HBM, and laid out as the forward; dw is summed in registers over a thread's rows and leaves as one partial row a
 // block, which fold_rows_kernel adds in a fixed order.
-template <typename T, bool kShift, bool kDrop, bool kWarp, int kChunks>
+template <typename T, bool kShift, bool kDrop, int kLanes, int kChunks>
 __global__ void __maxnreg__(bwd_regs(sizeof(T), kShift, kDrop))
 norm_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* __restrict__ h, const float* __restrict__ rstd,
                 const T* __restrict__ weight, Dropout d, T* __restrict__ dx, T* __restrict__ dres, float* __restrict__ partial,
                 long long rows, int cols) {
   // the next row's loads need as many registers again
   constexpr bool kPrefetch = !kShift && sizeof(T) == 2;
-  __shared__ float red[kWarp ? 1 : 128];
-  __shared__ float fold[kWarp ? 256 : 1];
+  __shared__ float red[kLanes != 0 ? 1 : 128];
+  __shared__ float fold[kLanes != 0 ? 256 : 1];
   int turn = 0;
   const MaskOf<kDrop> mask(d);
   const int blocks = (cols + 3) / 4;
   const long long total = rows * cols;
-  RowLoop<kWarp> at;
+  RowLoop<kLanes> at;
   const int off = kShift ? at.offset(cols) : 0;
   auto span = [&](int k) { return Span<kShift>(8 * (at.tid + k * at.width) - off, cols); };
   struct Row {
@@ -559,7 +563,7 @@ norm_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* _
         dot = fmaf(t, chunk_get(w[k], j), dot);
       }
     }
-    row_reduce<kWarp, false>(dot, unused, red, turn);
+    row_reduce<kLanes, false>(dot, unused, red, turn);
     const float m = dot / static_cast<float>(cols);
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
@@ -580,12 +584,12 @@ norm_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* _
   }
   if (partial == nullptr) return;
   float* mine = partial + static_cast<long long>(blockIdx.x) * cols;
-  if constexpr (kWarp) {
-    // the warps of a block add up in turn
+  if constexpr (kLanes != 0) {
+    // the rows' lanes add up in turn
     for (int c = threadIdx.x; c < cols; c += kWarpBlock) fold[c] = 0.f;
     __syncthreads();
-    for (int i = 0; i < kWarpBlock / 32; ++i) {
-      if (static_cast<int>(threadIdx.x) / 32 == i) {
+    for (int i = 0; i < RowLoop<kLanes>::kPerBlock; ++i) {
+      if (static_cast<int>(threadIdx.x) / kLanes == i) {
 #pragma unroll
         for (int k = 0; k < kChunks; ++k)
 #pragma unroll
@@ -621,7 +625,7 @@ norm_fwd_long_kernel(const T* __restrict__ x, const T* __restrict__ residual, co
   note_used(d, used);
   const int blocks = (cols + 3) / 4;
   const long long total = rows * cols;
-  for (RowLoop<false> at; at.row < rows; at.row += at.step) {
+  for (RowLoop<0> at; at.row < rows; at.row += at.step) {
     const long long base = at.row * cols;
     const int first = 8 * at.tid - (kShift ? at.offset(cols) : 0);
     auto value = [&](const Span<kShift>& s, float* v) {  // h of a chunk, unrounded
@@ -659,7 +663,7 @@ norm_fwd_long_kernel(const T* __restrict__ x, const T* __restrict__ residual, co
         }
       }
     }
-    row_reduce<false, kE4M3>(sq, top, red, turn);
+    row_reduce<0, kE4M3>(sq, top, red, turn);
     const float r = weight != nullptr ? rsqrtf(sq / static_cast<float>(cols) + eps) : 1.0f;
     const RowScale by(top * r);
     if (at.tid == 0) {
@@ -712,7 +716,7 @@ norm_bwd_long_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const
   extern __shared__ __align__(16) float shared_sums[];
   float* out_row = partial != nullptr ? partial + static_cast<long long>(blockIdx.x) * cols : nullptr;
   bool first_row = true;
-  for (RowLoop<false> at; at.row < rows; at.row += at.step, first_row = false) {
+  for (RowLoop<0> at; at.row < rows; at.row += at.step, first_row = false) {
     const long long base = at.row * cols;
     const int first = 8 * at.tid - (kShift ? at.offset(cols) : 0);
     const float r = rstd[at.row];
@@ -741,7 +745,7 @@ norm_bwd_long_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const
         else add_sums(out_row + c, v, s, first_row);
       }
     }
-    row_reduce<false, false>(dot, unused, red, turn);
+    row_reduce<0, false>(dot, unused, red, turn);
     const float m = dot / static_cast<float>(cols);
     for (int c = first; c < cols; c += 8 * kLongThreads) {
       const Span<kShift> s(c, cols);
@@ -816,20 +820,23 @@ inline int make_dropout(double p, const int64_t* rng, int64_t stream_id, Dropout
   return kOk;
 }
 
-// How a launch covers the rows: chunks a thread (1: a warp a row; 2 or 4: a block of `threads` a row; 0: the kernels for
-// long rows).  Two chunks a thread as far as they reach, in blocks of exactly as many warps as the row needs.
+// How a launch covers the rows: one chunk a thread and 8, 16 or 32 lanes a row (`lanes`); or a block of `threads` a row with
+// two or four chunks a thread, two as far as they reach, in exactly as many warps as the row needs; or (chunks = 0) the
+// kernels for long rows.  A whole warp for rows of 64 columns: 178 us forward, 308 us backward at 2^20 rows of bf16; eight lanes:
+// 84 and 122 us.
 struct RowPlan {
   bool shift;
-  int chunks, threads;
+  int lanes, chunks, threads;
   int64_t grid;
 };
 inline RowPlan row_plan(int64_t rows, int64_t cols, int dtype, bool backward, bool drop) {
   RowPlan p;
   p.shift = cols % 8 != 0;
   const int64_t n = (cols + (p.shift ? 14 : 7)) / 8;  // chunks a row may touch
+  p.lanes = n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : 0;
   p.chunks = n <= 32 ? 1 : n <= 2 * kMaxThreads ? 2 : n <= 4 * kMaxThreads && !backward ? 4 : 0;
   p.threads = p.chunks == 1 ? kWarpBlock : p.chunks == 0 ? kLongThreads : static_cast<int>((n + 32 * p.chunks - 1) / (32 * p.chunks) * 32);
-  const int64_t per_block = p.chunks == 1 ? kWarpBlock / 32 : 1, need = (rows + per_block - 1) / per_block;
+  const int64_t per_block = p.lanes != 0 ? kWarpBlock / p.lanes : 1, need = (rows + per_block - 1) / per_block;
   const int elem = dtype == 2 ? 4 : 2, regs = backward ? bwd_regs(elem, p.shift, drop) : fwd_regs(elem, p.shift, p.chunks);
   const int fit = p.chunks == 0 ? (backward && cols > kSharedCols / 2 && cols <= kSharedCols ? 1 : 2) : threads_per_sm(regs) / p.threads;
   const int64_t cap = std::max(static_cast<int64_t>(sm_count()) * std::min(std::max(fit, 1), 32) / 8, int64_t{1}) * 8;  // kShift: rows advance by multiples of 8
@@ -859,14 +866,20 @@ template <class F>
 int by_flag(bool flag, F&& f) {
   return flag ? f(std::true_type()) : f(std::false_type());
 }
+template <int kLanes_, int kChunks_>
+struct Shape {
+  static constexpr int kLanes = kLanes_, kChunks = kChunks_;
+};
 template <bool kBackward, class F>
-int by_chunks(int chunks, F&& f) {
-  if (chunks == 1) return f(std::integral_constant<int, 1>());
-  if (chunks == 2) return f(std::integral_constant<int, 2>());
+int by_shape(const RowPlan& p, F&& f) {
+  if (p.lanes == 8) return f(Shape<8, 1>());
+  if (p.lanes == 16) return f(Shape<16, 1>());
+  if (p.lanes == 32) return f(Shape<32, 1>());
+  if (p.chunks == 2) return f(Shape<0, 2>());
   if constexpr (!kBackward) {
-    if (chunks == 4) return f(std::integral_constant<int, 4>());
+    if (p.chunks == 4) return f(Shape<0, 4>());
   }
-  return f(std::integral_constant<int, 0>());
+  return f(Shape<0, 0>());
 }
 
 template <bool kE4M3>
@@ -876,13 +889,13 @@ int launch_norm_fwd(const void* x, const void* residual, const void* weight, flo
   return by_dtype(dtype, [&](auto t) {
     return by_flag(plan.shift, [&](auto shift) {
       return by_flag(!kE4M3 && d.rng != nullptr, [&](auto drop) {
-        return by_chunks<false>(plan.chunks, [&](auto chunks) {
+        return by_shape<false>(plan, [&](auto shape) {
           using T = decltype(t);
           constexpr bool kShift = decltype(shift)::value, kDrop = !kE4M3 && decltype(drop)::value;
-          constexpr int kChunks = decltype(chunks)::value;
+          constexpr int kLanes = decltype(shape)::kLanes, kChunks = decltype(shape)::kChunks;
           auto kern = [] {
             if constexpr (kChunks == 0) return norm_fwd_long_kernel<T, kShift, kDrop, kE4M3>;
-            else return norm_fwd_kernel<T, kShift, kDrop, kChunks == 1, kChunks, kE4M3>;
+            else return norm_fwd_kernel<T, kShift, kDrop, kLanes, kChunks, kE4M3>;
           }();
           kern<<<static_cast<int>(plan.grid), plan.threads, 0, static_cast<cudaStream_t>(stream)>>>(
               static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const T*>(weight), eps, d,
@@ -976,12 +989,12 @@ extern "C" int coda_b200_add_rmsnorm_bwd(const void* dout, const void* dh, const
     using T = decltype(t);
     const int rc2 = by_flag(plan.shift, [&](auto shift) {
       return by_flag(d.rng != nullptr, [&](auto drop) {
-        return by_chunks<true>(plan.chunks, [&](auto chunks) {
+        return by_shape<true>(plan, [&](auto shape) {
           constexpr bool kShift = decltype(shift)::value, kDrop = decltype(drop)::value;
-          constexpr int kChunks = decltype(chunks)::value;
+          constexpr int kLanes = decltype(shape)::kLanes, kChunks = decltype(shape)::kChunks;
           auto kern = [] {
             if constexpr (kChunks == 0) return norm_bwd_long_kernel<T, kShift, kDrop>;
-            else return norm_bwd_kernel<T, kShift, kDrop, kChunks == 1, kChunks>;
+            else return norm_bwd_kernel<T, kShift, kDrop, kLanes, kChunks>;
           }();
           int shared = 0;
           if (kChunks == 0 && dweight != nullptr && cols <= kSharedCols) {

@@ -152,13 +152,13 @@ def check_norm(dtype, p, x, res, w, dout, dh, out, h, dx, dres, dw):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,cols,p", [(1, 1, 0.0), (1, 4096, 0.1), (2, 7, 0.5), (33, 64, 0.1), (5, 1000, 0.0), (130, 1531, 0.25),
-                                         (1200, 128, 0.1), (700, 2056, 0.0), (9, 8192, 0.1), (3, 20004, 0.1), (2, 33001, 0.0)])
+                                         (1200, 128, 0.1), (700, 2056, 0.0), (9, 8192, 0.1), (3, 20004, 0.1), (2, 33001, 0.0), (30001, 50, 0.1), (2051, 121, 0.2), (10007, 3, 0.5)])
 def test_add_rms_norm(ck, dtype, rows, cols, p):
     check_norm(dtype, p, *norm_case(ck, dtype, rows, cols, p))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,cols", [(1, 8), (65, 513), (300, 4096), (4, 16384), (2, 40000), (2, 60001), (2000, 257), (3000, 250), (700, 8190), (1300, 4095)])
+@pytest.mark.parametrize("rows,cols", [(1, 8), (65, 513), (300, 4096), (4, 16384), (2, 40000), (2, 60001), (2000, 257), (3000, 250), (4099, 65), (20000, 64), (777, 128), (5003, 13), (700, 8190), (1300, 4095)])
 def test_rms_norm(ck, dtype, rows, cols):
     check_norm(dtype, 0.0, *norm_case(ck, dtype, rows, cols, 0.0, residual=False))
 
@@ -260,7 +260,7 @@ def check_e4m3(q, scale, want):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 4096), (3, 7), (64, 128), (37, 1531), (500, 2048), (2, 16384), (3, 20001)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 4096), (3, 7), (64, 128), (37, 1531), (500, 2048), (2, 16384), (3, 20001), (9001, 64), (8191, 57), (3001, 100)])
 def test_rows_in_e4m3(ck, dtype, rows, cols):
     x, res, w = randn(rows, cols, dtype=dtype), randn(rows, cols, dtype=dtype, seed=1), randn(cols, dtype=dtype, seed=2, mean=1.0, std=0.2)
     h64 = x.double() + res.double()
