@@ -84,8 +84,12 @@ SIGNATURES = {
     "coda_b200_rows_e4m3": (_I, [_P, _P, _P, _F, _P, _P, _P, _L, _L, _I, _P]),
     "coda_b200_gemm_e4m3_workspace_bytes": (_L, [_I, _I, _I]),
     "coda_b200_gemm_e4m3": (_I, [_P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P, _L, _P, _P]),
-    "coda_b200_ce_loss": (_I, [_P, _L, _L, _P, _L, _L, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P]),
-    "coda_b200_gemm_softmax_grad": (_I, [_P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _P, _L, _I, _I, _I, _P, _P]),
+    "coda_b200_ce_compacts": (_I, [_I, _I, _I]),
+    "coda_b200_ce_compact": (_I, [_P, _P, _I, _P, _P, _P, _P, _I, _I, _P]),
+    "coda_b200_ce_scatter": (_I, [_P, _P, _P, _I, _I, _P]),
+    "coda_b200_gemm_live": (_I, [_P, _L, _P, _L, _P, _P, _L, _I, _P, _P, _I, _I, _I, _I, _P, _P]),
+    "coda_b200_ce_loss": (_I, [_P, _L, _L, _P, _L, _L, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P]),
+    "coda_b200_gemm_softmax_grad": (_I, [_P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _P, _P, _L, _I, _I, _I, _P, _P]),
 }
 
 
@@ -143,7 +147,7 @@ class option_override:
     puts the previous value (as set through this module; the library's default otherwise) back afterwards.  Options are
     process-wide and read once per launch, so this is for the thread that issues the launches."""
 
-    _defaults = {"max_ctas": 0, "group_m": 0, "tile_n": 0, "cta_group": 2, "epi_tma": 1, "split_tail": 1, "probe_ld_kb": 0, "probe_st_kb": 0}
+    _defaults = {"max_ctas": 0, "group_m": 0, "tile_n": 0, "cta_group": 2, "epi_tma": 1, "split_tail": 1, "ce_compact": 1, "probe_ld_kb": 0, "probe_st_kb": 0}
 
     def __init__(self, name: str, value: int):
         self.name, self.value = name, int(value)

@@ -183,7 +183,20 @@ struct ProNone {
   static constexpr int kWarps = 0;
   static constexpr uint32_t kStageExtraBytes = 0;
   static constexpr bool kE4M3 = false;
+  static constexpr int kLive = 0;
   struct Params {};
+};
+
+// No prologue, but the device knows how much of the product there is: only the first *live rows (kLive = 1), or the first
+// *live elements of the contraction (kLive = 2), count.  Both are rounded up to 64, so at least one block of the
+// contraction and whole 32-row sub-tiles are always worked on; the operands have to be defined (and, along the contraction,
+// zero in one of them) up to there.
+template <int kLive_>
+struct ProLive : ProNone {
+  static constexpr int kLive = kLive_;
+  struct Params {
+    const int* live;
+  };
 };
 
 // No prologue, but e4m3 operands (both K-major).  Everything in front of the MMA moves bytes, so a k-block of 64 two-byte
@@ -201,6 +214,7 @@ struct ProE4M3 : ProNone {
 struct ProDSigmoid {
   static constexpr int kWarps = 4;
   static constexpr bool kE4M3 = false;
+  static constexpr int kLive = 0;
   static constexpr uint32_t kStageExtraBytes = kBlockM * kBlockK * 2;  // the dout tile
   struct Params {
     alignas(64) CUtensorMap tm_dout;  // dout as [M, Kc], box 64 x 128, 128-byte swizzle (the A operand's geometry)
@@ -223,9 +237,25 @@ struct ProDSigmoid {
   }
 };
 
+template <class Pro, int kTileM>
+__device__ __forceinline__ GemmShape live_shape(const GemmShape& given, const typename Pro::Params& pp) {
+  if constexpr (Pro::kLive == 0) return given;
+  else {
+    GemmShape s = given;
+    const int live = (max(__ldg(pp.live), 1) + 63) / 64 * 64;
+    if constexpr (Pro::kLive == 1) {
+      s.M = min(given.M, live);
+      s.tiles_m = (s.M + kTileM - 1) / kTileM;
+    } else {
+      s.K = min(given.K, live);
+    }
+    return s;
+  }
+}
+
 template <int kCtaGroup, int kBN, bool kAMn, bool kBMn, class Epi, class Pro = ProNone>
 __global__ void __launch_bounds__(kNumThreads + Pro::kWarps * 32, 1)
-gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const GemmShape shape,
+gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const GemmShape given,
             const __grid_constant__ typename Epi::Params ep, int* __restrict__ status,
             const __grid_constant__ typename Pro::Params pp) {
   using Cfg = GemmCfg<kCtaGroup, kBN, Epi::kLoadRingBytes, Pro::kStageExtraBytes>;
@@ -236,6 +266,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
   constexpr int kBNcta = Cfg::kBNcta;
   constexpr uint32_t kABytes = Cfg::kABytes;
   constexpr uint32_t kStageBytes = Cfg::kStageBytes;
+  const GemmShape shape = live_shape<Pro, kBlockM * kCtaGroup>(given, pp);
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);

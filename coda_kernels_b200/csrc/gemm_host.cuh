@@ -39,6 +39,7 @@ struct Options {
   std::atomic<int> tile_n{0};     // 0 = choose per problem; 64, 128 or 256 forces the column-tile width where it is built
   std::atomic<int> epi_tma{1};    // 1 = epilogues stage their output in shared memory and store it with TMA; 0 = per-thread stores
   std::atomic<int> split_tail{1};  // 1 = a plain GEMM given a workspace may cut the tiles of its last round along K
+  std::atomic<int> ce_compact{1};  // 1 = the piecewise cross entropy leaves ignored rows out of large products
   // Measurement aid: KB of extra global loads / shared stores per k-block and CTA issued by the epilogue warps while the
   // mainloop runs (the traffic an operand-transforming prologue would add); results are unaffected.  0 = off.
   std::atomic<int> probe_ld_kb{0};

@@ -30,6 +30,9 @@ extern "C" int coda_b200_set_option(const char* name, int value) {
   } else if (!strcmp(name, "split_tail")) {
     if (value != 0 && value != 1) return fail(kBadArgument, "split_tail must be 0 or 1");
     o.split_tail = value;
+  } else if (!strcmp(name, "ce_compact")) {
+    if (value != 0 && value != 1) return fail(kBadArgument, "ce_compact must be 0 or 1");
+    o.ce_compact = value;
   } else if (!strcmp(name, "probe_ld_kb") || !strcmp(name, "probe_st_kb")) {
     if (value < 0 || value > 256) return fail(kBadArgument, "probe traffic must be between 0 and 256 KB per k-block");
     (name[6] == 'l' ? o.probe_ld_kb : o.probe_st_kb) = value;

@@ -549,10 +549,25 @@ Tensor linear_e4m3(const Tensor& x_in, const Tensor& x_scale, const Tensor& weig
   return out;
 }
 
-// (loss, inv_count, lse); every matrix operand is dense, so its strides are its extents
-std::tuple<Tensor, Tensor, Tensor> run_ce(const Tensor& x, const Tensor& weight, const Tensor& target, int64_t ignore_index, bool mean,
-                                          const Tensor& status) {
-  const c10::cuda::CUDAGuard guard(x.device());
+// What the loss's products work on: x and target, or, where that pays, the rows that count put first (then `live` says how
+// many, and `position` where each row went).  Every matrix operand is dense, so its strides are its extents.
+struct CeRows {
+  Tensor x, target, position, live;
+};
+CeRows ce_rows(const Tensor& x, const Tensor& target, int64_t ignore_index, int64_t V) {
+  const int M = static_cast<int>(x.size(0)), K = static_cast<int>(x.size(1));
+  if (M == 0 || !coda_b200_ce_compacts(M, static_cast<int>(V), K)) return {x, target, Tensor(), Tensor()};
+  CeRows r{at::empty_like(x), at::empty_like(target), at::empty_like(target), at::empty({1}, target.options())};
+  check(coda_b200_ce_compact(x.data_ptr(), target.data_ptr<int32_t>(), static_cast<int>(ignore_index), r.position.data_ptr<int32_t>(),
+                             r.target.data_ptr<int32_t>(), r.live.data_ptr<int32_t>(), r.x.data_ptr(), M, K, stream_of(x)),
+        "ce_compact");
+  return r;
+}
+inline const int32_t* live_ptr(const Tensor& live) { return live.defined() ? live.data_ptr<int32_t>() : nullptr; }
+
+// (loss, inv_count, lse)
+std::tuple<Tensor, Tensor, Tensor> run_ce(const CeRows& r, const Tensor& weight, int64_t ignore_index, bool mean, const Tensor& status) {
+  const Tensor& x = r.x;
   const int64_t M = x.size(0), V = weight.size(0), K = x.size(1);
   const auto f32 = x.options().dtype(at::kFloat);
   if (M == 0)  // a sum over nothing, and 0 / 0
@@ -560,18 +575,19 @@ std::tuple<Tensor, Tensor, Tensor> run_ce(const Tensor& x, const Tensor& weight,
   const int64_t tiles = coda_b200_lse_tiles(static_cast<int>(V));
   Tensor parts = at::empty({2 * M * tiles + 2 * M}, f32), lse = at::empty({M}, f32), loss = at::empty({}, f32), inv_count = at::empty({}, f32);
   float* part = parts.data_ptr<float>();
-  check(coda_b200_ce_loss(x.data_ptr(), K, 1, weight.data_ptr(), 1, K, target.data_ptr<int32_t>(), static_cast<int>(ignore_index), mean, part,
-                          part + M * tiles, part + 2 * M * tiles, lse.data_ptr<float>(), part + 2 * M * tiles + M, loss.data_ptr<float>(),
-                          inv_count.data_ptr<float>(), static_cast<int>(M), static_cast<int>(V), static_cast<int>(K), status_ptr(status),
-                          stream_of(x)),
+  check(coda_b200_ce_loss(x.data_ptr(), K, 1, weight.data_ptr(), 1, K, r.target.data_ptr<int32_t>(), static_cast<int>(ignore_index), mean,
+                          live_ptr(r.live), part, part + M * tiles, part + 2 * M * tiles, lse.data_ptr<float>(), part + 2 * M * tiles + M,
+                          loss.data_ptr<float>(), inv_count.data_ptr<float>(), static_cast<int>(M), static_cast<int>(V), static_cast<int>(K),
+                          status_ptr(status), stream_of(x)),
         "ce_loss");
   return {loss, inv_count, lse};
 }
 
 // Walks the vocabulary in pieces of `piece` columns with one [M, piece] buffer: the piece's softmax gradient, then its
 // rows of dweight, then its share of dx, summed over the pieces in fp32.
-OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tensor& lse, const Tensor& x, const Tensor& weight,
-                        const Tensor& target, int64_t ignore_index, int64_t piece, bool need_dx, bool need_dw, const Tensor& status) {
+OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tensor& lse, const CeRows& r, const Tensor& weight,
+                        int64_t ignore_index, int64_t piece, bool need_dx, bool need_dw, const Tensor& status) {
+  const Tensor& x = r.x;
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t M = x.size(0), V = weight.size(0), K = x.size(1);
   OptTensor dx, dw, dx32;
@@ -582,6 +598,7 @@ OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tens
   }
   const Tensor xs = x.as_strided({M, K}, {K, 1}), ws = weight.as_strided({V, K}, {K, 1});
   const OptTensor alpha = (dloss * inv_count).reshape({1}).to(at::kFloat);
+  const int32_t* live = live_ptr(r.live);
   const int64_t width = std::min(piece, V), ldg = (width + 7) / 8 * 8;
   Tensor g = new_matrix(x, M, ldg, at::kBFloat16);
   if (need_dx) dx = new_matrix(x, M, K, at::kBFloat16);
@@ -590,30 +607,54 @@ OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tens
   for (int64_t c0 = 0; c0 < V; c0 += width) {
     const int64_t n = std::min(width, V - c0);
     const Tensor w = ws.narrow(0, c0, n), gp = g.as_strided({M, n}, {ldg, 1});
-    check(coda_b200_gemm_softmax_grad(xs.data_ptr(), K, 1, w.data_ptr(), 1, K, lse.data_ptr<float>(), target.data_ptr<int32_t>(),
-                                      static_cast<int>(ignore_index), static_cast<int>(c0), gp.data_ptr(), ldg, static_cast<int>(M),
+    check(coda_b200_gemm_softmax_grad(xs.data_ptr(), K, 1, w.data_ptr(), 1, K, lse.data_ptr<float>(), r.target.data_ptr<int32_t>(),
+                                      static_cast<int>(ignore_index), static_cast<int>(c0), live, gp.data_ptr(), ldg, static_cast<int>(M),
                                       static_cast<int>(n), static_cast<int>(K), status_ptr(status), stream_of(x)),
           "gemm_softmax_grad");
     if (need_dw) {
       Tensor out = dw->narrow(0, c0, n);
-      gemm_out(gp.t(), xs, out, alpha, c10::nullopt, status);
+      if (live == nullptr)
+        gemm_out(gp.t(), xs, out, alpha, c10::nullopt, status);
+      else
+        check(coda_b200_gemm_live(gp.data_ptr(), ldg, xs.data_ptr(), K, nullptr, out.data_ptr(), K, 0, alpha->data_ptr<float>(), live, 1,
+                                  static_cast<int>(n), static_cast<int>(K), static_cast<int>(M), status_ptr(status), stream_of(x)),
+              "gemm_live");
     }
     if (need_dx) {
-      Tensor out = c0 + n < V ? *dx32 : *dx;
-      gemm_out(gp, w, out, alpha, c0 > 0 ? dx32 : c10::nullopt, status);
+      const bool last = c0 + n == V;
+      Tensor out = last ? *dx : *dx32;
+      // a product with so few tiles that its last round is cut along the contraction runs over all rows (what it makes of the
+      // others is not looked at): 1003 x 1032 x 32003, 404 us a step instead of 613
+      const bool cut = c0 == 0 && coda_b200_gemm_workspace_bytes(static_cast<int>(M), static_cast<int>(K), static_cast<int>(n)) > 0;
+      if (live == nullptr || cut)
+        gemm_out(gp, w, out, alpha, c0 > 0 ? dx32 : c10::nullopt, status);
+      else
+        check(coda_b200_gemm_live(gp.data_ptr(), ldg, w.data_ptr(), K, c0 > 0 ? dx32->data_ptr<float>() : nullptr, out.data_ptr(), K, !last,
+                                  alpha->data_ptr<float>(), live, 0, static_cast<int>(M), static_cast<int>(K), static_cast<int>(n),
+                                  status_ptr(status), stream_of(x)),
+              "gemm_live");
     }
+  }
+  if (need_dx && live != nullptr) {
+    Tensor out = new_matrix(x, M, K, at::kBFloat16);
+    check(coda_b200_ce_scatter(dx->data_ptr(), r.position.data_ptr<int32_t>(), out.data_ptr(), static_cast<int>(M), static_cast<int>(K),
+                               stream_of(x)),
+          "ce_scatter");
+    dx = out;
   }
   return {dx, dw};
 }
 
 class CePiecesNode : public torch::autograd::Function<CePiecesNode> {
  public:
-  static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& weight_in, const Tensor& target_in, int64_t ignore_index,
-                        bool mean, int64_t piece, const Tensor& status) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight_in, const Tensor& target, int64_t ignore_index, bool mean,
+                        int64_t piece, const Tensor& status) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor x = aligned16(x_in), weight = aligned16(weight_in), target = target_in.contiguous();
-    auto [loss, inv_count, lse] = run_ce(x, weight, target, ignore_index, mean, status);
-    ctx->save_for_backward({x, weight, target, lse, inv_count});
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor weight = aligned16(weight_in);
+    const CeRows r = ce_rows(aligned16(x), target.contiguous(), ignore_index, weight.size(0));
+    auto [loss, inv_count, lse] = run_ce(r, weight, ignore_index, mean, status);
+    ctx->save_for_backward({r.x, weight, r.target, lse, inv_count, r.position, r.live});
     ctx->saved_data["ignore_index"] = ignore_index;
     ctx->saved_data["piece"] = piece;
     ctx->saved_data["status"] = status;
@@ -622,7 +663,7 @@ class CePiecesNode : public torch::autograd::Function<CePiecesNode> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     require_first_order("linear_cross_entropy_pieces");
     const auto s = ctx->get_saved_variables();
-    auto [dx, dw] = run_ce_backward(grads[0], s[4], s[3], s[0], s[1], s[2], ctx->saved_data["ignore_index"].toInt(),
+    auto [dx, dw] = run_ce_backward(grads[0], s[4], s[3], CeRows{s[0], s[2], s[5], s[6]}, s[1], ctx->saved_data["ignore_index"].toInt(),
                                     ctx->saved_data["piece"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1),
                                     ctx->saved_data["status"].toTensor());
     return {dx.value_or(Tensor()), dw.value_or(Tensor()), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
@@ -643,7 +684,9 @@ Tensor linear_cross_entropy_pieces(const Tensor& x, const Tensor& weight, const 
   TORCH_CHECK_VALUE(x.size(0) <= INT_MAX && weight.size(0) <= INT_MAX - 256, "extents must fit 31 bits");
   if (wants_grad({&x, &weight})) return CePiecesNode::apply(x, weight, target, ignore_index, mean, piece, status);
   at::AutoDispatchBelowADInplaceOrView below;
-  return std::get<0>(run_ce(aligned16(x), aligned16(weight), target.contiguous(), ignore_index, mean, status));
+  const c10::cuda::CUDAGuard guard(x.device());
+  return std::get<0>(run_ce(ce_rows(aligned16(x), target.contiguous(), ignore_index, weight.size(0)), aligned16(weight), ignore_index, mean,
+                            status));
 }
 
 }  // namespace

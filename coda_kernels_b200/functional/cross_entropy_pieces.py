@@ -5,6 +5,9 @@ batch, ``2 M V`` bytes, from forward to backward.  Here the node keeps the rows'
 backward walks the vocabulary in pieces, computes each piece's logits again and turns them into its part of the two
 gradients.  The price is that one product (a third more work in the backward); what it saves is everything of size
 ``M V`` but one ``[M, piece]`` buffer during the backward.
+
+Ignored rows have no part in the products where those are large enough to be worth it: the rows that count are first put
+together on the device, and the products end where they end, without the host knowing where that is.
 """
 
 from __future__ import annotations
@@ -20,14 +23,14 @@ from ..ops_rows import _require_first_order, call_native
 
 
 class LinearCrossEntropyPieces(torch.autograd.Function):
-    """Saves ``(x, weight, target, lse, inv_count)``."""
+    """Saves the rows (``x``, or its rows that count, put first), their labels, the weight, the log-sum-exp and ``inv_count``."""
 
     @staticmethod
     @input_guard
     @autocast_custom_fwd
     def forward(ctx, x, weight, target, ignore_index: int, reduction: str, piece: int) -> torch.Tensor:
-        loss, inv_count, lse = ce_pieces_forward(x, weight, target, ignore_index, reduction == "mean")
-        ctx.save_for_backward(x, weight, target, lse, inv_count)
+        loss, inv_count, lse, rows, labels, position, live = ce_pieces_forward(x, weight, target, ignore_index, reduction == "mean")
+        ctx.save_for_backward(rows, weight, labels, lse, inv_count, position, live)
         ctx.ignore_index, ctx.piece = ignore_index, piece
         return loss
 
@@ -36,10 +39,10 @@ class LinearCrossEntropyPieces(torch.autograd.Function):
     @autocast_custom_bwd
     def backward(ctx, dloss: torch.Tensor):
         _require_first_order("linear_cross_entropy_pieces")
-        x, weight, target, lse, inv_count = ctx.saved_tensors
+        rows, weight, labels, lse, inv_count, position, live = ctx.saved_tensors
         need_dx, need_dw = ctx.needs_input_grad[:2]
-        return (*ce_pieces_backward(dloss, inv_count, lse, x, weight, target, ctx.ignore_index, ctx.piece, need_dx, need_dw),
-                None, None, None, None)
+        return (*ce_pieces_backward(dloss, inv_count, lse, rows, weight, labels, position, live, ctx.ignore_index, ctx.piece, need_dx,
+                                    need_dw), None, None, None, None)
 
 
 def linear_cross_entropy_pieces(

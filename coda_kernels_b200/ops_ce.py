@@ -16,33 +16,64 @@ from ._lib import check, lib
 from .ops import _noop_fake, _require, _require_cuda_bf16, _stream, gemm, lse_tiles, status_word
 
 
+def _ptr(t: Optional[Tensor]):
+    return None if t is None else t.data_ptr()
+
+
 @torch.library.custom_op("coda_b200::ce_loss_out", mutates_args=("parts", "lse", "loss", "inv_count"), device_types="cuda")
-def _ce_loss_out(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, mean: bool, parts: Tensor, lse: Tensor, loss: Tensor,
-                 inv_count: Tensor) -> None:
+def _ce_loss_out(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, mean: bool, live: Optional[Tensor], parts: Tensor,
+                 lse: Tensor, loss: Tensor, inv_count: Tensor) -> None:
     M, K = x.shape
     V = weight.shape[0]
     tiles = lse_tiles(V)
     base = parts.data_ptr()
     check(
-        lib.coda_b200_ce_loss(x.data_ptr(), K, 1, weight.data_ptr(), 1, K, target.data_ptr(), ignore_index, int(mean), base, base + 4 * M * tiles,
-                              base + 8 * M * tiles, lse.data_ptr(), base + 8 * M * tiles + 4 * M, loss.data_ptr(), inv_count.data_ptr(), M, V,
+        lib.coda_b200_ce_loss(x.data_ptr(), K, 1, weight.data_ptr(), 1, K, target.data_ptr(), ignore_index, int(mean), _ptr(live), base,
+                              base + 4 * M * tiles, base + 8 * M * tiles, lse.data_ptr(), base + 8 * M * tiles + 4 * M, loss.data_ptr(), inv_count.data_ptr(), M, V,
                               K, status_word(x.device).data_ptr(), _stream(x)),
         "ce_loss",
     )
 
 
 @torch.library.custom_op("coda_b200::gemm_softmax_grad_out", mutates_args=("grad",), device_types="cuda")
-def _gemm_softmax_grad_out(x: Tensor, weight: Tensor, lse: Tensor, target: Tensor, ignore_index: int, col0: int, grad: Tensor) -> None:
+def _gemm_softmax_grad_out(x: Tensor, weight: Tensor, lse: Tensor, target: Tensor, ignore_index: int, col0: int, live: Optional[Tensor],
+                           grad: Tensor) -> None:
     M, K = x.shape
     N = weight.shape[0]
     check(
         lib.coda_b200_gemm_softmax_grad(x.data_ptr(), K, 1, weight.data_ptr(), 1, K, lse.data_ptr(), target.data_ptr(), ignore_index, col0,
-                                        grad.data_ptr(), grad.shape[1], M, N, K, status_word(x.device).data_ptr(), _stream(x)),
+                                        _ptr(live), grad.data_ptr(), grad.shape[1], M, N, K, status_word(x.device).data_ptr(), _stream(x)),
         "gemm_softmax_grad",
     )
 
 
-for _op in (_ce_loss_out, _gemm_softmax_grad_out):
+@torch.library.custom_op("coda_b200::ce_compact_out", mutates_args=("position", "labels", "live", "rows"), device_types="cuda")
+def _ce_compact_out(x: Tensor, target: Tensor, ignore_index: int, position: Tensor, labels: Tensor, live: Tensor, rows: Tensor) -> None:
+    check(
+        lib.coda_b200_ce_compact(x.data_ptr(), target.data_ptr(), ignore_index, position.data_ptr(), labels.data_ptr(), live.data_ptr(),
+                                 rows.data_ptr(), x.shape[0], x.shape[1], _stream(x)),
+        "ce_compact",
+    )
+
+
+@torch.library.custom_op("coda_b200::ce_scatter_out", mutates_args=("dx",), device_types="cuda")
+def _ce_scatter_out(rows: Tensor, position: Tensor, dx: Tensor) -> None:
+    check(lib.coda_b200_ce_scatter(rows.data_ptr(), position.data_ptr(), dx.data_ptr(), rows.shape[0], rows.shape[1], _stream(rows)), "ce_scatter")
+
+
+@torch.library.custom_op("coda_b200::gemm_live_out", mutates_args=("out",), device_types="cuda")
+def _gemm_live_out(grad: Tensor, n: int, B: Tensor, C: Optional[Tensor], alpha: Tensor, live: Tensor, along_depth: bool, out: Tensor) -> None:
+    """``grad[:, :n] @ B`` over the counted rows, or ``grad[:, :n]^T @ B`` summed over them."""
+    M, N = grad.shape[0], B.shape[1]
+    check(
+        lib.coda_b200_gemm_live(grad.data_ptr(), grad.shape[1], B.data_ptr(), N, _ptr(C), out.data_ptr(), N, int(out.dtype == torch.float32),
+                                alpha.data_ptr(), live.data_ptr(), int(along_depth), n if along_depth else M, N, M if along_depth else n,
+                                status_word(B.device).data_ptr(), _stream(B)),
+        "gemm_live",
+    )
+
+
+for _op in (_ce_loss_out, _gemm_softmax_grad_out, _ce_compact_out, _ce_scatter_out, _gemm_live_out):
     _op.register_fake(_noop_fake)
 
 
@@ -69,22 +100,36 @@ def _require_ce(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int) ->
     _require(-(2**31) <= ignore_index < 2**31, "ignore_index must fit int32")
 
 
-def ce_pieces_forward(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, mean: bool) -> tuple[Tensor, Tensor, Tensor]:
-    """``(loss, inv_count, lse)``; nothing of size ``[M, V]`` is written."""
+def _compacts(M: int, V: int, K: int) -> bool:
+    # (a traced caller keeps all rows: the library cannot be asked there)
+    return M > 0 and not torch.compiler.is_compiling() and bool(lib.coda_b200_ce_compacts(M, V, K))
+
+
+def ce_pieces_forward(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, mean: bool):
+    """``(loss, inv_count, lse, rows, labels, position, live)``; nothing of size ``[M, V]`` is written.  ``rows`` and ``labels``
+    are ``x`` and ``target``, or, where that pays, the rows that count put first (``live`` of them, from ``position``)."""
     _require_ce(x, weight, target, ignore_index)
     ops._debug_check_targets(target, weight.shape[0], ignore_index)
     M = x.shape[0]
     f32 = dict(dtype=torch.float32, device=x.device)
     if M == 0:  # a sum over nothing, and 0 / 0
-        return torch.full((), float("nan") if mean else 0.0, **f32), torch.full((), float("inf") if mean else 1.0, **f32), torch.empty(0, **f32)
+        return (torch.full((), float("nan") if mean else 0.0, **f32), torch.full((), float("inf") if mean else 1.0, **f32),
+                torch.empty(0, **f32), x, target, None, None)
+    position = live = None
+    if _compacts(M, weight.shape[0], x.shape[1]):
+        rows, labels, position = torch.empty_like(x), torch.empty_like(target), torch.empty_like(target)
+        live = torch.empty(1, dtype=torch.int32, device=x.device)
+        _ce_compact_out(x, target, ignore_index, position, labels, live, rows)
+        x, target = rows, labels
     parts = torch.empty(2 * M * lse_tiles(weight.shape[0]) + 2 * M, **f32)
     lse, loss, inv_count = torch.empty(M, **f32), torch.empty((), **f32), torch.empty((), **f32)
-    _ce_loss_out(x, weight, target, ignore_index, mean, parts, lse, loss, inv_count)
-    return loss, inv_count, lse
+    _ce_loss_out(x, weight, target, ignore_index, mean, live, parts, lse, loss, inv_count)
+    return loss, inv_count, lse, x, target, position, live
 
 
-def ce_pieces_backward(dloss: Tensor, inv_count: Tensor, lse: Tensor, x: Tensor, weight: Tensor, target: Tensor, ignore_index: int,
-                       piece: int, need_dx: bool, need_dw: bool) -> tuple[Optional[Tensor], Optional[Tensor]]:
+def ce_pieces_backward(dloss: Tensor, inv_count: Tensor, lse: Tensor, x: Tensor, weight: Tensor, target: Tensor, position: Optional[Tensor],
+                       live: Optional[Tensor], ignore_index: int, piece: int, need_dx: bool,
+                       need_dw: bool) -> tuple[Optional[Tensor], Optional[Tensor]]:
     """Gradients from one ``[M, piece]`` buffer: per piece of the vocabulary its softmax gradient ``g`` (the logits are
     computed again), its rows of ``dweight = alpha g^T x``, and ``dx += alpha g @ weight`` in fp32."""
     M, K = x.shape
@@ -100,10 +145,22 @@ def ce_pieces_backward(dloss: Tensor, inv_count: Tensor, lse: Tensor, x: Tensor,
     for c0 in range(0, V, width):
         n = min(width, V - c0)
         w = weight[c0:c0 + n]
-        _gemm_softmax_grad_out(x, w, lse, target, ignore_index, c0, g)
-        gp = g[:, :n]
-        if need_dw:
-            gemm(gp.mT, x, out=dw[c0:c0 + n], alpha=alpha)
-        if need_dx:
-            gemm(gp, w, out=dx32 if c0 + n < V else dx, alpha=alpha, C=dx32 if c0 > 0 else None)
+        _gemm_softmax_grad_out(x, w, lse, target, ignore_index, c0, live, g)
+        sum_so_far = dx32 if c0 > 0 else None
+        if live is None:
+            gp = g[:, :n]
+            if need_dw:
+                gemm(gp.mT, x, out=dw[c0:c0 + n], alpha=alpha)
+            if need_dx:
+                gemm(gp, w, out=dx32 if c0 + n < V else dx, alpha=alpha, C=sum_so_far)
+        else:
+            if need_dw:
+                _gemm_live_out(g, n, x, None, alpha, live, True, dw[c0:c0 + n])
+            if need_dx and c0 == 0 and lib.coda_b200_gemm_workspace_bytes(M, K, n) > 0:  # few tiles, cut along the contraction: all rows
+                gemm(g[:, :n], w, out=dx32 if n < V else dx, alpha=alpha)
+            elif need_dx:
+                _gemm_live_out(g, n, w, sum_so_far, alpha, live, False, dx32 if c0 + n < V else dx)
+    if need_dx and live is not None:
+        rows, dx = dx, torch.empty_like(dx)
+        _ce_scatter_out(rows, position, dx)
     return dx, dw

@@ -50,7 +50,8 @@ const char* coda_b200_last_error(void);
  * (1 = epilogues stage output tiles in shared memory and write them with TMA
  * stores, the default; 0 = per-thread 16-byte stores), "split_tail" (1 = a plain
  * GEMM that is given a workspace may cut the tiles of its last round along K, the
- * default; 0 = never: see coda_b200_gemm_ws).  Options are
+ * default; 0 = never: see coda_b200_gemm_ws), "ce_compact" (1 = coda_b200_ce_compacts
+ * may answer yes, the default; 0 = never).  Options are
  * process-wide atomics: a launch reads them once at its start, so changing one
  * from another host thread is safe and affects later launches only.
  * "probe_ld_kb" / "probe_st_kb" (0 = off) are a measurement aid: KB of extra
@@ -399,20 +400,40 @@ int coda_b200_gemm_e4m3(const void* A, const float* a_scale, const void* B, cons
                         int d_is_fp32, int M, int N, int K, void* workspace, int64_t workspace_bytes, int* dev_status,
                         void* stream);
 
-/* Cross entropy of the logits A @ B over all N columns (any N), storing none of them: lse fp32 [M], losses fp32 [M] (zero
- * in ignored rows, NaN for a label outside [0, N)), and the scalars loss = inv_count * sum(losses) and inv_count
+/* Cross entropy of the logits A @ B over all N columns (any N), storing none of them: lse fp32 [M], losses fp32 [M] (both
+ * zero in ignored rows; NaN loss for a label outside [0, N)), and the scalars loss = inv_count * sum(losses) and inv_count
  * (1 / rows that are not ignored with `mean`, else 1).  part_max / part_sum fp32 [M, coda_b200_lse_tiles(N)] and
- * target_logit fp32 [M] are workspace. */
+ * target_logit fp32 [M] are workspace.  `live` (device int32, or NULL): see coda_b200_ce_compact. */
 int coda_b200_ce_loss(const void* A, int64_t a_stride_m, int64_t a_stride_k, const void* B, int64_t b_stride_k,
-                      int64_t b_stride_n, const int32_t* target, int ignore_index, int mean, float* part_max, float* part_sum,
-                      float* target_logit, float* lse, float* losses, float* loss, float* inv_count, int M, int N, int K,
-                      int* dev_status, void* stream);
+                      int64_t b_stride_n, const int32_t* target, int ignore_index, int mean, const int32_t* live, float* part_max,
+                      float* part_sum, float* target_logit, float* lse, float* losses, float* loss, float* inv_count, int M,
+                      int N, int K, int* dev_status, void* stream);
 
 /* G[r, j] = exp(z_rj - lse[r]) - (col0 + j == target[r]) in bf16 for the logits z = A @ B of one piece of the vocabulary
- * (N columns, the first of which is column col0 of the whole), zero in ignored rows.  ldg: a multiple of 8, >= N. */
+ * (N columns, the first of which is column col0 of the whole), zero in ignored rows.  ldg: a multiple of 8, >= N.  With `live`
+ * the rows behind the counted ones are written as zeros up to the next multiple of 64, and not at all beyond. */
 int coda_b200_gemm_softmax_grad(const void* A, int64_t a_stride_m, int64_t a_stride_k, const void* B, int64_t b_stride_k,
-                                int64_t b_stride_n, const float* lse, const int32_t* target, int ignore_index, int col0, void* G,
-                                int64_t ldg, int M, int N, int K, int* dev_status, void* stream);
+                                int64_t b_stride_n, const float* lse, const int32_t* target, int ignore_index, int col0,
+                                const int32_t* live, void* G, int64_t ldg, int M, int N, int K, int* dev_status, void* stream);
+
+/* Leaving ignored rows out of the products.  coda_b200_ce_compact puts the rows of x [M, K] (dense bf16) that count first, in
+ * their order: rows [M, K], labels int32 [M] (ignore_index behind them), position int32 [M] (where a row went, -1: ignored) and
+ * live, a device int32: how many count.  Row operands are zero from there to the next multiple of 64 and undefined beyond.
+ * coda_b200_ce_loss and coda_b200_gemm_softmax_grad then take rows, labels and live for x, target and NULL;
+ * coda_b200_gemm_live is the product behind them, and coda_b200_ce_scatter puts rows back: dx[i] = rows[position[i]], or zero.
+ * No count is read by the host.  coda_b200_ce_compacts says whether the products are large enough for it to pay (with cta_group
+ * 2, which these products need). */
+int coda_b200_ce_compacts(int M, int N, int K);
+int coda_b200_ce_compact(const void* x, const int32_t* target, int ignore_index, int32_t* position, int32_t* labels, int32_t* live,
+                         void* rows, int M, int K, void* stream);
+int coda_b200_ce_scatter(const void* rows, const int32_t* position, void* dx, int M, int K, void* stream);
+
+/* along_depth 0: D[m, n] = alpha * sum_k A[m, k] * B[k, n] + C[m, n] for the first *live rows (A [M, K], B [K, N], all row-major);
+ * along_depth 1: D[m, n] = alpha * sum_k A[k, m] * B[k, n] (+ C) over the first *live k (A [K, M], B [K, N] row-major).
+ * *live is rounded up to a multiple of 64 (at most M, or K).  C is fp32 with D's leading dimension, or NULL; it may be D. */
+int coda_b200_gemm_live(const void* A, int64_t lda, const void* B, int64_t ldb, const float* C, void* D, int64_t ldd,
+                        int d_is_fp32, const float* alpha, const int32_t* live, int along_depth, int M, int N, int K,
+                        int* dev_status, void* stream);
 
 #ifdef __cplusplus
 }

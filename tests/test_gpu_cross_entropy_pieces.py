@@ -103,11 +103,11 @@ def test_masks_that_leave_nothing(ck):
     t[:] = -100
     loss = ck.linear_cross_entropy_pieces(x, w, t, reduction="sum", piece=100)
     dx, dw = torch.autograd.grad(loss, (x, w))
-    assert float(loss) == 0.0 and not bool(dx.any()) and not bool(dw.any())
+    assert float(loss.detach()) == 0.0 and not bool(dx.any()) and not bool(dw.any())
     assert bool(ck.linear_cross_entropy_pieces(x, w, t).isnan())
     empty = ck.linear_cross_entropy_pieces(x[:0], w, t[:0], reduction="sum")
     dx, dw = torch.autograd.grad(empty, (x, w), allow_unused=True)
-    assert float(empty) == 0.0 and not bool(dw.any())
+    assert float(empty.detach()) == 0.0 and not bool(dw.any())
     assert bool(ck.linear_cross_entropy_pieces(x[:0], w, t[:0]).isnan())
 
 
@@ -236,3 +236,101 @@ def test_second_derivative_is_refused(ck):
     x, w, t = make(20, 64, 300)
     with pytest.raises(RuntimeError, match="once"):
         torch.autograd.grad(ck.linear_cross_entropy_pieces(x, w, t), x, create_graph=True)
+
+
+# ------------------------------------------------------------------------------------------------ ignored rows left out
+# Large enough for the rows that count to be put together first (2 M V K >= 5e10, V >= 8192).
+def large(M=1500, K=2048, V=8195, **kw):
+    from coda_kernels_b200._lib import lib
+
+    assert lib.coda_b200_ce_compacts(M, V, K) == 1
+    return make(M, K, V, **kw)
+
+
+@pytest.mark.parametrize("ignored", [0.0, 0.05, 0.6, 0.99])
+@pytest.mark.parametrize("M,K,V,piece", [(1500, 2048, 8195, 3000), (65, 4096, 100003, None), (4100, 776, 8200, None)])
+def test_counted_rows_against_the_definition(ck, M, K, V, piece, ignored):
+    x, w, t = large(M, K, V, ignored=ignored)
+    loss = ck.linear_cross_entropy_pieces(x, w, t, piece=piece)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    check(x, w, t, loss, dx, dw, "mean")
+    assert not bool(dx[t == -100].any())
+    with torch.no_grad():
+        assert torch.equal(loss, ck.linear_cross_entropy_pieces(x, w, t))
+    ck.ops.check_device_status(torch.device(DEV))
+
+
+@pytest.mark.parametrize("kept", [[], [0], [1499], list(range(64)), list(range(700, 765)), list(range(0, 1500, 7))])
+def test_counted_rows_at_the_edges(ck, kept):
+    x, w, t = large(ignored=0.0)
+    mask = torch.ones(1500, dtype=torch.bool, device=DEV)
+    mask[kept] = False
+    t = torch.where(mask, torch.full_like(t, -100), t)
+    loss = ck.linear_cross_entropy_pieces(x, w, t, reduction="sum", piece=3000)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    check(x, w, t, loss, dx, dw, "sum")
+    if not kept:
+        assert float(loss.detach()) == 0.0 and not bool(dx.any()) and not bool(dw.any())
+
+
+def test_ignored_rows_are_not_read_by_the_products(ck):
+    x, w, t = large(ignored=0.3)
+    clean = ck.linear_cross_entropy_pieces(x, w, t, piece=5000)
+    grads = torch.autograd.grad(clean, (x, w))
+    bad = x.detach().clone()
+    bad[t == -100] = float("nan")
+    bad.requires_grad_(True)
+    loss = ck.linear_cross_entropy_pieces(bad, w, t, piece=5000)
+    assert torch.equal(loss, clean)
+    for a, b in zip(torch.autograd.grad(loss, (bad, w)), grads):
+        assert torch.equal(a, b)
+
+
+def test_counted_rows_follow_the_labels_of_a_replay(ck):
+    """The number of rows that count is read on the device: a captured step takes other masks than it was captured with."""
+    x, w, t = large(ignored=0.5)
+
+    def step():
+        loss = ck.linear_cross_entropy_pieces(x, w, t, piece=3000)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = step()
+    for seed, ignored in ((5, 0.0), (6, 0.95), (7, 0.2)):
+        _, _, t2 = large(ignored=ignored, seed=seed)
+        t.copy_(t2)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(static, step()):
+            assert torch.equal(a, b)
+
+
+def test_counted_rows_in_both_bindings_and_with_partial_gradients(ck):
+    from importlib import import_module
+
+    node = import_module("coda_kernels_b200.functional.cross_entropy_pieces").LinearCrossEntropyPieces
+    x, w, t = large(ignored=0.3)
+    loss = ck.linear_cross_entropy_pieces(x, w, t, piece=5000)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    other = node.apply(x, w, t, -100, "mean", 5000)
+    for a, b in zip((loss, dx, dw), (other, *torch.autograd.grad(other, (x, w)))):
+        assert torch.equal(a, b)
+    (only_x,) = torch.autograd.grad(ck.linear_cross_entropy_pieces(x, w.detach(), t, piece=5000), x)
+    (only_w,) = torch.autograd.grad(ck.linear_cross_entropy_pieces(x.detach(), w, t, piece=5000), w)
+    assert torch.equal(only_x, dx) and torch.equal(only_w, dw)
+    # with one CTA a tile, or by option, all rows take part: the definition decides
+    for option, value, default in (("cta_group", 1, 2), ("ce_compact", 0, 1)):
+        ck.set_option(option, value)
+        try:
+            loss = ck.linear_cross_entropy_pieces(x, w, t, piece=5000)
+            grads = torch.autograd.grad(loss, (x, w))
+            torch.cuda.synchronize()
+        finally:
+            ck.set_option(option, default)
+        check(x, w, t, loss, *grads, "mean")

@@ -47,9 +47,32 @@ def test_c_entries_refuse_on_the_host():
     refused(lib.coda_b200_gemm_e4m3(p, p, p, p, p, 16, 0, 0, 16, 32, None, 0, p, None), b"positive")
     refused(lib.coda_b200_gemm_e4m3(p, p, p, p, p, 16, 0, 4, 16, 32, p + 4, 64, p, None), b"16-byte")
     assert lib.coda_b200_gemm_e4m3_workspace_bytes(50, 6144, 4096) > 0 == lib.coda_b200_gemm_e4m3_workspace_bytes(1, 6144, 4096)
-    refused(lib.coda_b200_gemm_softmax_grad(p, 64, 1, p, 1, 64, p, p, -100, 0, p, 12, 4, 12, 64, p, None), b"ldg")
-    refused(lib.coda_b200_gemm_softmax_grad(p, 64, 1, p, 1, 64, p, p, -100, -1, p, 16, 4, 12, 64, p, None), b"col0")
-    refused(lib.coda_b200_ce_loss(p, 60, 1, p, 1, 60, p, -100, 1, p, p, p, p, p, p, p, 4, 12, 60, p, None), b"K must")
+    refused(lib.coda_b200_gemm_softmax_grad(p, 64, 1, p, 1, 64, p, p, -100, 0, None, p, 12, 4, 12, 64, p, None), b"ldg")
+    refused(lib.coda_b200_gemm_softmax_grad(p, 64, 1, p, 1, 64, p, p, -100, -1, None, p, 16, 4, 12, 64, p, None), b"col0")
+    refused(lib.coda_b200_ce_loss(p, 60, 1, p, 1, 60, p, -100, 1, None, p, p, p, p, p, p, p, 4, 12, 60, p, None), b"K must")
+
+
+def test_products_of_counted_rows_refuse_on_the_host():
+    from coda_kernels_b200 import _lib
+
+    lib, p = _lib.lib, 1 << 20
+
+    def refused(rc, text):
+        assert rc in (-1, -2) and text in lib.coda_b200_last_error(), (rc, lib.coda_b200_last_error())
+
+    assert lib.coda_b200_ce_compacts(8192, 128256, 4096) == 1 and lib.coda_b200_ce_compacts(256, 8000, 512) == 0
+    refused(lib.coda_b200_ce_compact(p, p, -100, p, p, None, p, 4, 64, None), b"NULL")
+    refused(lib.coda_b200_ce_compact(p, p, -100, p, p, p, p, 4, 60, None), b"multiple of 8")
+    refused(lib.coda_b200_ce_scatter(p + 4, p, p, 4, 64, None), b"16-byte")
+    refused(lib.coda_b200_gemm_live(p, 64, p, 64, None, p, 64, 0, None, None, 0, 4, 64, 64, p, None), b"NULL")
+    refused(lib.coda_b200_gemm_live(p, 64, p, 60, None, p, 60, 0, None, p, 0, 4, 60, 64, p, None), b"multiples of 8")
+    refused(lib.coda_b200_gemm_live(p, 56, p, 64, None, p, 64, 0, None, p, 0, 4, 64, 64, p, None), b"leading")
+    refused(lib.coda_b200_gemm_softmax_grad(p, 1, 64, p, 1, 64, p, p, -100, 0, p, p, 16, 64, 16, 64, p, None), b"contiguous along")
+    assert lib.coda_b200_set_option(b"cta_group", 1) == 0
+    try:
+        assert lib.coda_b200_ce_compacts(8192, 128256, 4096) == 0
+    finally:
+        assert lib.coda_b200_set_option(b"cta_group", 2) == 0
 
 
 def test_cpu_tensors_are_refused():
