@@ -261,7 +261,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
   using Cfg = GemmCfg<kCtaGroup, kBN, Epi::kLoadRingBytes, Pro::kStageExtraBytes>;
   constexpr bool kProlog = Pro::kWarps > 0;
   static_assert(!kProlog || !kAMn, "transform warps build a K-major A tile");
-  static_assert(!Pro::kE4M3 || (!kAMn && !kBMn), "e4m3 operands are K-major");
+  static_assert(!Pro::kE4M3 || (!kAMn && !kBMn && kCtaGroup == 2), "e4m3 operands are K-major and worked on by pairs");
   constexpr int kStages = Cfg::kStages;
   constexpr int kBNcta = Cfg::kBNcta;
   constexpr uint32_t kABytes = Cfg::kABytes;
@@ -429,7 +429,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
           for (int k = 0; k < kBlockK / kUmmaK; ++k) {
             const uint64_t adesc = make_smem_desc(a_addr + k * a_step, a_lbo, a_sbo);
             const uint64_t bdesc = make_smem_desc(b_addr + k * b_step, b_lbo, b_sbo);
-            if constexpr (Pro::kE4M3) umma_f8<kCtaGroup>(d_tmem, adesc, bdesc, idesc, (kb != w.kb0 || k != 0) ? 1u : 0u);
+            if constexpr (Pro::kE4M3) umma_e4m3_pair(d_tmem, adesc, bdesc, idesc, (kb != w.kb0 || k != 0) ? 1u : 0u);
             else umma_bf16<kCtaGroup>(d_tmem, adesc, bdesc, idesc, (kb != w.kb0 || k != 0) ? 1u : 0u);
           }
           umma_commit<kCtaGroup>(bar_empty + 8 * s);  // frees the stage (in both CTAs) once these MMAs retire

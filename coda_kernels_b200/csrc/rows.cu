@@ -328,7 +328,7 @@ __device__ __forceinline__ void row_reduce(float& a, float& b, float* red, int& 
 // A stream of chunks of the whole matrix, drop_unroll() of them in flight a thread, by four blocks an SM (eight: 158 instead of
 // 147 us for 16384 x 14336 bf16 without a mask; 32 bytes a thread suffice, a second fp32 chunk costs 52 instead of 43 us at 8192
 // x 4096).  Without the mask, and in fp32, bound by HBM (6.2 to 6.4 TB/s).  With it a 2-byte type is bound by the integer
-// multiplier, 19 wide products for 4 elements: 233 us, one element a nanosecond, whatever the occupancy.
+// multiplier, 19 wide products for 4 elements: 225 us, one element a nanosecond, whatever the occupancy.
 constexpr int kDropThreads = 256, kDropBlocksPerSm = 4;
 constexpr int drop_unroll(int elem_bytes) { return elem_bytes == 4 ? 1 : 2; }
 template <typename T, bool kShift, bool kDrop>
