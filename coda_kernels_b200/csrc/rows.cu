@@ -407,12 +407,21 @@ dropout_kernel(const T* __restrict__ x, T* __restrict__ out, long long total, lo
 // and written.  A thread stays on the same columns for all of its rows (kShift: the grid's row stride is a multiple of 8, so
 // `off` stays too), so the weights are loaded once.
 constexpr int kWarpBlock = 256, kMaxThreads = 512;
-// Registers a thread, and so threads an SM.  Forward: two chunks of a 2-byte type fit 64; fp32 chunks and the shift's masks
-// take 80, four chunks 128.  Backward: with sums and the next row's loads two chunks of a 2-byte type take 128 (16384 x
-// 4096 bf16: 96 us; 102 us with 80 registers and no loads ahead, 133 us with 96 registers and loads ahead); fp32, which loads
-// nothing ahead, takes 96 (16384 x 4096: 203 us, 128: 236 us), but 128 with dropout (8192 x 8192: 220 us, 96: 255 us).
-constexpr int fwd_regs(int elem_bytes, bool shift, int chunks) { return chunks == 4 ? 128 : (elem_bytes == 4 || shift) ? 80 : 64; }
-constexpr int bwd_regs(int elem_bytes, bool shift, bool drop) { return shift ? 80 : elem_bytes == 4 && !drop ? 96 : 128; }
+// Registers a thread, and so threads an SM.  Forward: two chunks of a 2-byte type fit 64, of fp32 80; four chunks take 128.
+// Backward: with sums and the next row's loads two chunks of a 2-byte type take 128 (16384 x 4096 bf16: 96 us; 102 us with 80
+// registers and no loads ahead, 133 us with 96 registers and loads ahead); fp32, which loads nothing ahead, takes 96 (16384 x
+// 4096: 203 us, 128: 236 us), but 128 with dropout (8192 x 8192: 220 us, 96: 255 us).  With the shift 96 (16384 x 4095 bf16, forward,
+// backward, e4m3: 96, 155 and 107 us; with 80 105, 191 and 121 us), but 80 for one chunk a thread (300000 x 129: 98 and 133 us;
+// with 96 114 and 164 us) and for fp32 forward (16384 x 2047: 89 us, 96: 105 us).
+constexpr int fwd_regs(int elem_bytes, bool shift, int chunks, bool e4m3) {
+  if (chunks == 4) return 128;
+  if (shift) return chunks == 1 || (elem_bytes == 4 && !e4m3) ? 80 : 96;
+  return elem_bytes == 4 ? 80 : 64;
+}
+constexpr int bwd_regs(int elem_bytes, bool shift, bool drop, int chunks) {
+  if (shift) return chunks == 1 ? 80 : 96;
+  return elem_bytes == 4 && !drop ? 96 : 128;
+}
 constexpr int threads_per_sm(int regs) { return 512 / regs * 4 * 32; }  // whole warps in each quarter of the SM
 
 template <int kLanes>
@@ -430,7 +439,7 @@ struct RowLoop {
 };
 
 template <typename T, bool kShift, bool kDrop, int kLanes, int kChunks, bool kE4M3>
-__global__ void __maxnreg__(fwd_regs(sizeof(T), kShift, kChunks))
+__global__ void __maxnreg__(fwd_regs(sizeof(T), kShift, kChunks, kE4M3))
 norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T* __restrict__ weight, float eps, Dropout d,
                 long long* __restrict__ used, T* __restrict__ h, T* __restrict__ out, float* __restrict__ rstd,
                 __nv_fp8_e4m3* __restrict__ q, float* __restrict__ scale, long long rows, int cols) {
@@ -518,7 +527,7 @@ norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T
 // Bound by HBM, and laid out as the forward; dw is summed in registers over a thread's rows and leaves as one partial row a
 // block, which fold_rows_kernel adds in a fixed order.
 template <typename T, bool kShift, bool kDrop, int kLanes, int kChunks>
-__global__ void __maxnreg__(bwd_regs(sizeof(T), kShift, kDrop))
+__global__ void __maxnreg__(bwd_regs(sizeof(T), kShift, kDrop, kChunks))
 norm_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* __restrict__ h, const float* __restrict__ rstd,
                 const T* __restrict__ weight, Dropout d, T* __restrict__ dx, T* __restrict__ dres, float* __restrict__ partial,
                 long long rows, int cols) {
@@ -845,7 +854,7 @@ struct RowPlan {
   int lanes, chunks, threads;
   int64_t grid;
 };
-inline RowPlan row_plan(int64_t rows, int64_t cols, int dtype, bool backward, bool drop) {
+inline RowPlan row_plan(int64_t rows, int64_t cols, int dtype, bool backward, bool drop, bool e4m3 = false) {
   RowPlan p;
   p.shift = cols % 8 != 0;
   const int64_t n = (cols + (p.shift ? 14 : 7)) / 8;  // chunks a row may touch
@@ -853,7 +862,7 @@ inline RowPlan row_plan(int64_t rows, int64_t cols, int dtype, bool backward, bo
   p.chunks = n <= 32 ? 1 : n <= 2 * kMaxThreads ? 2 : n <= 4 * kMaxThreads && !backward ? 4 : 0;
   p.threads = p.chunks == 1 ? kWarpBlock : p.chunks == 0 ? kLongThreads : static_cast<int>((n + 32 * p.chunks - 1) / (32 * p.chunks) * 32);
   const int64_t per_block = p.lanes != 0 ? kWarpBlock / p.lanes : 1, need = (rows + per_block - 1) / per_block;
-  const int elem = dtype == 2 ? 4 : 2, regs = backward ? bwd_regs(elem, p.shift, drop) : fwd_regs(elem, p.shift, p.chunks);
+  const int elem = dtype == 2 ? 4 : 2, regs = backward ? bwd_regs(elem, p.shift, drop, p.chunks) : fwd_regs(elem, p.shift, p.chunks, e4m3);
   const int fit = p.chunks == 0 ? (backward && cols > kSharedCols / 2 && cols <= kSharedCols ? 1 : 2) : threads_per_sm(regs) / p.threads;
   const int64_t cap = std::max(static_cast<int64_t>(sm_count()) * std::min(std::max(fit, 1), 32) / 8, int64_t{1}) * 8;  // kShift: rows advance by multiples of 8
   p.grid = std::min(need, cap);
@@ -901,7 +910,7 @@ int by_shape(const RowPlan& p, F&& f) {
 template <bool kE4M3>
 int launch_norm_fwd(const void* x, const void* residual, const void* weight, float eps, const Dropout& d, int64_t* used, void* h, void* out,
                     float* rstd, void* q, float* scale, int64_t rows, int64_t cols, int dtype, void* stream) {
-  const RowPlan plan = row_plan(rows, cols, dtype, false, d.rng != nullptr);
+  const RowPlan plan = row_plan(rows, cols, dtype, false, d.rng != nullptr, kE4M3);
   return by_dtype(dtype, [&](auto t) {
     return by_flag(plan.shift, [&](auto shift) {
       return by_flag(!kE4M3 && d.rng != nullptr, [&](auto drop) {
