@@ -135,17 +135,18 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// The scale of a row of e4m3 values, and what divides by it.  The quotient has to be the correctly rounded one: values of
-// a 2-byte type lie exactly between two e4m3 values all the time (with max|y| = 21 / 8, say, where y / scale = 512 y / 3),
-// and a quotient one step off moves them all to the same side.  A division for every element made the kernel slower than its
-// memory traffic, though.  So: with inv = 1 / s rounded correctly and q = v inv, the residual v - q s is exact in an fma, and
-// q + residual * inv is v / s rounded correctly (Markstein, "Computation of elementary functions on the IBM RISC System/6000
-// processor", 1990; quantize 16384 x 4096 bf16: 44 us, 41 us with q alone).  Where the residual falls below the smallest fp32,
-// |v| < 2^-100, the last bit may be lost.
+// The scale of a row of e4m3 values, and what divides by it.  Both quotients have to be the correctly rounded ones: values of
+// a 2-byte type lie exactly between two e4m3 values all the time (with max|y| = 21 / 8, say, where the scale is 3 / 512 and
+// y / scale = 512 y / 3), and a scale or a quotient one step off moves them all to the same side (fp32's 1 / 448 is too large:
+// a product with it is one step off in every other row whose maximum is a multiple of 7).  A division for every element made the
+// kernel slower than its memory traffic, though.  So: with inv = 1 / s rounded correctly and q = v inv, the residual v - q s
+// is exact in an fma, and q + residual * inv is v / s rounded correctly (Markstein, "Computation of elementary functions on
+// the IBM RISC System/6000 processor", 1990; quantize 16384 x 4096 bf16: 44 us, 41 us with q alone).  Where the residual falls
+// below the smallest fp32, |v| < 2^-100, the last bit may be lost.
 struct RowScale {
   float scale, inv, s;  // s: the scale, or 0 if that is infinite, so that finite values over it come out as 0
   __device__ explicit RowScale(float top)
-      : scale(max_nan(top * (1.0f / 448.0f), 1.17549435e-38f)), inv(1.0f / scale), s(isinf(scale) ? 0.0f : scale) {}
+      : scale(max_nan(top / 448.0f, 1.17549435e-38f)), inv(1.0f / scale), s(isinf(scale) ? 0.0f : scale) {}
   __device__ float over(float v) const {
     const float q = v * inv;
     return fmaf(fmaf(-q, s, v), inv, q);

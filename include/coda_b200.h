@@ -384,8 +384,8 @@ int coda_b200_add_rmsnorm_bwd(const void* dout, const void* dh, const void* h, c
                               int64_t scratch_bytes, int64_t rows, int64_t cols, int dtype, void* stream);
 
 /* Rows as e4m3 values with one fp32 scale each: y = residual + x, normalised and weighted as above when weight != NULL
- * (residual and h may be NULL; h receives residual + x); scale = max(max|y| / 448, 2^-126), with / 448 as the product
- * with the fp32 reciprocal, and q = y / scale, the quotient rounded to fp32 and then to e4m3 (ties to even).
+ * (residual and h may be NULL; h receives residual + x); scale = max(max|y| / 448, 2^-126) and q = y / scale, both
+ * quotients rounded to fp32, the second then to e4m3 (ties to even).
  * A row that holds NaN gets the scale NaN. */
 int coda_b200_rows_e4m3(const void* x, const void* residual, const void* weight, float eps, void* h, void* q, float* scale,
                         int64_t rows, int64_t cols, int dtype, void* stream);
