@@ -67,10 +67,16 @@ __global__ void __launch_bounds__(1024) ce_total_kernel(const float* __restrict_
       s += sums[i];
       n += counts[i];
     }
-    const float inv = mean ? 1.0f / static_cast<float>(n) : 1.0f;
-    *loss = s * inv;
+    // the mean over nothing is NaN, and nothing depends on anything
+    const float inv = n == 0 ? 0.0f : mean ? 1.0f / static_cast<float>(n) : 1.0f;
+    *loss = n == 0 && mean ? NAN : s * inv;
     *inv_count = inv;
   }
+}
+
+// What the gradients' products are multiplied by: zero where no row counts, whatever dloss is (1 / 0 behind a sum of nothing).
+__global__ void ce_alpha_kernel(const float* __restrict__ dloss, const float* __restrict__ inv_count, float* __restrict__ alpha) {
+  *alpha = *inv_count == 0.0f ? 0.0f : *dloss * *inv_count;
 }
 
 // ------------------------------------------------------------------ the rows that count
@@ -238,6 +244,12 @@ extern "C" int coda_b200_ce_loss(const void* A, int64_t a_stride_m, int64_t a_st
   if (rc != kOk) return rc;
   ce_total_kernel<<<1, 1024, 0, st>>>(losses, target, ignore_index, mean, loss, inv_count, M);
   return launch_check("cross-entropy total launch");
+}
+
+extern "C" int coda_b200_ce_alpha(const float* dloss, const float* inv_count, float* alpha, void* stream) {
+  if (!dloss || !inv_count || !alpha) return fail(kBadArgument, "NULL pointer");
+  ce_alpha_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(dloss, inv_count, alpha);
+  return launch_check("cross-entropy factor launch");
 }
 
 extern "C" int coda_b200_gemm_softmax_grad(const void* A, int64_t a_stride_m, int64_t a_stride_k, const void* B, int64_t b_stride_k,

@@ -571,7 +571,7 @@ std::tuple<Tensor, Tensor, Tensor> run_ce(const CeRows& r, const Tensor& weight,
   const int64_t M = x.size(0), V = weight.size(0), K = x.size(1);
   const auto f32 = x.options().dtype(at::kFloat);
   if (M == 0)  // a sum over nothing, and 0 / 0
-    return {at::full({}, mean ? NAN : 0.0, f32), at::full({}, mean ? INFINITY : 1.0, f32), at::empty({0}, f32)};
+    return {at::full({}, mean ? NAN : 0.0, f32), at::zeros({}, f32), at::empty({0}, f32)};
   const int64_t tiles = coda_b200_lse_tiles(static_cast<int>(V));
   Tensor parts = at::empty({2 * M * tiles + 2 * M}, f32), lse = at::empty({M}, f32), loss = at::empty({}, f32), inv_count = at::empty({}, f32);
   float* part = parts.data_ptr<float>();
@@ -597,7 +597,9 @@ OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tens
     return {dx, dw};
   }
   const Tensor xs = x.as_strided({M, K}, {K, 1}), ws = weight.as_strided({V, K}, {K, 1});
-  const OptTensor alpha = (dloss * inv_count).reshape({1}).to(at::kFloat);
+  const Tensor dl = dloss.to(at::kFloat);
+  const OptTensor alpha = at::empty({1}, inv_count.options());
+  check(coda_b200_ce_alpha(dl.data_ptr<float>(), inv_count.data_ptr<float>(), alpha->data_ptr<float>(), stream_of(x)), "ce_alpha");
   const int32_t* live = live_ptr(r.live);
   const int64_t width = std::min(piece, V), ldg = (width + 7) / 8 * 8;
   Tensor g = new_matrix(x, M, ldg, at::kBFloat16);

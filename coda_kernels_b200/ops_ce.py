@@ -73,7 +73,12 @@ def _gemm_live_out(grad: Tensor, n: int, B: Tensor, C: Optional[Tensor], alpha: 
     )
 
 
-for _op in (_ce_loss_out, _gemm_softmax_grad_out, _ce_compact_out, _ce_scatter_out, _gemm_live_out):
+@torch.library.custom_op("coda_b200::ce_alpha_out", mutates_args=("alpha",), device_types="cuda")
+def _ce_alpha_out(dloss: Tensor, inv_count: Tensor, alpha: Tensor) -> None:
+    check(lib.coda_b200_ce_alpha(dloss.data_ptr(), inv_count.data_ptr(), alpha.data_ptr(), _stream(alpha)), "ce_alpha")
+
+
+for _op in (_ce_loss_out, _ce_alpha_out, _gemm_softmax_grad_out, _ce_compact_out, _ce_scatter_out, _gemm_live_out):
     _op.register_fake(_noop_fake)
 
 
@@ -113,7 +118,7 @@ def ce_pieces_forward(x: Tensor, weight: Tensor, target: Tensor, ignore_index: i
     M = x.shape[0]
     f32 = dict(dtype=torch.float32, device=x.device)
     if M == 0:  # a sum over nothing, and 0 / 0
-        return (torch.full((), float("nan") if mean else 0.0, **f32), torch.full((), float("inf") if mean else 1.0, **f32),
+        return (torch.full((), float("nan") if mean else 0.0, **f32), torch.zeros((), **f32),
                 torch.empty(0, **f32), x, target, None, None)
     position = live = None
     if _compacts(M, weight.shape[0], x.shape[1]):
@@ -136,7 +141,8 @@ def ce_pieces_backward(dloss: Tensor, inv_count: Tensor, lse: Tensor, x: Tensor,
     V = weight.shape[0]
     if M == 0:
         return (torch.zeros_like(x) if need_dx else None), (torch.zeros_like(weight) if need_dw else None)
-    alpha = (dloss * inv_count).reshape(1).to(dtype=torch.float32)
+    alpha = torch.empty(1, dtype=torch.float32, device=x.device)
+    _ce_alpha_out(dloss.to(torch.float32), inv_count, alpha)
     width = min(piece, V)
     g = torch.empty(M, -(-width // 8) * 8, dtype=x.dtype, device=x.device)
     dx = torch.empty_like(x) if need_dx else None

@@ -1,0 +1,54 @@
+"""``linear_cross_entropy_pieces`` where labels are missing or wrong: gradients of a batch without a label, labels outside the
+vocabulary.  Each at a size whose products run over all rows and at one where the rows that count are put first, through the
+compiled operators and through the Python nodes."""
+
+from importlib import import_module
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+SIZES = [(40, 64, 300, 128), (1500, 2048, 8195, 3000)]  # rows, dim, vocabulary, piece: all rows; the rows that count
+
+
+@pytest.fixture(scope="module")
+def ck():
+    import coda_kernels_b200 as ck
+
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    return ck
+
+
+def make(M, K, V, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(M, K, generator=g).bfloat16().to(DEV).requires_grad_(True)
+    w = (torch.randn(V, K, generator=g) * K**-0.5).bfloat16().to(DEV).requires_grad_(True)
+    return x, w, torch.randint(0, V, (M,), generator=g, dtype=torch.int32).to(DEV)
+
+
+def loss_of(ck, binding):
+    if binding == "compiled":
+        return lambda x, w, t, reduction, piece: ck.linear_cross_entropy_pieces(x, w, t, reduction=reduction, piece=piece)
+    node = import_module("coda_kernels_b200.functional.cross_entropy_pieces").LinearCrossEntropyPieces
+    return lambda x, w, t, reduction, piece: node.apply(x, w, t, -100, reduction, piece)
+
+
+@pytest.mark.parametrize("binding", ["compiled", "python"])
+@pytest.mark.parametrize("M,K,V,piece", SIZES)
+def test_no_label_counts(ck, M, K, V, piece, binding):
+    """The mean over nothing is NaN, and its gradients are zeros, as those of torch's own cross entropy: a fully masked
+    micro-batch adds nothing to the accumulated gradients."""
+    assert ck._lib.lib.coda_b200_ce_compacts(M, V, K) == (M > 1000)
+    x, w, t = make(M, K, V)
+    loss = loss_of(ck, binding)(x, w, torch.full_like(t, -100), "mean", piece)
+    assert bool(loss.isnan())
+    dx, dw = torch.autograd.grad(loss, (x, w), torch.tensor(0.25, device=DEV))
+    assert torch.equal(dx, torch.zeros_like(dx)) and torch.equal(dw, torch.zeros_like(dw))
+    total = loss_of(ck, binding)(x, w, torch.full_like(t, -100), "sum", piece)
+    assert float(total.detach()) == 0.0
+    for g in torch.autograd.grad(total / 0.0, (x, w)):  # a sum divided by the number of labels
+        assert not bool(g.any())
+    logits = (x.detach().float() @ w.detach().float().T).requires_grad_(True)
+    torch.nn.functional.cross_entropy(logits, torch.full_like(t, -100).long()).backward()
+    assert not bool(logits.grad.any())  # what is meant by "as those of torch's own"
