@@ -31,10 +31,12 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const float* __restrict__ 
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane == 0) {
-    const float l = mx + logf(s);
+    // No tile has picked a logit for a label outside the vocabulary: its loss is NaN rather than a wrong number, and so is
+    // its log-sum-exp, which makes the row's gradient NaN.
+    const bool outside = t < 0 || t >= vocab;
+    const float l = outside ? NAN : mx + logf(s);
     lse[row] = l;
-    // no tile has picked a logit for a label outside the vocabulary: its loss is NaN rather than a wrong number
-    losses[row] = (t < 0 || t >= vocab) ? NAN : l - target_logit[row];
+    losses[row] = outside ? NAN : l - target_logit[row];
   }
 }
 

@@ -56,8 +56,8 @@ def linear_cross_entropy_pieces(
     """``x [M, K]``, ``weight [V, K]`` (any ``V``), int32 ``target [M]`` -> the scalar loss of ``linear_cross_entropy``.
 
     ``piece`` is the number of vocabulary columns the backward works on at once (default: as many as make its buffer
-    512 MiB, at least 8192).  A label outside ``[0, V)`` that is not ``ignore_index`` makes the loss NaN; ``"mean"``
-    over no label at all is NaN, with gradients of zero."""
+    512 MiB, at least 8192).  A label outside ``[0, V)`` that is not ``ignore_index`` makes the loss, its row of
+    ``dx`` and ``dweight`` NaN; ``"mean"`` over no label at all is NaN, with gradients of zero."""
     assert reduction in ("mean", "sum")
     assert target.dtype == torch.int32
     if piece is None:

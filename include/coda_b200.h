@@ -401,9 +401,10 @@ int coda_b200_gemm_e4m3(const void* A, const float* a_scale, const void* B, cons
                         void* stream);
 
 /* Cross entropy of the logits A @ B over all N columns (any N), storing none of them: lse fp32 [M], losses fp32 [M] (both
- * zero in ignored rows; NaN loss for a label outside [0, N)), and the scalars inv_count (1 / rows that are not ignored
- * with `mean`, else 1; 0 where all rows are ignored) and loss = inv_count * sum(losses) (NaN with `mean` where all are).  part_max / part_sum fp32 [M, coda_b200_lse_tiles(N)] and
- * target_logit fp32 [M] are workspace.  `live` (device int32, or NULL): see coda_b200_ce_compact. */
+ * zero in ignored rows, both NaN for a label outside [0, N), and so the gradients made from lse), and the scalars inv_count
+ * (1 / rows that are not ignored with `mean`, else 1; 0 where all rows are ignored) and loss = inv_count * sum(losses) (NaN
+ * with `mean` where all are).  part_max / part_sum fp32 [M, coda_b200_lse_tiles(N)] and target_logit fp32 [M] are workspace.
+ * `live` (device int32, or NULL): see coda_b200_ce_compact. */
 int coda_b200_ce_loss(const void* A, int64_t a_stride_m, int64_t a_stride_k, const void* B, int64_t b_stride_k,
                       int64_t b_stride_n, const int32_t* target, int ignore_index, int mean, const int32_t* live, float* part_max,
                       float* part_sum, float* target_logit, float* lse, float* losses, float* loss, float* inv_count, int M,

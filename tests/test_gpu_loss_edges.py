@@ -52,3 +52,23 @@ def test_no_label_counts(ck, M, K, V, piece, binding):
     logits = (x.detach().float() @ w.detach().float().T).requires_grad_(True)
     torch.nn.functional.cross_entropy(logits, torch.full_like(t, -100).long()).backward()
     assert not bool(logits.grad.any())  # what is meant by "as those of torch's own"
+
+
+@pytest.mark.parametrize("binding", ["compiled", "python"])
+@pytest.mark.parametrize("label", [-1, -2**31, 2**31 - 1, "V"])
+@pytest.mark.parametrize("M,K,V,piece", SIZES)
+def test_label_outside_the_vocabulary_reaches_the_gradients(ck, M, K, V, piece, label, binding):
+    """The loss is NaN, and so are the row's dx and all of dweight: a program that does not look at the loss sees it there.
+    The other rows' dx is what it is with a label in its place."""
+    x, w, t = make(M, K, V)
+    t[1] = -100
+    good = loss_of(ck, binding)(x, w, t, "sum", piece)
+    (dx_good,) = torch.autograd.grad(good, x)
+    t2 = t.clone()
+    t2[2] = V if label == "V" else label
+    loss = loss_of(ck, binding)(x, w, t2, "sum", piece)
+    assert bool(loss.isnan())
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    assert bool(dx[2].isnan().all()) and bool(dw.isnan().all())
+    rows = [i for i in range(M) if i != 2]
+    assert torch.equal(dx[rows], dx_good[rows])
