@@ -124,6 +124,15 @@ __global__ void __launch_bounds__(256) ce_gather_kernel(const uint4* __restrict_
     for (int c = threadIdx.x; c < K8; c += 256) rows[static_cast<long long>(n + i) * K8 + c] = make_uint4(0u, 0u, 0u, 0u);
 }
 
+// rows[i] = x[i], zero where row i is ignored: 0 * NaN would take what such a row holds into the weight gradient.
+__global__ void __launch_bounds__(256) ce_mask_kernel(const uint4* __restrict__ x, const int* __restrict__ target, int ignore_index,
+                                                      uint4* __restrict__ rows, int K8) {
+  const int i = blockIdx.x;
+  const bool counts = target[i] != ignore_index;
+  for (int c = threadIdx.x; c < K8; c += 256)
+    rows[static_cast<long long>(i) * K8 + c] = counts ? x[static_cast<long long>(i) * K8 + c] : make_uint4(0u, 0u, 0u, 0u);
+}
+
 // dx[i] = rows[position[i]], or zero
 __global__ void __launch_bounds__(256) ce_scatter_kernel(const uint4* __restrict__ rows, const int* __restrict__ position,
                                                          uint4* __restrict__ dx, int K8) {
@@ -159,6 +168,15 @@ extern "C" int coda_b200_ce_compact(const void* x, const int32_t* target, int ig
   if (rc != kOk) return rc;
   ce_gather_kernel<<<M, 256, 0, st>>>(static_cast<const uint4*>(x), position, live, static_cast<uint4*>(rows), M, K / 8);
   return launch_check("cross-entropy gather launch");
+}
+
+extern "C" int coda_b200_ce_mask(const void* x, const int32_t* target, int ignore_index, void* rows, int M, int K, void* stream) {
+  if (!x || !target || !rows) return fail(kBadArgument, "NULL pointer");
+  if (M <= 0 || K <= 0 || K % 8 != 0) return fail(kBadArgument, "M and K must be positive, K a multiple of 8");
+  if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows)) & 15u) != 0) return fail(kBadArgument, "matrices must be 16-byte aligned");
+  ce_mask_kernel<<<M, 256, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const uint4*>(x), target, ignore_index, static_cast<uint4*>(rows),
+                                                                   K / 8);
+  return launch_check("cross-entropy mask launch");
 }
 
 extern "C" int coda_b200_ce_scatter(const void* rows, const int32_t* position, void* dx, int M, int K, void* stream) {

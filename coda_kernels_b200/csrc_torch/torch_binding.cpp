@@ -605,6 +605,13 @@ OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tens
   Tensor g = new_matrix(x, M, ldg, at::kBFloat16);
   if (need_dx) dx = new_matrix(x, M, K, at::kBFloat16);
   if (need_dw) dw = new_matrix(x, V, K, at::kBFloat16);
+  Tensor counted = xs;  // the rows of the weight gradient
+  if (need_dw && live == nullptr) {
+    counted = at::empty_like(xs);
+    check(coda_b200_ce_mask(xs.data_ptr(), r.target.data_ptr<int32_t>(), static_cast<int>(ignore_index), counted.data_ptr(),
+                            static_cast<int>(M), static_cast<int>(K), stream_of(x)),
+          "ce_mask");
+  }
   if (need_dx && width < V) dx32 = new_matrix(x, M, K, at::kFloat);
   for (int64_t c0 = 0; c0 < V; c0 += width) {
     const int64_t n = std::min(width, V - c0);
@@ -616,7 +623,7 @@ OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tens
     if (need_dw) {
       Tensor out = dw->narrow(0, c0, n);
       if (live == nullptr)
-        gemm_out(gp.t(), xs, out, alpha, c10::nullopt, status);
+        gemm_out(gp.t(), counted, out, alpha, c10::nullopt, status);
       else
         check(coda_b200_gemm_live(gp.data_ptr(), ldg, xs.data_ptr(), K, nullptr, out.data_ptr(), K, 0, alpha->data_ptr<float>(), live, 1,
                                   static_cast<int>(n), static_cast<int>(K), static_cast<int>(M), status_ptr(status), stream_of(x)),

@@ -56,6 +56,11 @@ def _ce_compact_out(x: Tensor, target: Tensor, ignore_index: int, position: Tens
     )
 
 
+@torch.library.custom_op("coda_b200::ce_mask_out", mutates_args=("rows",), device_types="cuda")
+def _ce_mask_out(x: Tensor, target: Tensor, ignore_index: int, rows: Tensor) -> None:
+    check(lib.coda_b200_ce_mask(x.data_ptr(), target.data_ptr(), ignore_index, rows.data_ptr(), x.shape[0], x.shape[1], _stream(x)), "ce_mask")
+
+
 @torch.library.custom_op("coda_b200::ce_scatter_out", mutates_args=("dx",), device_types="cuda")
 def _ce_scatter_out(rows: Tensor, position: Tensor, dx: Tensor) -> None:
     check(lib.coda_b200_ce_scatter(rows.data_ptr(), position.data_ptr(), dx.data_ptr(), rows.shape[0], rows.shape[1], _stream(rows)), "ce_scatter")
@@ -78,7 +83,7 @@ def _ce_alpha_out(dloss: Tensor, inv_count: Tensor, alpha: Tensor) -> None:
     check(lib.coda_b200_ce_alpha(dloss.data_ptr(), inv_count.data_ptr(), alpha.data_ptr(), _stream(alpha)), "ce_alpha")
 
 
-for _op in (_ce_loss_out, _ce_alpha_out, _gemm_softmax_grad_out, _ce_compact_out, _ce_scatter_out, _gemm_live_out):
+for _op in (_ce_loss_out, _ce_alpha_out, _gemm_softmax_grad_out, _ce_compact_out, _ce_mask_out, _ce_scatter_out, _gemm_live_out):
     _op.register_fake(_noop_fake)
 
 
@@ -148,6 +153,10 @@ def ce_pieces_backward(dloss: Tensor, inv_count: Tensor, lse: Tensor, x: Tensor,
     dx = torch.empty_like(x) if need_dx else None
     dw = torch.empty_like(weight) if need_dw else None
     dx32 = torch.empty(M, K, dtype=torch.float32, device=x.device) if need_dx and width < V else None
+    counted = x  # the rows of the weight gradient: whatever an ignored row holds has no part in it
+    if need_dw and live is None:
+        counted = torch.empty_like(x)
+        _ce_mask_out(x, target, ignore_index, counted)
     for c0 in range(0, V, width):
         n = min(width, V - c0)
         w = weight[c0:c0 + n]
@@ -156,7 +165,7 @@ def ce_pieces_backward(dloss: Tensor, inv_count: Tensor, lse: Tensor, x: Tensor,
         if live is None:
             gp = g[:, :n]
             if need_dw:
-                gemm(gp.mT, x, out=dw[c0:c0 + n], alpha=alpha)
+                gemm(gp.mT, counted, out=dw[c0:c0 + n], alpha=alpha)
             if need_dx:
                 gemm(gp, w, out=dx32 if c0 + n < V else dx, alpha=alpha, C=sum_so_far)
         else:

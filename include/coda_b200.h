@@ -432,6 +432,10 @@ int coda_b200_ce_compact(const void* x, const int32_t* target, int ignore_index,
                          void* rows, int M, int K, void* stream);
 int coda_b200_ce_scatter(const void* rows, const int32_t* position, void* dx, int M, int K, void* stream);
 
+/* Where the rows are not put together: rows[i] = x[i] (dense bf16 [M, K]), zero where target[i] is ignore_index, so that whatever an
+ * ignored row holds stays out of the weight gradient. */
+int coda_b200_ce_mask(const void* x, const int32_t* target, int ignore_index, void* rows, int M, int K, void* stream);
+
 /* along_depth 0: D[m, n] = alpha * sum_k A[m, k] * B[k, n] + C[m, n] for the first *live rows (A [M, K], B [K, N], all row-major);
  * along_depth 1: D[m, n] = alpha * sum_k A[k, m] * B[k, n] (+ C) over the first *live k (A [K, M], B [K, N] row-major).
  * *live is rounded up to a multiple of 64 (at most M, or K).  C is fp32 with D's leading dimension, or NULL; it may be D. */

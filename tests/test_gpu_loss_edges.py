@@ -1,5 +1,5 @@
 """``linear_cross_entropy_pieces`` where labels are missing or wrong: gradients of a batch without a label, labels outside the
-vocabulary.  Each at a size whose products run over all rows and at one where the rows that count are put first, through the
+vocabulary, ignored rows that hold anything.  Each at a size whose products run over all rows and at one where the rows that count are put first, through the
 compiled operators and through the Python nodes."""
 
 from importlib import import_module
@@ -72,3 +72,26 @@ def test_label_outside_the_vocabulary_reaches_the_gradients(ck, M, K, V, piece, 
     assert bool(dx[2].isnan().all()) and bool(dw.isnan().all())
     rows = [i for i in range(M) if i != 2]
     assert torch.equal(dx[rows], dx_good[rows])
+
+
+@pytest.mark.parametrize("binding", ["compiled", "python"])
+@pytest.mark.parametrize("M,K,V,piece", SIZES)
+def test_ignored_rows_may_hold_anything(ck, M, K, V, piece, binding):
+    """Rows whose label is ignored take no part in loss, dx or dweight, whatever they hold, at every size."""
+    x, w, t = make(M, K, V)
+    t[5:9] = -100
+    t[M - 1] = -100
+    fn = loss_of(ck, binding)
+    clean = fn(x, w, t, "mean", piece)
+    grads = torch.autograd.grad(clean, (x, w))
+    bad = x.detach().clone()
+    bad[5], bad[6, 3], bad[M - 1] = float("nan"), float("inf"), float("-inf")
+    bad.requires_grad_(True)
+    loss = fn(bad, w, t, "mean", piece)
+    assert torch.equal(loss, clean)
+    for a, b in zip(torch.autograd.grad(loss, (bad, w)), grads):
+        assert torch.equal(a, b)
+    assert not bool(grads[0][t == -100].any())
+    # the weight's gradient alone, and an x that needs none
+    loss = fn(bad.detach(), w, t, "mean", piece)
+    assert torch.equal(torch.autograd.grad(loss, w)[0], grads[1])
