@@ -328,7 +328,13 @@ inline void require_dropout(const Tensor& x, double p, const OptTensor& rng, int
     TORCH_CHECK_VALUE(rng->device() == x.device() && rng->scalar_type() == at::kLong && rng->dim() == 1 && rng->size(0) == 2,
                       "rng must be an int64 tensor [seed, step] on x's device");
 }
+// A tangent would be dropped without a word by the plain path: the result would read as if the derivative were zero.
+inline void require_no_tangent(const char* name, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), name, " has no forward-mode derivative");
+}
 inline void require_no_grad(const char* name, std::initializer_list<const Tensor*> tensors) {
+  require_no_tangent(name, tensors);
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor* t : tensors)
     TORCH_CHECK(!t->defined() || !t->requires_grad(), name, " has no backward: call it under torch.no_grad() or on detached tensors");
@@ -381,6 +387,7 @@ class DropoutNode : public torch::autograd::Function<DropoutNode> {
 Tensor dropout(const Tensor& x, double p, const OptTensor& rng, int64_t stream) {
   require_rows(x);
   require_dropout(x, p, rng, stream);
+  require_no_tangent("dropout", {&x});
   if (wants_grad({&x})) return DropoutNode::apply(x, p, rng, stream);
   at::AutoDispatchBelowADInplaceOrView below;
   return run_dropout(aligned16(x), p, dense(rng), stream, nullptr);
@@ -470,6 +477,7 @@ class AddRMSNormNode : public torch::autograd::Function<AddRMSNormNode> {
 Tensor rms_norm(const Tensor& x, const Tensor& weight, double eps) {
   require_rows(x);
   require_weight(weight, x);
+  require_no_tangent("rms_norm", {&x, &weight});
   if (wants_grad({&x, &weight})) return RMSNormNode::apply(x, weight, eps);
   at::AutoDispatchBelowADInplaceOrView below;
   return run_norm(aligned16(x), Tensor(), aligned16(weight), eps, 0.0, Tensor(), 0).out;
@@ -481,6 +489,7 @@ std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& residual,
   require_like(residual, x, "residual");
   require_weight(weight, x);
   require_dropout(x, p, rng, stream);
+  require_no_tangent("add_rms_norm", {&x, &residual, &weight});
   if (wants_grad({&x, &residual, &weight})) {
     auto r = AddRMSNormNode::apply(x, residual, weight, eps, p, rng, stream);
     return {r[0], r[1]};
@@ -691,6 +700,7 @@ Tensor linear_cross_entropy_pieces(const Tensor& x, const Tensor& weight, const 
   TORCH_CHECK_VALUE(target.dim() == 1 && target.size(0) == x.size(0) && target.scalar_type() == at::kInt, "target must have one label per row");
   TORCH_CHECK_VALUE(ignore_index >= INT_MIN && ignore_index <= INT_MAX, "ignore_index must fit int32");
   TORCH_CHECK_VALUE(x.size(0) <= INT_MAX && weight.size(0) <= INT_MAX - 256, "extents must fit 31 bits");
+  require_no_tangent("linear_cross_entropy_pieces", {&x, &weight});
   if (wants_grad({&x, &weight})) return CePiecesNode::apply(x, weight, target, ignore_index, mean, piece, status);
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::cuda::CUDAGuard guard(x.device());

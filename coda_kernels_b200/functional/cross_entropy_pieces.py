@@ -6,8 +6,8 @@ backward walks the vocabulary in pieces, computes each piece's logits again and 
 gradients.  The price is that one product (a third more work in the backward); what it saves is everything of size
 ``M V`` but one ``[M, piece]`` buffer during the backward.
 
-Ignored rows may hold anything.  They have no part in the products where those are large enough to be worth it: the rows that count are first put
-together on the device, and the products end where they end, without the host knowing where that is.
+Ignored rows may hold anything.  They have no part in the products where those are large enough to be worth it: the rows that
+count are first put together on the device, and the products end where they end, without the host knowing where that is.
 """
 
 from __future__ import annotations

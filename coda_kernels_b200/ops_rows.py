@@ -12,6 +12,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from ._lib import CodaB200Error, check, lib
 from .ops import _aligned16, _noop_fake, _require, _stream, status_word
@@ -148,6 +149,8 @@ def _require_first_order(name: str) -> None:
 
 
 def _require_no_grad(name: str, *tensors: Optional[Tensor]) -> None:
+    if not torch.compiler.is_compiling() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no backward: call it under torch.no_grad() or on detached tensors")
 
