@@ -296,8 +296,10 @@ std::tuple<OptTensor, OptTensor, Tensor> qknorm_rope_bwd(const Tensor& dq, const
 }
 
 // ---------------------------------------------------------------------------------------- around the fused linears
-// Operators whose kernels take microseconds: the whole call, autograd node and argument checks included, is C++.
-// Registered for the Autograd key, they run the forward directly when nothing needs a gradient.
+// Operators whose kernels take microseconds: the whole call, autograd node and argument checks included, is C++, in two
+// layers.  The functions on the CUDA key check the arguments and launch; those on the Autograd key (namespace autograd)
+// decide whether a node is needed, and they and the nodes reach the CUDA functions through the dispatcher, forward and
+// backward, so that a tracer or a dispatch mode sees every computation as an operator.
 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
@@ -348,6 +350,12 @@ inline bool wants_grad(std::initializer_list<const Tensor*> tensors) {
     if (t->requires_grad()) return true;
   return false;
 }
+// An operator of this file through the dispatcher: below autograd, but seen by modes.
+template <typename Signature>
+c10::TypedOperatorHandle<Signature> operator_named(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
+}
+inline OptTensor optional(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 inline int row_dtype(const Tensor& t) {
   return t.scalar_type() == at::kBFloat16 ? 0 : t.scalar_type() == at::kHalf ? 1 : 2;
 }
@@ -355,9 +363,13 @@ inline const int64_t* rng_ptr(const Tensor& rng) { return rng.defined() ? rng.da
 inline void* ptr_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 inline Tensor dense(const OptTensor& t) { return t.has_value() ? aligned16(*t) : Tensor(); }
 
-// dropout of dense x from rng; `used` (when wanted) receives the [seed, step] the mask was made from
-Tensor run_dropout(const Tensor& x, double p, const Tensor& rng, int64_t stream, Tensor* used) {
-  const c10::cuda::CUDAGuard guard(x.device());
+// dropout of x from rng; `used` (when wanted) receives the [seed, step] the mask was made from
+Tensor run_dropout(const Tensor& x_in, double p, const OptTensor& rng_in, int64_t stream, Tensor* used) {
+  require_rows(x_in);
+  require_dropout(x_in, p, rng_in, stream);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::cuda::CUDAGuard guard(x_in.device());
+  const Tensor x = aligned16(x_in), rng = dense(rng_in);
   Tensor out = at::empty_like(x);
   if (used != nullptr) *used = at::empty({2}, x.options().dtype(at::kLong));
   check(coda_b200_dropout(x.data_ptr(), out.data_ptr(), x.numel() / x.size(-1), x.size(-1), row_dtype(x), p, rng_ptr(rng), stream,
@@ -365,57 +377,53 @@ Tensor run_dropout(const Tensor& x, double p, const Tensor& rng, int64_t stream,
         "dropout");
   return out;
 }
+Tensor dropout(const Tensor& x, double p, const OptTensor& rng, int64_t stream) { return run_dropout(x, p, rng, stream, nullptr); }
+// (out, the [seed, step] used)
+std::tuple<Tensor, Tensor> dropout_fwd(const Tensor& x, double p, const OptTensor& rng, int64_t stream) {
+  Tensor used, out = run_dropout(x, p, rng, stream, &used);
+  return {out, used};
+}
 
-class DropoutNode : public torch::autograd::Function<DropoutNode> {
- public:
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, double p, const OptTensor& rng, int64_t stream) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    Tensor used, out = run_dropout(aligned16(x), p, dense(rng), stream, &used);
-    ctx->save_for_backward({used});
-    ctx->saved_data["p"] = p;
-    ctx->saved_data["stream"] = stream;
-    return out;
-  }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    require_first_order("dropout");
-    const Tensor used = ctx->get_saved_variables()[0];
-    return {run_dropout(aligned16(grads[0]), ctx->saved_data["p"].toDouble(), used, ctx->saved_data["stream"].toInt(), nullptr), Tensor(),
-            Tensor(), Tensor()};
-  }
-};
-
-Tensor dropout(const Tensor& x, double p, const OptTensor& rng, int64_t stream) {
-  require_rows(x);
-  require_dropout(x, p, rng, stream);
-  require_no_tangent("dropout", {&x});
-  if (wants_grad({&x})) return DropoutNode::apply(x, p, rng, stream);
+// (out, h or nothing without a residual, rstd, the [seed, step] used or nothing without dropout)
+std::tuple<Tensor, OptTensor, Tensor, OptTensor> norm_fwd(const Tensor& x_in, const OptTensor& residual_in, const Tensor& weight_in, double eps,
+                                                          double p, const OptTensor& rng_in, int64_t stream) {
+  require_rows(x_in);
+  if (residual_in.has_value()) require_like(*residual_in, x_in, "residual");
+  require_weight(weight_in, x_in);
+  require_dropout(x_in, p, rng_in, stream);
+  TORCH_CHECK_VALUE(p == 0.0 || residual_in.has_value(), "dropout needs a residual");
   at::AutoDispatchBelowADInplaceOrView below;
-  return run_dropout(aligned16(x), p, dense(rng), stream, nullptr);
-}
-
-struct NormForward {
-  Tensor out, h, rstd, used;  // h only with a residual, used only with dropout
-};
-NormForward run_norm(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps, double p, const Tensor& rng, int64_t stream) {
-  const c10::cuda::CUDAGuard guard(x.device());
+  const c10::cuda::CUDAGuard guard(x_in.device());
+  const Tensor x = aligned16(x_in), residual = dense(residual_in), weight = aligned16(weight_in), rng = dense(rng_in);
   const int64_t cols = x.size(-1), rows = x.numel() / cols;
-  NormForward f;
-  f.out = at::empty_like(x);
-  f.rstd = at::empty({rows}, x.options().dtype(at::kFloat));
-  if (residual.defined()) f.h = at::empty_like(x);
-  if (p > 0.0) f.used = at::empty({2}, x.options().dtype(at::kLong));
+  Tensor out = at::empty_like(x), rstd = at::empty({rows}, x.options().dtype(at::kFloat));
+  OptTensor h, used;
+  if (residual.defined()) h = at::empty_like(x);
+  if (p > 0.0) used = at::empty({2}, x.options().dtype(at::kLong));
   check(coda_b200_add_rmsnorm_fwd(x.data_ptr(), ptr_or_null(residual), weight.data_ptr(), static_cast<float>(eps), p, rng_ptr(rng), stream,
-                                  f.used.defined() ? f.used.data_ptr<int64_t>() : nullptr, ptr_or_null(f.h), f.out.data_ptr(),
-                                  f.rstd.data_ptr<float>(), rows, cols, row_dtype(x), stream_of(x)),
+                                  used.has_value() ? used->data_ptr<int64_t>() : nullptr, h.has_value() ? h->data_ptr() : nullptr,
+                                  out.data_ptr(), rstd.data_ptr<float>(), rows, cols, row_dtype(x), stream_of(x)),
         "add_rmsnorm");
-  return f;
+  return {out, h, rstd, used};
 }
-// (dx, dres, dweight), undefined where not wanted
-variable_list run_norm_backward(const Tensor& dout, const Tensor& dh, const Tensor& h, const Tensor& rstd, const Tensor& weight, double p,
-                                const Tensor& rng, int64_t stream, bool need_dx, bool need_dres, bool need_dw) {
-  const c10::cuda::CUDAGuard guard(h.device());
+// (dx, dres, dweight), nothing where not wanted; dout undefined: only h was used
+std::tuple<OptTensor, OptTensor, OptTensor> norm_bwd(const OptTensor& dout_in, const OptTensor& dh_in, const Tensor& h_in, const Tensor& rstd,
+                                                     const Tensor& weight_in, double p, const OptTensor& rng_in, int64_t stream, bool need_dx,
+                                                     bool need_dres, bool need_dw) {
+  require_rows(h_in);
+  if (dout_in.has_value()) require_like(*dout_in, h_in, "dout");
+  if (dh_in.has_value()) require_like(*dh_in, h_in, "dh");
+  require_weight(weight_in, h_in);
+  require_dropout(h_in, p, rng_in, stream);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::cuda::CUDAGuard guard(h_in.device());
+  const Tensor h = aligned16(h_in), weight = aligned16(weight_in), rng = dense(rng_in), dh = dense(dh_in);
+  const Tensor dout = dout_in.has_value() ? aligned16(*dout_in) : at::zeros_like(h);
   const int64_t cols = h.size(-1), rows = h.numel() / cols;
-  Tensor dx, dres, dw, scratch;
+  TORCH_CHECK_VALUE(rstd.device() == h.device() && rstd.scalar_type() == at::kFloat && rstd.is_contiguous() && rstd.numel() == rows,
+                    "rstd must be float32 with one entry per row");
+  OptTensor dx, dres, dw;
+  Tensor scratch;
   if (need_dx) dx = at::empty_like(h);
   if (need_dres) dres = at::empty_like(h);
   int64_t scratch_bytes = 0;
@@ -424,93 +432,27 @@ variable_list run_norm_backward(const Tensor& dout, const Tensor& dh, const Tens
     scratch_bytes = coda_b200_add_rmsnorm_bwd_scratch_bytes(rows, cols);
     scratch = at::empty({scratch_bytes / 4}, h.options().dtype(at::kFloat));
   }
+  auto to = [](const OptTensor& t) { return t.has_value() ? t->data_ptr() : nullptr; };
   check(coda_b200_add_rmsnorm_bwd(dout.data_ptr(), ptr_or_null(dh), h.data_ptr(), rstd.data_ptr<float>(), weight.data_ptr(), p, rng_ptr(rng),
-                                  stream, ptr_or_null(dx), ptr_or_null(dres), ptr_or_null(dw), ptr_or_null(scratch), scratch_bytes, rows, cols,
-                                  row_dtype(h), stream_of(h)),
+                                  stream, to(dx), to(dres), to(dw), ptr_or_null(scratch), scratch_bytes, rows, cols, row_dtype(h),
+                                  stream_of(h)),
         "add_rmsnorm backward");
   return {dx, dres, dw};
 }
-
-class RMSNormNode : public torch::autograd::Function<RMSNormNode> {
- public:
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, double eps) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor xc = aligned16(x), w = aligned16(weight);
-    NormForward f = run_norm(xc, Tensor(), w, eps, 0.0, Tensor(), 0);
-    ctx->save_for_backward({xc, w, f.rstd});
-    return f.out;
-  }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    require_first_order("rms_norm");
-    const auto saved = ctx->get_saved_variables();
-    auto g = run_norm_backward(aligned16(grads[0]), Tensor(), saved[0], saved[2], saved[1], 0.0, Tensor(), 0, false, ctx->needs_input_grad(0),
-                               ctx->needs_input_grad(1));
-    return {g[1], g[2], Tensor()};
-  }
-};
-
-class AddRMSNormNode : public torch::autograd::Function<AddRMSNormNode> {
- public:
-  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const Tensor& weight, double eps, double p,
-                               const OptTensor& rng, int64_t stream) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor w = aligned16(weight);
-    NormForward f = run_norm(aligned16(x), aligned16(residual), w, eps, p, dense(rng), stream);
-    ctx->save_for_backward({f.h, w, f.rstd, f.used});
-    ctx->saved_data["p"] = p;
-    ctx->saved_data["stream"] = stream;
-    ctx->set_materialize_grads(false);
-    return {f.out, f.h};
-  }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    require_first_order("add_rms_norm");
-    const auto saved = ctx->get_saved_variables();
-    const Tensor& h = saved[0];
-    const Tensor dout = grads[0].defined() ? aligned16(grads[0]) : at::zeros_like(h);  // undefined: only h was used
-    const Tensor dh = grads[1].defined() ? aligned16(grads[1]) : Tensor();
-    auto g = run_norm_backward(dout, dh, h, saved[2], saved[1], ctx->saved_data["p"].toDouble(), saved[3], ctx->saved_data["stream"].toInt(),
-                               ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2));
-    return {g[0], g[1], g[2], Tensor(), Tensor(), Tensor(), Tensor()};
-  }
-};
-
 Tensor rms_norm(const Tensor& x, const Tensor& weight, double eps) {
-  require_rows(x);
-  require_weight(weight, x);
-  require_no_tangent("rms_norm", {&x, &weight});
-  if (wants_grad({&x, &weight})) return RMSNormNode::apply(x, weight, eps);
-  at::AutoDispatchBelowADInplaceOrView below;
-  return run_norm(aligned16(x), Tensor(), aligned16(weight), eps, 0.0, Tensor(), 0).out;
+  return std::get<0>(norm_fwd(x, c10::nullopt, weight, eps, 0.0, c10::nullopt, 0));
 }
-
 std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps, double p,
                                         const OptTensor& rng, int64_t stream) {
-  require_rows(x);
-  require_like(residual, x, "residual");
-  require_weight(weight, x);
-  require_dropout(x, p, rng, stream);
-  require_no_tangent("add_rms_norm", {&x, &residual, &weight});
-  if (wants_grad({&x, &residual, &weight})) {
-    auto r = AddRMSNormNode::apply(x, residual, weight, eps, p, rng, stream);
-    return {r[0], r[1]};
-  }
-  at::AutoDispatchBelowADInplaceOrView below;
-  NormForward f = run_norm(aligned16(x), aligned16(residual), aligned16(weight), eps, p, dense(rng), stream);
-  return {f.out, f.h};
+  auto f = norm_fwd(x, residual, weight, eps, p, rng, stream);
+  return {std::get<0>(f), *std::get<1>(f)};
 }
 
 // (q, scale, h or nothing)
 std::tuple<Tensor, Tensor, OptTensor> rows_e4m3(const Tensor& x_in, const OptTensor& residual_in, const OptTensor& weight_in, double eps) {
   require_rows(x_in);
-  require_no_grad("the e4m3 output", {&x_in});
-  if (residual_in.has_value()) {
-    require_like(*residual_in, x_in, "residual");
-    require_no_grad("the e4m3 output", {&*residual_in});
-  }
-  if (weight_in.has_value()) {
-    require_weight(*weight_in, x_in);
-    require_no_grad("the e4m3 output", {&*weight_in});
-  }
+  if (residual_in.has_value()) require_like(*residual_in, x_in, "residual");
+  if (weight_in.has_value()) require_weight(*weight_in, x_in);
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::cuda::CUDAGuard guard(x_in.device());
   const Tensor x = aligned16(x_in), residual = dense(residual_in), weight = dense(weight_in);
@@ -542,7 +484,6 @@ Tensor linear_e4m3(const Tensor& x_in, const Tensor& x_scale, const Tensor& weig
   TORCH_CHECK_VALUE(weight_scale.scalar_type() == at::kFloat && weight_scale.dim() == 1 && weight_scale.size(0) == N,
                     "weight_scale must be float32 with one entry per row");
   TORCH_CHECK_VALUE(M <= INT_MAX && N <= INT_MAX && K <= INT_MAX, "extents must fit 31 bits");
-  require_no_grad("linear_e4m3", {&x_in, &x_scale, &weight_in, &weight_scale});
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::cuda::CUDAGuard guard(x_in.device());
   const Tensor x = aligned16(x_in), xs = x_scale.contiguous(), weight = aligned16(weight_in), ws = weight_scale.contiguous();
@@ -563,9 +504,14 @@ Tensor linear_e4m3(const Tensor& x_in, const Tensor& x_scale, const Tensor& weig
 struct CeRows {
   Tensor x, target, position, live;
 };
-CeRows ce_rows(const Tensor& x, const Tensor& target, int64_t ignore_index, int64_t V) {
+inline bool ce_compacts(const Tensor& x, const Tensor& weight) {
+  for (const int64_t n : {x.size(0), weight.size(0), x.size(-1)})
+    if (n < 1 || n > INT_MAX) return false;
+  return coda_b200_ce_compacts(static_cast<int>(x.size(0)), static_cast<int>(weight.size(0)), static_cast<int>(x.size(-1))) != 0;
+}
+CeRows ce_rows(const Tensor& x, const Tensor& target, int64_t ignore_index, bool compact) {
+  if (!compact) return {x, target, Tensor(), Tensor()};
   const int M = static_cast<int>(x.size(0)), K = static_cast<int>(x.size(1));
-  if (M == 0 || !coda_b200_ce_compacts(M, static_cast<int>(V), K)) return {x, target, Tensor(), Tensor()};
   CeRows r{at::empty_like(x), at::empty_like(target), at::empty_like(target), at::empty({1}, target.options())};
   check(coda_b200_ce_compact(x.data_ptr(), target.data_ptr<int32_t>(), static_cast<int>(ignore_index), r.position.data_ptr<int32_t>(),
                              r.target.data_ptr<int32_t>(), r.live.data_ptr<int32_t>(), r.x.data_ptr(), M, K, stream_of(x)),
@@ -663,33 +609,7 @@ OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tens
   return {dx, dw};
 }
 
-class CePiecesNode : public torch::autograd::Function<CePiecesNode> {
- public:
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight_in, const Tensor& target, int64_t ignore_index, bool mean,
-                        int64_t piece, const Tensor& status) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    const c10::cuda::CUDAGuard guard(x.device());
-    const Tensor weight = aligned16(weight_in);
-    const CeRows r = ce_rows(aligned16(x), target.contiguous(), ignore_index, weight.size(0));
-    auto [loss, inv_count, lse] = run_ce(r, weight, ignore_index, mean, status);
-    ctx->save_for_backward({r.x, weight, r.target, lse, inv_count, r.position, r.live});
-    ctx->saved_data["ignore_index"] = ignore_index;
-    ctx->saved_data["piece"] = piece;
-    ctx->saved_data["status"] = status;
-    return loss;
-  }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    require_first_order("linear_cross_entropy_pieces");
-    const auto s = ctx->get_saved_variables();
-    auto [dx, dw] = run_ce_backward(grads[0], s[4], s[3], CeRows{s[0], s[2], s[5], s[6]}, s[1], ctx->saved_data["ignore_index"].toInt(),
-                                    ctx->saved_data["piece"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1),
-                                    ctx->saved_data["status"].toTensor());
-    return {dx.value_or(Tensor()), dw.value_or(Tensor()), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
-  }
-};
-
-Tensor linear_cross_entropy_pieces(const Tensor& x, const Tensor& weight, const Tensor& target, int64_t ignore_index, bool mean, int64_t piece,
-                                   const Tensor& status) {
+inline void require_ce(const Tensor& x, const Tensor& weight, const Tensor& target, int64_t ignore_index) {
   for (const Tensor* t : {&x, &weight}) {
     require_cuda(*t);
     TORCH_CHECK_NOT_IMPLEMENTED(t->scalar_type() == at::kBFloat16, "coda_b200 operators take bfloat16 matrices, got ", t->scalar_type());
@@ -700,14 +620,212 @@ Tensor linear_cross_entropy_pieces(const Tensor& x, const Tensor& weight, const 
   TORCH_CHECK_VALUE(target.dim() == 1 && target.size(0) == x.size(0) && target.scalar_type() == at::kInt, "target must have one label per row");
   TORCH_CHECK_VALUE(ignore_index >= INT_MIN && ignore_index <= INT_MAX, "ignore_index must fit int32");
   TORCH_CHECK_VALUE(x.size(0) <= INT_MAX && weight.size(0) <= INT_MAX - 256, "extents must fit 31 bits");
+}
+
+// (loss, inv_count, lse, and with `compact` the rows that count, put first, their labels, position and live).  Whether to is
+// the caller's to say: a recorded program keeps what it was recorded with, whatever the options are when it runs.
+std::tuple<Tensor, Tensor, Tensor, OptTensor, OptTensor, OptTensor, OptTensor> ce_pieces_fwd(const Tensor& x, const Tensor& weight,
+                                                                                            const Tensor& target, int64_t ignore_index,
+                                                                                            bool mean, bool compact, const Tensor& status) {
+  require_ce(x, weight, target, ignore_index);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::cuda::CUDAGuard guard(x.device());
+  const CeRows r = ce_rows(aligned16(x), target.contiguous(), ignore_index, compact && x.size(0) > 0);
+  auto [loss, inv_count, lse] = run_ce(r, aligned16(weight), ignore_index, mean, status);
+  if (!r.live.defined()) return {loss, inv_count, lse, c10::nullopt, c10::nullopt, c10::nullopt, c10::nullopt};
+  return {loss, inv_count, lse, r.x, r.target, r.position, r.live};
+}
+
+// x and target: those of the forward, or the rows and labels it put first, with position and live
+OptPair ce_pieces_bwd(const Tensor& dloss, const Tensor& inv_count, const Tensor& lse, const Tensor& x, const Tensor& weight,
+                      const Tensor& target, const OptTensor& position, const OptTensor& live, int64_t ignore_index, int64_t piece, bool need_dx,
+                      bool need_dw, const Tensor& status) {
+  require_ce(x, weight, target, ignore_index);
+  TORCH_CHECK_VALUE(piece >= 1, "piece must be at least 1");
+  for (const Tensor* t : {&inv_count, &lse})
+    TORCH_CHECK_VALUE(t->device() == x.device() && t->scalar_type() == at::kFloat && t->is_contiguous(), "float32 statistics expected");
+  TORCH_CHECK_VALUE(inv_count.numel() == 1 && dloss.numel() == 1 && lse.numel() == x.size(0), "one dloss, inv_count, and one lse a row expected");
+  TORCH_CHECK_VALUE(position.has_value() == live.has_value(), "position and live belong together");
+  if (live.has_value())
+    TORCH_CHECK_VALUE(position->device() == x.device() && position->scalar_type() == at::kInt && position->is_contiguous() &&
+                          position->numel() == x.size(0) && live->device() == x.device() && live->scalar_type() == at::kInt && live->numel() == 1,
+                      "position must be int32 with one entry per row, live one int32");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return run_ce_backward(dloss, inv_count, lse, CeRows{aligned16(x), target.contiguous(), position.value_or(Tensor()), live.value_or(Tensor())},
+                         aligned16(weight), ignore_index, piece, need_dx, need_dw, status);
+}
+
+Tensor linear_cross_entropy_pieces(const Tensor& x, const Tensor& weight, const Tensor& target, int64_t ignore_index, bool mean, int64_t,
+                                   const Tensor& status) {
+  return std::get<0>(ce_pieces_fwd(x, weight, target, ignore_index, mean, ce_compacts(x, weight), status));
+}
+
+// ---------------------------------------------------------------------------------------- their gradients
+namespace autograd {
+
+Tensor call_dropout(const Tensor& x, double p, const OptTensor& rng, int64_t stream) {
+  static const auto op = operator_named<Tensor(const Tensor&, double, const OptTensor&, int64_t)>("coda_b200n::dropout");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, p, rng, stream);
+}
+auto call_norm_fwd(const Tensor& x, const OptTensor& residual, const Tensor& weight, double eps, double p, const OptTensor& rng, int64_t stream) {
+  static const auto op = operator_named<std::tuple<Tensor, OptTensor, Tensor, OptTensor>(
+      const Tensor&, const OptTensor&, const Tensor&, double, double, const OptTensor&, int64_t)>("coda_b200n::norm_fwd");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, residual, weight, eps, p, rng, stream);
+}
+auto call_norm_bwd(const OptTensor& dout, const OptTensor& dh, const Tensor& h, const Tensor& rstd, const Tensor& weight, double p,
+                   const OptTensor& rng, int64_t stream, bool need_dx, bool need_dres, bool need_dw) {
+  static const auto op =
+      operator_named<std::tuple<OptTensor, OptTensor, OptTensor>(const OptTensor&, const OptTensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                                 double, const OptTensor&, int64_t, bool, bool, bool)>("coda_b200n::norm_bwd");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(dout, dh, h, rstd, weight, p, rng, stream, need_dx, need_dres, need_dw);
+}
+
+class DropoutNode : public torch::autograd::Function<DropoutNode> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, double p, const OptTensor& rng, int64_t stream) {
+    static const auto op =
+        operator_named<std::tuple<Tensor, Tensor>(const Tensor&, double, const OptTensor&, int64_t)>("coda_b200n::dropout_fwd");
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [out, used] = op.call(x, p, rng, stream);
+    ctx->save_for_backward({used});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["stream"] = stream;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    require_first_order("dropout");
+    const Tensor used = ctx->get_saved_variables()[0];
+    return {call_dropout(grads[0], ctx->saved_data["p"].toDouble(), used, ctx->saved_data["stream"].toInt()), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+class RMSNormNode : public torch::autograd::Function<RMSNormNode> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& weight, double eps) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor x = x_in.contiguous();
+    auto f = call_norm_fwd(x, c10::nullopt, weight, eps, 0.0, c10::nullopt, 0);
+    ctx->save_for_backward({x, weight, std::get<2>(f)});
+    return std::get<0>(f);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    require_first_order("rms_norm");
+    const auto saved = ctx->get_saved_variables();
+    auto g = call_norm_bwd(grads[0], c10::nullopt, saved[0], saved[2], saved[1], 0.0, c10::nullopt, 0, false, ctx->needs_input_grad(0),
+                           ctx->needs_input_grad(1));
+    return {std::get<1>(g).value_or(Tensor()), std::get<2>(g).value_or(Tensor()), Tensor()};
+  }
+};
+
+class AddRMSNormNode : public torch::autograd::Function<AddRMSNormNode> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const Tensor& weight, double eps, double p,
+                               const OptTensor& rng, int64_t stream) {
+    auto f = call_norm_fwd(x, residual, weight, eps, p, rng, stream);
+    const Tensor &out = std::get<0>(f), &h = *std::get<1>(f);
+    ctx->save_for_backward({h, weight, std::get<2>(f), std::get<3>(f).value_or(Tensor())});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["stream"] = stream;
+    ctx->set_materialize_grads(false);
+    return {out, h};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    require_first_order("add_rms_norm");
+    const auto saved = ctx->get_saved_variables();
+    auto g = call_norm_bwd(optional(grads[0]), optional(grads[1]), saved[0], saved[2], saved[1], ctx->saved_data["p"].toDouble(),
+                           optional(saved[3]), ctx->saved_data["stream"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                           ctx->needs_input_grad(2));
+    return {std::get<0>(g).value_or(Tensor()), std::get<1>(g).value_or(Tensor()), std::get<2>(g).value_or(Tensor()), Tensor(), Tensor(), Tensor(),
+            Tensor()};
+  }
+};
+
+class CePiecesNode : public torch::autograd::Function<CePiecesNode> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& weight_in, const Tensor& target_in, int64_t ignore_index,
+                        bool mean, int64_t piece, const Tensor& status) {
+    static const auto op = operator_named<std::tuple<Tensor, Tensor, Tensor, OptTensor, OptTensor, OptTensor, OptTensor>(
+        const Tensor&, const Tensor&, const Tensor&, int64_t, bool, bool, const Tensor&)>("coda_b200n::ce_pieces_fwd");
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor x = x_in.contiguous(), weight = weight_in.contiguous(), target = target_in.contiguous();
+    auto [loss, inv_count, lse, rows, labels, position, live] = op.call(x, weight, target, ignore_index, mean, ce_compacts(x, weight), status);
+    ctx->save_for_backward({rows.value_or(x), weight, labels.value_or(target), lse, inv_count, position.value_or(Tensor()), live.value_or(Tensor())});
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["piece"] = piece;
+    ctx->saved_data["status"] = status;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    static const auto op = operator_named<OptPair(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                  const OptTensor&, const OptTensor&, int64_t, int64_t, bool, bool, const Tensor&)>(
+        "coda_b200n::ce_pieces_bwd");
+    require_first_order("linear_cross_entropy_pieces");
+    const auto s = ctx->get_saved_variables();
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [dx, dw] = op.call(grads[0], s[4], s[3], s[0], s[1], s[2], optional(s[5]), optional(s[6]), ctx->saved_data["ignore_index"].toInt(),
+                            ctx->saved_data["piece"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                            ctx->saved_data["status"].toTensor());
+    return {dx.value_or(Tensor()), dw.value_or(Tensor()), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor dropout(const Tensor& x, double p, const OptTensor& rng, int64_t stream) {
+  require_no_tangent("dropout", {&x});
+  return wants_grad({&x}) ? DropoutNode::apply(x, p, rng, stream) : call_dropout(x, p, rng, stream);
+}
+
+Tensor rms_norm(const Tensor& x, const Tensor& weight, double eps) {
+  static const auto op = operator_named<Tensor(const Tensor&, const Tensor&, double)>("coda_b200n::rms_norm");
+  require_no_tangent("rms_norm", {&x, &weight});
+  if (wants_grad({&x, &weight})) return RMSNormNode::apply(x, weight, eps);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, weight, eps);
+}
+
+std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps, double p,
+                                        const OptTensor& rng, int64_t stream) {
+  static const auto op = operator_named<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, double, double, const OptTensor&,
+                                                                   int64_t)>("coda_b200n::add_rms_norm");
+  require_no_tangent("add_rms_norm", {&x, &residual, &weight});
+  if (wants_grad({&x, &residual, &weight})) {
+    auto r = AddRMSNormNode::apply(x, residual, weight, eps, p, rng, stream);
+    return {r[0], r[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, residual, weight, eps, p, rng, stream);
+}
+
+std::tuple<Tensor, Tensor, OptTensor> rows_e4m3(const Tensor& x, const OptTensor& residual, const OptTensor& weight, double eps) {
+  static const auto op = operator_named<std::tuple<Tensor, Tensor, OptTensor>(const Tensor&, const OptTensor&, const OptTensor&, double)>(
+      "coda_b200n::rows_e4m3");
+  const Tensor none;
+  require_no_grad("the e4m3 output", {&x, residual.has_value() ? &*residual : &none, weight.has_value() ? &*weight : &none});
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, residual, weight, eps);
+}
+
+Tensor linear_e4m3(const Tensor& x, const Tensor& x_scale, const Tensor& weight, const Tensor& weight_scale, bool out_fp32, const Tensor& status) {
+  static const auto op =
+      operator_named<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, bool, const Tensor&)>("coda_b200n::linear_e4m3");
+  require_no_grad("linear_e4m3", {&x, &x_scale, &weight, &weight_scale});
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, x_scale, weight, weight_scale, out_fp32, status);
+}
+
+Tensor linear_cross_entropy_pieces(const Tensor& x, const Tensor& weight, const Tensor& target, int64_t ignore_index, bool mean, int64_t piece,
+                                   const Tensor& status) {
+  static const auto op = operator_named<Tensor(const Tensor&, const Tensor&, const Tensor&, int64_t, bool, int64_t, const Tensor&)>(
+      "coda_b200n::linear_cross_entropy_pieces");
   require_no_tangent("linear_cross_entropy_pieces", {&x, &weight});
   if (wants_grad({&x, &weight})) return CePiecesNode::apply(x, weight, target, ignore_index, mean, piece, status);
   at::AutoDispatchBelowADInplaceOrView below;
-  const c10::cuda::CUDAGuard guard(x.device());
-  return std::get<0>(run_ce(ce_rows(aligned16(x), target.contiguous(), ignore_index, weight.size(0)), aligned16(weight), ignore_index, mean,
-                            status));
+  return op.call(x, weight, target, ignore_index, mean, piece, status);
 }
 
+}  // namespace autograd
 }  // namespace
 
 TORCH_LIBRARY(coda_b200n, m) {
@@ -744,6 +862,14 @@ TORCH_LIBRARY(coda_b200n, m) {
         "Tensor status) -> (Tensor?, Tensor?, Tensor)");
 
   m.def("dropout(Tensor x, float p, Tensor? rng, int stream) -> Tensor");
+  m.def("dropout_fwd(Tensor x, float p, Tensor? rng, int stream) -> (Tensor, Tensor)");
+  m.def("norm_fwd(Tensor x, Tensor? residual, Tensor weight, float eps, float p, Tensor? rng, int stream) -> (Tensor, Tensor?, Tensor, Tensor?)");
+  m.def("norm_bwd(Tensor? dout, Tensor? dh, Tensor h, Tensor rstd, Tensor weight, float p, Tensor? rng, int stream, bool need_dx, "
+        "bool need_dres, bool need_dw) -> (Tensor?, Tensor?, Tensor?)");
+  m.def("ce_pieces_fwd(Tensor x, Tensor weight, Tensor target, int ignore_index, bool mean, bool compact, Tensor status) -> "
+        "(Tensor, Tensor, Tensor, Tensor?, Tensor?, Tensor?, Tensor?)");
+  m.def("ce_pieces_bwd(Tensor dloss, Tensor inv_count, Tensor lse, Tensor x, Tensor weight, Tensor target, Tensor? position, Tensor? live, "
+        "int ignore_index, int piece, bool need_dx, bool need_dw, Tensor status) -> (Tensor?, Tensor?)");
   m.def("rms_norm(Tensor x, Tensor weight, float eps) -> Tensor");
   m.def("add_rms_norm(Tensor x, Tensor residual, Tensor weight, float eps, float p, Tensor? rng, int stream) -> (Tensor, Tensor)");
   m.def("rows_e4m3(Tensor x, Tensor? residual, Tensor? weight, float eps) -> (Tensor, Tensor, Tensor?)");
@@ -773,14 +899,24 @@ TORCH_LIBRARY_IMPL(coda_b200n, CUDA, m) {
   m.impl("qknorm_rope_bwd", qknorm_rope_bwd);
 }
 
-// The operators that bring their own autograd node sit on the Autograd key, and on the CUDA key for calls that come in
-// below it (inference mode).
-#define CODA_WITH_AUTOGRAD(m)                                          \
-  m.impl("dropout", dropout);                                           \
-  m.impl("rms_norm", rms_norm);                                         \
-  m.impl("add_rms_norm", add_rms_norm);                                 \
-  m.impl("rows_e4m3", rows_e4m3);                                       \
-  m.impl("linear_e4m3", linear_e4m3);                                   \
-  m.impl("linear_cross_entropy_pieces", linear_cross_entropy_pieces)
-TORCH_LIBRARY_IMPL(coda_b200n, AutogradCUDA, m) { CODA_WITH_AUTOGRAD(m); }
-TORCH_LIBRARY_IMPL(coda_b200n, CUDA, m) { CODA_WITH_AUTOGRAD(m); }
+TORCH_LIBRARY_IMPL(coda_b200n, CUDA, m) {
+  m.impl("dropout", dropout);
+  m.impl("dropout_fwd", dropout_fwd);
+  m.impl("norm_fwd", norm_fwd);
+  m.impl("norm_bwd", norm_bwd);
+  m.impl("rms_norm", rms_norm);
+  m.impl("add_rms_norm", add_rms_norm);
+  m.impl("rows_e4m3", rows_e4m3);
+  m.impl("linear_e4m3", linear_e4m3);
+  m.impl("ce_pieces_fwd", ce_pieces_fwd);
+  m.impl("ce_pieces_bwd", ce_pieces_bwd);
+  m.impl("linear_cross_entropy_pieces", linear_cross_entropy_pieces);
+}
+TORCH_LIBRARY_IMPL(coda_b200n, AutogradCUDA, m) {
+  m.impl("dropout", autograd::dropout);
+  m.impl("rms_norm", autograd::rms_norm);
+  m.impl("add_rms_norm", autograd::add_rms_norm);
+  m.impl("rows_e4m3", autograd::rows_e4m3);
+  m.impl("linear_e4m3", autograd::linear_e4m3);
+  m.impl("linear_cross_entropy_pieces", autograd::linear_cross_entropy_pieces);
+}

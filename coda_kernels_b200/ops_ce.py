@@ -13,7 +13,7 @@ from torch import Tensor
 
 from . import ops
 from ._lib import check, lib
-from .ops import _noop_fake, _require, _require_cuda_bf16, _stream, gemm, lse_tiles, status_word
+from .ops import _native, _noop_fake, _require, _require_cuda_bf16, _stream, gemm, lse_tiles, status_word
 
 
 def _ptr(t: Optional[Tensor]):
@@ -85,6 +85,23 @@ def _ce_alpha_out(dloss: Tensor, inv_count: Tensor, alpha: Tensor) -> None:
 
 for _op in (_ce_loss_out, _ce_alpha_out, _gemm_softmax_grad_out, _ce_compact_out, _ce_mask_out, _ce_scatter_out, _gemm_live_out):
     _op.register_fake(_noop_fake)
+
+
+if _native is not None:  # the compiled operators on fake tensors
+
+    @torch.library.register_fake("coda_b200n::linear_cross_entropy_pieces")
+    def _(x, weight, target, ignore_index, mean, piece, status):
+        return x.new_empty((), dtype=torch.float32)
+
+    @torch.library.register_fake("coda_b200n::ce_pieces_fwd")
+    def _(x, weight, target, ignore_index, mean, compact, status):
+        f32 = dict(dtype=torch.float32)
+        rows = [x.new_empty(x.shape), *(target.new_empty(n) for n in (x.shape[0], x.shape[0], 1))] if compact else [None] * 4
+        return x.new_empty((), **f32), x.new_empty((), **f32), x.new_empty(x.shape[0], **f32), *rows
+
+    @torch.library.register_fake("coda_b200n::ce_pieces_bwd")
+    def _(dloss, inv_count, lse, x, weight, target, position, live, ignore_index, piece, need_dx, need_dw, status):
+        return x.new_empty(x.shape) if need_dx else None, weight.new_empty(weight.shape) if need_dw else None
 
 
 # Default size of the [rows, piece] gradient buffer, in elements (512 MiB), and the narrowest piece it is cut down to for

@@ -15,7 +15,7 @@ from torch import Tensor
 from torch.autograd import forward_ad
 
 from ._lib import CodaB200Error, check, lib
-from .ops import _aligned16, _noop_fake, _require, _stream, status_word
+from .ops import _aligned16, _native, _noop_fake, _require, _stream, status_word
 
 _DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 E4M3 = torch.float8_e4m3fn
@@ -113,6 +113,52 @@ def _gemm_e4m3_out(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Ten
 
 for _op in (_dropout_out, _add_rmsnorm_out, _add_rmsnorm_bwd_out, _rows_e4m3_out, _gemm_e4m3_out):
     _op.register_fake(_noop_fake)
+
+
+# ------------------------------------------------------------------------------------------------ compiled operators on fake tensors
+def _like(x: Tensor) -> Tensor:
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def _rows_like(x: Tensor) -> Tensor:
+    return x.new_empty(x.shape[:-1].numel(), dtype=torch.float32)
+
+
+if _native is not None:
+
+    @torch.library.register_fake("coda_b200n::dropout")
+    def _(x, p, rng, stream):
+        return _like(x)
+
+    @torch.library.register_fake("coda_b200n::dropout_fwd")
+    def _(x, p, rng, stream):
+        return _like(x), x.new_empty(2, dtype=torch.int64)
+
+    @torch.library.register_fake("coda_b200n::norm_fwd")
+    def _(x, residual, weight, eps, p, rng, stream):
+        h = None if residual is None else _like(x)
+        return _like(x), h, _rows_like(x), x.new_empty(2, dtype=torch.int64) if p > 0.0 else None
+
+    @torch.library.register_fake("coda_b200n::norm_bwd")
+    def _(dout, dh, h, rstd, weight, p, rng, stream, need_dx, need_dres, need_dw):
+        return _like(h) if need_dx else None, _like(h) if need_dres else None, _like(weight) if need_dw else None
+
+    @torch.library.register_fake("coda_b200n::rms_norm")
+    def _(x, weight, eps):
+        return _like(x)
+
+    @torch.library.register_fake("coda_b200n::add_rms_norm")
+    def _(x, residual, weight, eps, p, rng, stream):
+        return _like(x), _like(x)
+
+    @torch.library.register_fake("coda_b200n::rows_e4m3")
+    def _(x, residual, weight, eps):
+        scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+        return x.new_empty(x.shape, dtype=E4M3), scale, None if residual is None else _like(x)
+
+    @torch.library.register_fake("coda_b200n::linear_e4m3")
+    def _(x, x_scale, weight, weight_scale, out_fp32, status):
+        return x.new_empty(x.shape[0], weight.shape[0], dtype=torch.float32 if out_fp32 else torch.bfloat16)
 
 
 # ------------------------------------------------------------------------------------------------ argument checks

@@ -1,4 +1,5 @@
-"""The operators around the fused linears under PyTorch's program transforms: forward-mode derivatives are refused."""
+"""The operators around the fused linears under PyTorch's program transforms: forward-mode derivatives are refused; tracers and
+dispatch modes see the computation."""
 
 import pytest
 import torch
@@ -69,3 +70,144 @@ def test_forward_mode_is_refused(ck, monkeypatch, name, whole_operators):
     fn(*inputs)  # and nothing is refused without one
     with fwd.dual_level():
         fn(*inputs)
+
+
+# ------------------------------------------------------------------------------------------------ tracers and modes
+def flat(out):
+    return [t for t in (out if isinstance(out, tuple) else (out,)) if t is not None]
+
+
+def step_of(fn, differentiable):
+    """The forward, and with gradients for every input where there are any, as a function of plain tensors."""
+    if not differentiable:
+        return lambda *inputs: flat(fn(*inputs))
+
+    def step(*inputs):
+        leaves = [t.detach().requires_grad_(True) for t in inputs]
+        outs = flat(fn(*leaves))
+        seeds = [torch.ones_like(o) * 0.5 for o in outs]
+        return [o.detach() for o in outs] + list(torch.autograd.grad(outs, leaves, seeds))
+
+    return step
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_traced_program_computes_on_other_inputs(ck, name):
+    """A graph recorded below autograd holds the kernels, not only their allocations."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    fn, inputs = calls(ck)[name]
+    step = step_of(fn, name in DIFFERENTIABLE)
+    graph = make_fx(step)(*inputs)
+    for seed in (0, 40):
+        _, others = calls(ck, seed)[name]
+        want = step(*others)
+        filler = [torch.full((64, 64), float("nan"), device=DEV) for _ in range(8)]
+        del filler  # what memory the replay gets holds something else
+        got = graph(*others)
+        assert len(want) == len(got)
+        for a, b in zip(want, got):
+            assert a.dtype == b.dtype and torch.equal(a.float(), b.float())
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_dispatch_modes_see_forward_and_backward(ck, name):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.names = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    fn, inputs = calls(ck)[name]
+    leaves = [t.clone().requires_grad_(name in DIFFERENTIABLE) for t in inputs]
+    plain = flat(fn(*leaves))
+    with Seen() as forward:
+        outs = flat(fn(*leaves))
+    assert any(n.startswith("coda_b200") for n in forward.names), forward.names
+    for a, b in zip(plain, outs):
+        assert torch.equal(a.detach().float(), b.detach().float())
+    if name in DIFFERENTIABLE:
+        seeds = [torch.ones_like(o) for o in plain]
+        want = torch.autograd.grad(plain, leaves, seeds)  # the forward ran outside of the mode
+        with Seen() as backward:
+            got = torch.autograd.grad(outs, leaves, seeds)
+        assert any(n.startswith("coda_b200") for n in backward.names), backward.names
+        for a, b in zip(want, got):
+            assert torch.equal(a, b)
+        outs = flat(fn(*leaves))
+        with Seen() as backward:
+            torch.autograd.grad(outs, leaves, seeds)
+        assert any(n.startswith("coda_b200") for n in backward.names), backward.names
+
+
+def test_selective_checkpointing_runs_the_policy(ck):
+    """A policy that keeps the norm's outputs finds the norm, and the gradients are those without checkpointing."""
+    from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selective_checkpoint_contexts
+
+    x, res, w = (randn(*s, seed=i).requires_grad_(True) for i, s in enumerate(((24, 64), (24, 64), (64,))))
+    rng, asked = rng_state(), []
+
+    def block(x, res, w):
+        out, h = ck.add_rms_norm(x, res, w, EPS, p=0.2, rng=rng)
+        return torch.sin(ck.dropout(out, 0.1, rng, stream=1).float()) + h.float()
+
+    def policy(ctx, op, *args, **kwargs):
+        asked.append(str(op))
+        return CheckpointPolicy.MUST_SAVE if str(op).startswith("coda_b200") else CheckpointPolicy.PREFER_RECOMPUTE
+
+    def context():
+        return create_selective_checkpoint_contexts(policy)
+
+    want = torch.autograd.grad(block(x, res, w).sum(), (x, res, w))
+    got = torch.autograd.grad(checkpoint(block, x, res, w, use_reentrant=False, context_fn=context).sum(), (x, res, w))
+    assert any(n.startswith("coda_b200") for n in asked)
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
+def test_shapes_without_a_device(ck):
+    """Fake tensors: shapes, types and devices of the row operators without a launch."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode() as mode:
+        x = torch.empty(6, 5, 64, dtype=torch.bfloat16, device=DEV)
+        w = torch.empty(64, dtype=torch.bfloat16, device=DEV)
+        rng = torch.empty(2, dtype=torch.int64, device=DEV)
+        assert ck.dropout(x, 0.5, rng).shape == x.shape
+        out, h = ck.add_rms_norm(x, x, w, EPS, p=0.5, rng=rng)
+        assert out.shape == h.shape == x.shape and out.dtype == x.dtype and out.device == x.device
+        assert ck.rms_norm(x, w, EPS).shape == x.shape
+        q, scale, h = ck.add_rms_norm_e4m3(x, x, w, EPS)
+        assert q.shape == x.shape and q.dtype == torch.float8_e4m3fn and scale.shape == (6, 5) and scale.dtype == torch.float32
+        leaf = x.clone().requires_grad_(True)
+        (grad,) = torch.autograd.grad(ck.rms_norm(leaf, w, EPS).sum(), leaf)
+        assert grad.shape == x.shape
+
+
+def test_recorded_loss_keeps_its_way_when_options_change(ck):
+    """Whether the rows that count are put first is decided when a program is recorded, for forward and backward together."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    g = torch.Generator().manual_seed(0)
+    M, K, V = 1500, 2048, 8195
+    x, w = (torch.randn(*s, generator=g).bfloat16().to(DEV) for s in ((M, K), (V, K)))
+    w *= K**-0.5
+    target = torch.randint(0, V, (M,), generator=g, dtype=torch.int32).to(DEV)
+    target[::3] = -100
+    assert ck._lib.lib.coda_b200_ce_compacts(M, V, K) == 1
+    step = step_of(lambda x, w: ck.linear_cross_entropy_pieces(x, w, target, piece=3000), True)
+    for recorded, later in ((1, 0), (0, 1)):
+        ck.set_option("ce_compact", recorded)
+        try:
+            want = step(x, w)
+            graph = make_fx(step)(x, w)
+            ck.set_option("ce_compact", later)
+            for a, b in zip(want, graph(x, w)):
+                assert torch.equal(a, b)
+        finally:
+            ck.set_option("ce_compact", 1)
