@@ -70,6 +70,9 @@ def _ce_scatter_out(rows: Tensor, position: Tensor, dx: Tensor) -> None:
 def _gemm_live_out(grad: Tensor, n: int, B: Tensor, C: Optional[Tensor], alpha: Tensor, live: Tensor, along_depth: bool, out: Tensor) -> None:
     """``grad[:, :n] @ B`` over the counted rows, or ``grad[:, :n]^T @ B`` summed over them."""
     M, N = grad.shape[0], B.shape[1]
+    if not along_depth and C is None and lib.coda_b200_gemm_workspace_bytes(M, N, n) > 0:  # few tiles, cut along the contraction: all rows
+        gemm(grad[:, :n], B, out=out, alpha=alpha)
+        return
     check(
         lib.coda_b200_gemm_live(grad.data_ptr(), grad.shape[1], B.data_ptr(), N, _ptr(C), out.data_ptr(), N, int(out.dtype == torch.float32),
                                 alpha.data_ptr(), live.data_ptr(), int(along_depth), n if along_depth else M, N, M if along_depth else n,
@@ -127,9 +130,14 @@ def _require_ce(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int) ->
     _require(-(2**31) <= ignore_index < 2**31, "ignore_index must fit int32")
 
 
+@torch.compiler.assume_constant_result
+def _options_allow_compacting() -> bool:
+    return bool(lib.coda_b200_ce_compacts(1 << 20, 1 << 20, 1 << 10))
+
+
 def _compacts(M: int, V: int, K: int) -> bool:
-    # (a traced caller keeps all rows: the library cannot be asked there)
-    return M > 0 and not torch.compiler.is_compiling() and bool(lib.coda_b200_ce_compacts(M, V, K))
+    """``coda_b200_ce_compacts`` in a form that can be traced.  A compiled program keeps the options it was traced with."""
+    return M > 0 and V >= 8192 and 2 * M * V * K >= 50_000_000_000 and _options_allow_compacting()
 
 
 def ce_pieces_forward(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, mean: bool):
@@ -188,9 +196,7 @@ def ce_pieces_backward(dloss: Tensor, inv_count: Tensor, lse: Tensor, x: Tensor,
         else:
             if need_dw:
                 _gemm_live_out(g, n, x, None, alpha, live, True, dw[c0:c0 + n])
-            if need_dx and c0 == 0 and lib.coda_b200_gemm_workspace_bytes(M, K, n) > 0:  # few tiles, cut along the contraction: all rows
-                gemm(g[:, :n], w, out=dx32 if n < V else dx, alpha=alpha)
-            elif need_dx:
+            if need_dx:
                 _gemm_live_out(g, n, w, sum_so_far, alpha, live, False, dx32 if c0 + n < V else dx)
     if need_dx and live is not None:
         rows, dx = dx, torch.empty_like(dx)

@@ -1,5 +1,5 @@
 """``linear_cross_entropy_pieces`` where labels are missing or wrong: gradients of a batch without a label, labels outside the
-vocabulary, ignored rows that hold anything.  Each at a size whose products run over all rows and at one where the rows that count are put first, through the
+vocabulary, ignored rows that hold anything, and traced programs.  Each at a size whose products run over all rows and at one where the rows that count are put first, through the
 compiled operators and through the Python nodes."""
 
 from importlib import import_module
@@ -95,3 +95,30 @@ def test_ignored_rows_may_hold_anything(ck, M, K, V, piece, binding):
     # the weight's gradient alone, and an x that needs none
     loss = fn(bad.detach(), w, t, "mean", piece)
     assert torch.equal(torch.autograd.grad(loss, w)[0], grads[1])
+
+
+def test_compiled_program_leaves_ignored_rows_out(ck):
+    """Traced, the loss takes the same rows into its products as an eager call does: the same bits, and ignored rows may hold
+    anything."""
+    M, K, V, piece = SIZES[1]
+    x, w, t = make(M, K, V)
+    t[torch.rand(M, generator=torch.Generator().manual_seed(1)).to(DEV) < 0.4] = -100
+
+    def step(x, w, t):
+        return ck.linear_cross_entropy_pieces(x, w, t, piece=piece)
+
+    eager = step(x, w, t)
+    want = (eager.detach(), *torch.autograd.grad(eager, (x, w)))
+    bad = torch.where((t == -100)[:, None], torch.full_like(x, float("nan")), x.detach()).requires_grad_(True)
+    traced = torch.compile(step, fullgraph=True, dynamic=False)
+    for rows in (x, bad):
+        loss = traced(rows, w, t)
+        for a, b in zip((loss.detach(), *torch.autograd.grad(loss, (rows, w))), want):
+            assert torch.equal(a, b)
+    with torch.no_grad():
+        assert torch.equal(traced(bad, w, t), want[0])
+    # labels of another call
+    t2 = t.roll(7)
+    loss, plain = traced(x, w, t2), step(x, w, t2)
+    for a, b in zip(torch.autograd.grad(loss, (x, w)), torch.autograd.grad(plain, (x, w))):
+        assert torch.equal(a, b)
