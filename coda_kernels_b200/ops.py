@@ -322,7 +322,7 @@ if os.environ.get("CODA_B200_DISPATCH", "native") != "ctypes":
 
     class _Native:
         """``torch.ops.coda_b200n`` with argument errors re-raised as the package's own exception type, so both bindings
-        report a rejected call the same way."""
+        report a rejected call the same way.  Errors of another kind (no memory, a CUDA error) stay what they are."""
 
         def __getattr__(self, name):
             op = getattr(torch.ops.coda_b200n, name)
@@ -331,6 +331,8 @@ if os.environ.get("CODA_B200_DISPATCH", "native") != "ctypes":
                 try:
                     return op(*args)
                 except RuntimeError as ex:
+                    if type(ex) is not RuntimeError:
+                        raise
                     raise _lib_module.CodaB200Error(str(ex).split("\n")[0]) from None
 
             setattr(self, name, call)

@@ -8,6 +8,7 @@ more than that.  While ``torch.compile`` traces, or with ``CODA_B200_DISPATCH`` 
 
 from __future__ import annotations
 
+import re
 from typing import Optional
 
 import torch
@@ -22,19 +23,22 @@ E4M3 = torch.float8_e4m3fn
 
 
 _native_ops: dict = {}
+_REFUSED = re.compile(r" failed \(code -?\d+\): ")  # how the dispatch layer reports a library call's status, as ``check`` does
 
 
 def call_native(name: str, *args):
-    """An operator of the compiled dispatch layer; what the library refuses is raised as the package's own exception."""
+    """An operator of the compiled dispatch layer; what the library refuses is raised as the package's own exception, all else
+    (a refused argument, no memory, a CUDA error) as it is."""
     op = _native_ops.get(name)
     if op is None:
         op = _native_ops[name] = getattr(torch.ops.coda_b200n, name).default
     try:
         return op(*args)
-    except NotImplementedError:
-        raise
     except RuntimeError as ex:
-        raise CodaB200Error(str(ex).split("\n")[0]) from None
+        text = str(ex).split("\n")[0]
+        if type(ex) is RuntimeError and _REFUSED.search(text):
+            raise CodaB200Error(text) from ex
+        raise
 
 
 def _ptr(t: Optional[Tensor]):
