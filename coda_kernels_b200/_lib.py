@@ -88,6 +88,7 @@ SIGNATURES = {
     "coda_b200_ce_compact": (_I, [_P, _P, _I, _P, _P, _P, _P, _I, _I, _P]),
     "coda_b200_ce_mask": (_I, [_P, _P, _I, _P, _I, _I, _P]),
     "coda_b200_ce_scatter": (_I, [_P, _P, _P, _I, _I, _P]),
+    "coda_b200_gemm_ragged": (_I, [_P, _L, _L, _P, _L, _L, _P, _P, _L, _I, _I, _I, _I, _P, _P, _L, _P, _P]),
     "coda_b200_gemm_live": (_I, [_P, _L, _P, _L, _P, _P, _L, _I, _P, _P, _I, _I, _I, _I, _P, _P]),
     "coda_b200_ce_loss": (_I, [_P, _L, _L, _P, _L, _L, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P]),
     "coda_b200_ce_alpha": (_I, [_P, _P, _P, _P]),

@@ -192,7 +192,8 @@ namespace {
 template <class Epi, int kLive, bool kAMn, bool kBMn>
 int launch_live(const void* a, long long lda, const void* b, long long ldb, int M, int N, int K, typename Epi::Params& ep, const int* live,
                 int* dev_status, cudaStream_t stream) {
-  const LaunchOptions opt = launch_options();
+  LaunchOptions opt = launch_options();
+  opt.ragged = true;  // a piece of the vocabulary may have any number of columns
   if (opt.cta_group != 2) return fail(kBadArgument, "products of counted rows are built for CTA pairs only (cta_group = 2)");
   if (M <= 0 || N <= 0 || K <= 0) return fail(kBadArgument, "GEMM extents must be positive");
   if (dev_status == nullptr) return fail(kBadArgument, "device status word is required");

@@ -91,12 +91,13 @@ inline EncodeTiledFn encode_tiled_fn() {
 
 // bf16 matrix with `inner` contiguous elements per line and `outer` lines
 // `ld` elements apart; box = 64 x box_outer, 128-byte swizzle, zero fill.
-// `inner` may be any length (elements beyond it read as zero); only the lines must start on 16-byte boundaries.
-inline int make_tmap_bf16(CUtensorMap* m, const void* ptr, long long inner, long long outer, long long ld, int box_outer) {
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (!fn) return fail(kNoDriverEntry, "cuTensorMapEncodeTiled not available from the CUDA driver");
+// `ragged`: `inner` may be any length (elements beyond it read as zero); the lines still start on 16-byte boundaries.
+inline int make_tmap_bf16(CUtensorMap* m, const void* ptr, long long inner, long long outer, long long ld, int box_outer, bool ragged = false) {
   if ((reinterpret_cast<uintptr_t>(ptr) & 15u) != 0) return fail(kBadArgument, "operand base address must be 16-byte aligned");
   if (outer > 1 && (ld * 2) % 16 != 0) return fail(kBadArgument, "operand leading dimension must be a multiple of 8 elements");
+  if (!ragged && inner % 8 != 0) return fail(kBadArgument, "operand contiguous extent must be a multiple of 8 elements");
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return fail(kNoDriverEntry, "cuTensorMapEncodeTiled not available from the CUDA driver");
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
   cuuint64_t strides[1] = {static_cast<cuuint64_t>((outer > 1 ? ld : (inner + 7) / 8 * 8) * 2)};
   cuuint32_t box[2] = {64u, static_cast<cuuint32_t>(box_outer)};
@@ -150,6 +151,7 @@ inline int sm_count() {
 // The options one launch works with, read once.
 struct LaunchOptions {
   int cta_group, group_m, max_ctas, tile_n, epi_tma, probe_ld_kb, probe_st_kb, split_tail;
+  bool ragged = false;  // set by the launches whose operands may have any contiguous extent
 };
 inline LaunchOptions launch_options() {
   const Options& o = options();
@@ -258,11 +260,11 @@ int launch_gemm_cfg(const void* a_ptr, long long lda, const void* b_ptr, long lo
   CUtensorMap ta, tb;
   int rc;
   // K-major: lines run along K; box = 64 k x (rows of the tile).  MN-major: lines run along M/N; box = 64 x 64 k.
-  if (!kBMn) rc = make_tmap_bf16(&tb, b_ptr, K, N, ldb, Cfg::kBNcta);
-  else rc = make_tmap_bf16(&tb, b_ptr, N, K, ldb, kBlockK);
+  if (!kBMn) rc = make_tmap_bf16(&tb, b_ptr, K, N, ldb, Cfg::kBNcta, opt.ragged);
+  else rc = make_tmap_bf16(&tb, b_ptr, N, K, ldb, kBlockK, opt.ragged);
   if (rc != kOk) return rc;
-  if (!kAMn) rc = make_tmap_bf16(&ta, a_ptr, K, M, lda, kBlockM);
-  else rc = make_tmap_bf16(&ta, a_ptr, M, K, lda, kBlockK);
+  if (!kAMn) rc = make_tmap_bf16(&ta, a_ptr, K, M, lda, kBlockM, opt.ragged);
+  else rc = make_tmap_bf16(&ta, a_ptr, M, K, lda, kBlockK, opt.ragged);
   if (rc != kOk) return rc;
 
   GemmShape shape;
@@ -370,14 +372,15 @@ inline int choose_tile_n(int M, int N, const LaunchOptions& opt, bool has64) {
 // The caller has encoded the output tensor maps of `ep`; `ep.use_tma` is filled in here from the options.
 template <class Epi, int kAllowMajors, int kNarrow = 0>
 int launch_gemm(const Operand& A, const Operand& B, int M, int N, int K, typename Epi::Params& ep, int* status,
-                cudaStream_t stream) {
+                cudaStream_t stream, bool ragged = false) {
   if (M <= 0 || N <= 0 || K <= 0) return fail(kBadArgument, "GEMM extents must be positive");
   if (status == nullptr) return fail(kBadArgument, "device status word is required");
   bool a_mn, b_mn;
   long long lda, ldb;
   if (!classify(A, M, K, &a_mn, &lda)) return fail(kBadLayout, "A must be contiguous along one of its two dimensions");
   if (!classify(B, N, K, &b_mn, &ldb)) return fail(kBadLayout, "B must be contiguous along one of its two dimensions");
-  const LaunchOptions opt = launch_options();
+  LaunchOptions opt = launch_options();
+  opt.ragged = ragged;
   ep.use_tma = opt.epi_tma;
   const bool two = opt.cta_group == 2;
   int tile_n = 256;

@@ -46,7 +46,7 @@ namespace {
 template <typename OutT, Act kAct>
 int run_store(const void* A, int64_t asm_, int64_t ask, const void* B, int64_t bsk, int64_t bsn, const void* C, int64_t ldc,
               int c_is_fp32, void* D, int64_t ldd, int M, int N, int K, const float* alpha, int* dev_status, void* stream,
-              void* workspace = nullptr, int64_t workspace_bytes = 0) {
+              void* workspace = nullptr, int64_t workspace_bytes = 0, bool ragged = false) {
   if (D == nullptr || A == nullptr || B == nullptr) return fail(kBadArgument, "NULL matrix pointer");
   if ((reinterpret_cast<uintptr_t>(D) & 15u) != 0) return fail(kBadArgument, "D must be 16-byte aligned");
   if (N % 8 != 0 || ldd % 8 != 0 || ldd < N) return fail(kBadArgument, "N and ldd must be multiples of 8 with ldd >= N");
@@ -68,7 +68,7 @@ int run_store(const void* A, int64_t asm_, int64_t ask, const void* B, int64_t b
   if (rc != kOk) return rc;
   Operand a{A, asm_, ask};
   Operand b{B, bsn, bsk};
-  return launch_gemm<EpiStore<OutT, kAct>, 3, 2>(a, b, M, N, K, ep, dev_status, static_cast<cudaStream_t>(stream));
+  return launch_gemm<EpiStore<OutT, kAct>, 3, 2>(a, b, M, N, K, ep, dev_status, static_cast<cudaStream_t>(stream), ragged);
 }
 }  // namespace
 
@@ -103,6 +103,17 @@ extern "C" int coda_b200_gemm_ws(const void* A, int64_t a_stride_m, int64_t a_st
                                         dev_status, stream, workspace, workspace_bytes);
   return run_store<__nv_bfloat16, Act::kNone>(A, a_stride_m, a_stride_k, B, b_stride_k, b_stride_n, nullptr, 0, 0, D, ldd, M, N, K,
                                               alpha, dev_status, stream, workspace, workspace_bytes);
+}
+
+extern "C" int coda_b200_gemm_ragged(const void* A, int64_t a_stride_m, int64_t a_stride_k, const void* B, int64_t b_stride_k,
+                                     int64_t b_stride_n, const float* C, void* D, int64_t ldd, int d_is_fp32, int M, int N, int K,
+                                     const float* alpha, void* workspace, int64_t workspace_bytes, int* dev_status, void* stream) {
+  if (workspace_bytes < 0) return fail(kBadArgument, "workspace_bytes must not be negative");
+  if (d_is_fp32)
+    return run_store<float, Act::kNone>(A, a_stride_m, a_stride_k, B, b_stride_k, b_stride_n, C, ldd, 1, D, ldd, M, N, K, alpha, dev_status,
+                                        stream, workspace, workspace_bytes, true);
+  return run_store<__nv_bfloat16, Act::kNone>(A, a_stride_m, a_stride_k, B, b_stride_k, b_stride_n, C, ldd, 1, D, ldd, M, N, K, alpha,
+                                              dev_status, stream, workspace, workspace_bytes, true);
 }
 
 extern "C" int coda_b200_gemm(const void* A, int64_t a_stride_m, int64_t a_stride_k, const void* B, int64_t b_stride_k,

@@ -538,6 +538,18 @@ std::tuple<Tensor, Tensor, Tensor> run_ce(const CeRows& r, const Tensor& weight,
   return {loss, inv_count, lse};
 }
 
+// out = alpha A @ B (+ C, fp32 of out's layout) for operands of any contiguous extent
+void gemm_ragged(const Tensor& A, const Tensor& B, const Tensor& out, const Tensor& alpha, const OptTensor& C, const Tensor& status) {
+  const int M = static_cast<int>(A.size(0)), N = static_cast<int>(B.size(1)), K = static_cast<int>(A.size(1));
+  const int64_t ws_bytes = C.has_value() ? 0 : coda_b200_gemm_workspace_bytes(M, N, K);
+  Tensor ws;
+  if (ws_bytes > 0) ws = at::empty({ws_bytes / 4}, alpha.options());
+  check(coda_b200_gemm_ragged(A.data_ptr(), A.stride(0), A.stride(1), B.data_ptr(), B.stride(0), B.stride(1),
+                              C.has_value() ? C->data_ptr<float>() : nullptr, out.data_ptr(), out.stride(0), out.scalar_type() == at::kFloat,
+                              M, N, K, alpha.data_ptr<float>(), ptr_or_null(ws), ws_bytes, status_ptr(status), stream_of(A)),
+        "gemm_ragged");
+}
+
 // Walks the vocabulary in pieces of `piece` columns with one [M, piece] buffer: the piece's softmax gradient, then its
 // rows of dweight, then its share of dx, summed over the pieces in fp32.
 OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tensor& lse, const CeRows& r, const Tensor& weight,
@@ -553,8 +565,8 @@ OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tens
   }
   const Tensor xs = x.as_strided({M, K}, {K, 1}), ws = weight.as_strided({V, K}, {K, 1});
   const Tensor dl = dloss.to(at::kFloat);
-  const OptTensor alpha = at::empty({1}, inv_count.options());
-  check(coda_b200_ce_alpha(dl.data_ptr<float>(), inv_count.data_ptr<float>(), alpha->data_ptr<float>(), stream_of(x)), "ce_alpha");
+  const Tensor alpha = at::empty({1}, inv_count.options());
+  check(coda_b200_ce_alpha(dl.data_ptr<float>(), inv_count.data_ptr<float>(), alpha.data_ptr<float>(), stream_of(x)), "ce_alpha");
   const int32_t* live = live_ptr(r.live);
   const int64_t width = std::min(piece, V), ldg = (width + 7) / 8 * 8;
   Tensor g = new_matrix(x, M, ldg, at::kBFloat16);
@@ -578,9 +590,9 @@ OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tens
     if (need_dw) {
       Tensor out = dw->narrow(0, c0, n);
       if (live == nullptr)
-        gemm_out(gp.t(), counted, out, alpha, c10::nullopt, status);
+        gemm_ragged(gp.t(), counted, out, alpha, c10::nullopt, status);
       else
-        check(coda_b200_gemm_live(gp.data_ptr(), ldg, xs.data_ptr(), K, nullptr, out.data_ptr(), K, 0, alpha->data_ptr<float>(), live, 1,
+        check(coda_b200_gemm_live(gp.data_ptr(), ldg, xs.data_ptr(), K, nullptr, out.data_ptr(), K, 0, alpha.data_ptr<float>(), live, 1,
                                   static_cast<int>(n), static_cast<int>(K), static_cast<int>(M), status_ptr(status), stream_of(x)),
               "gemm_live");
     }
@@ -591,10 +603,10 @@ OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tens
       // others is not looked at): 1003 x 1032 x 32003, 404 us a step instead of 613
       const bool cut = c0 == 0 && coda_b200_gemm_workspace_bytes(static_cast<int>(M), static_cast<int>(K), static_cast<int>(n)) > 0;
       if (live == nullptr || cut)
-        gemm_out(gp, w, out, alpha, c0 > 0 ? dx32 : c10::nullopt, status);
+        gemm_ragged(gp, w, out, alpha, c0 > 0 ? dx32 : c10::nullopt, status);
       else
         check(coda_b200_gemm_live(gp.data_ptr(), ldg, w.data_ptr(), K, c0 > 0 ? dx32->data_ptr<float>() : nullptr, out.data_ptr(), K, !last,
-                                  alpha->data_ptr<float>(), live, 0, static_cast<int>(M), static_cast<int>(K), static_cast<int>(n),
+                                  alpha.data_ptr<float>(), live, 0, static_cast<int>(M), static_cast<int>(K), static_cast<int>(n),
                                   status_ptr(status), stream_of(x)),
               "gemm_live");
     }

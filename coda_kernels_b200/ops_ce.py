@@ -13,7 +13,7 @@ from torch import Tensor
 
 from . import ops
 from ._lib import check, lib
-from .ops import _native, _noop_fake, _require, _require_cuda_bf16, _stream, gemm, lse_tiles, status_word
+from .ops import _native, _noop_fake, _require, _require_cuda_bf16, _stream, lse_tiles, status_word
 
 
 def _ptr(t: Optional[Tensor]):
@@ -66,12 +66,30 @@ def _ce_scatter_out(rows: Tensor, position: Tensor, dx: Tensor) -> None:
     check(lib.coda_b200_ce_scatter(rows.data_ptr(), position.data_ptr(), dx.data_ptr(), rows.shape[0], rows.shape[1], _stream(rows)), "ce_scatter")
 
 
+@torch.library.custom_op("coda_b200::gemm_ragged_out", mutates_args=("out",), device_types="cuda")
+def _gemm_ragged_out(A: Tensor, B: Tensor, C: Optional[Tensor], alpha: Tensor, out: Tensor) -> None:
+    """``out = alpha A @ B (+ C)`` for operands of any contiguous extent; ``C`` is fp32 and laid out as ``out``."""
+    _gemm_ragged(A, B, C, alpha, out)
+
+
+def _gemm_ragged(A: Tensor, B: Tensor, C: Optional[Tensor], alpha: Tensor, out: Tensor) -> None:
+    (M, K), N = A.shape, B.shape[1]
+    ws_bytes = int(lib.coda_b200_gemm_workspace_bytes(M, N, K)) if C is None else 0
+    ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=A.device) if ws_bytes > 0 else None
+    check(
+        lib.coda_b200_gemm_ragged(A.data_ptr(), A.stride(0), A.stride(1), B.data_ptr(), B.stride(0), B.stride(1), _ptr(C), out.data_ptr(),
+                                  out.stride(0), int(out.dtype == torch.float32), M, N, K, alpha.data_ptr(), _ptr(ws), ws_bytes,
+                                  status_word(A.device).data_ptr(), _stream(A)),
+        "gemm_ragged",
+    )
+
+
 @torch.library.custom_op("coda_b200::gemm_live_out", mutates_args=("out",), device_types="cuda")
 def _gemm_live_out(grad: Tensor, n: int, B: Tensor, C: Optional[Tensor], alpha: Tensor, live: Tensor, along_depth: bool, out: Tensor) -> None:
     """``grad[:, :n] @ B`` over the counted rows, or ``grad[:, :n]^T @ B`` summed over them."""
     M, N = grad.shape[0], B.shape[1]
     if not along_depth and C is None and lib.coda_b200_gemm_workspace_bytes(M, N, n) > 0:  # few tiles, cut along the contraction: all rows
-        gemm(grad[:, :n], B, out=out, alpha=alpha)
+        _gemm_ragged(grad[:, :n], B, None, alpha, out)
         return
     check(
         lib.coda_b200_gemm_live(grad.data_ptr(), grad.shape[1], B.data_ptr(), N, _ptr(C), out.data_ptr(), N, int(out.dtype == torch.float32),
@@ -86,7 +104,7 @@ def _ce_alpha_out(dloss: Tensor, inv_count: Tensor, alpha: Tensor) -> None:
     check(lib.coda_b200_ce_alpha(dloss.data_ptr(), inv_count.data_ptr(), alpha.data_ptr(), _stream(alpha)), "ce_alpha")
 
 
-for _op in (_ce_loss_out, _ce_alpha_out, _gemm_softmax_grad_out, _ce_compact_out, _ce_mask_out, _ce_scatter_out, _gemm_live_out):
+for _op in (_ce_loss_out, _ce_alpha_out, _gemm_softmax_grad_out, _ce_compact_out, _ce_mask_out, _ce_scatter_out, _gemm_ragged_out, _gemm_live_out):
     _op.register_fake(_noop_fake)
 
 
@@ -190,9 +208,9 @@ def ce_pieces_backward(dloss: Tensor, inv_count: Tensor, lse: Tensor, x: Tensor,
         if live is None:
             gp = g[:, :n]
             if need_dw:
-                gemm(gp.mT, counted, out=dw[c0:c0 + n], alpha=alpha)
+                _gemm_ragged_out(gp.mT, counted, None, alpha, dw[c0:c0 + n])
             if need_dx:
-                gemm(gp, w, out=dx32 if c0 + n < V else dx, alpha=alpha, C=sum_so_far)
+                _gemm_ragged_out(gp, w, sum_so_far, alpha, dx32 if c0 + n < V else dx)
         else:
             if need_dw:
                 _gemm_live_out(g, n, x, None, alpha, live, True, dw[c0:c0 + n])

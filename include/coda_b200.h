@@ -420,6 +420,12 @@ int coda_b200_gemm_softmax_grad(const void* A, int64_t a_stride_m, int64_t a_str
                                 int64_t b_stride_n, const float* lse, const int32_t* target, int ignore_index, int col0,
                                 const int32_t* live, void* G, int64_t ldg, int M, int N, int K, int* dev_status, void* stream);
 
+/* coda_b200_gemm_ws (+ C, fp32 with D's leading dimension, or NULL) for operands of any contiguous extent, which the other GEMMs
+ * want a multiple of 8: a piece of the vocabulary may have any number of columns.  Lines still start on 16-byte boundaries. */
+int coda_b200_gemm_ragged(const void* A, int64_t a_stride_m, int64_t a_stride_k, const void* B, int64_t b_stride_k,
+                          int64_t b_stride_n, const float* C, void* D, int64_t ldd, int d_is_fp32, int M, int N, int K,
+                          const float* alpha, void* workspace, int64_t workspace_bytes, int* dev_status, void* stream);
+
 /* Leaving ignored rows out of the products.  coda_b200_ce_compact puts the rows of x [M, K] (dense bf16) that count first, in
  * their order: rows [M, K], labels int32 [M] (ignore_index behind them), position int32 [M] (where a row went, -1: ignored) and
  * live, a device int32: how many count.  Row operands are zero from there to the next multiple of 64 and undefined beyond.
