@@ -869,10 +869,12 @@ inline RowPlan row_plan(int64_t rows, int64_t cols, int dtype, bool backward, bo
   p.grid = std::min(need, cap);
   return p;
 }
-// the widest backward grid of any type, with and without dropout
+// the widest backward grid of any type, with and without dropout: each block leaves a partial row
 inline int64_t most_partial_rows(int64_t rows, int64_t cols) {
-  const int64_t a = row_plan(rows, cols, 0, true, false).grid, b = row_plan(rows, cols, 2, true, false).grid;
-  return a > b ? a : b;
+  int64_t most = 0;
+  for (const int dtype : {0, 1, 2})
+    for (const bool drop : {false, true}) most = std::max(most, row_plan(rows, cols, dtype, true, drop).grid);
+  return most;
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
