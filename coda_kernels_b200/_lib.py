@@ -86,6 +86,7 @@ SIGNATURES = {
     "coda_b200_gemm_e4m3": (_I, [_P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P, _L, _P, _P]),
     "coda_b200_ce_compacts": (_I, [_I, _I, _I]),
     "coda_b200_ce_compact": (_I, [_P, _P, _I, _P, _P, _P, _P, _I, _I, _P]),
+    "coda_b200_ce_gather": (_I, [_P, _P, _P, _P, _I, _I, _P]),
     "coda_b200_ce_mask": (_I, [_P, _P, _I, _P, _I, _I, _P]),
     "coda_b200_ce_scatter": (_I, [_P, _P, _P, _I, _I, _P]),
     "coda_b200_gemm_ragged": (_I, [_P, _L, _L, _P, _L, _L, _P, _P, _L, _I, _I, _I, _I, _P, _P, _L, _P, _P]),

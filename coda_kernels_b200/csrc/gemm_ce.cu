@@ -164,9 +164,16 @@ extern "C" int coda_b200_ce_compact(const void* x, const int32_t* target, int ig
   if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows)) & 15u) != 0) return fail(kBadArgument, "matrices must be 16-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   ce_positions_kernel<<<1, 1024, 0, st>>>(target, ignore_index, position, labels, live, M);
-  int rc = launch_check("cross-entropy positions launch");
-  if (rc != kOk) return rc;
-  ce_gather_kernel<<<M, 256, 0, st>>>(static_cast<const uint4*>(x), position, live, static_cast<uint4*>(rows), M, K / 8);
+  const int rc = launch_check("cross-entropy positions launch");
+  return rc != kOk ? rc : coda_b200_ce_gather(x, position, live, rows, M, K, stream);
+}
+
+extern "C" int coda_b200_ce_gather(const void* x, const int32_t* position, const int32_t* live, void* rows, int M, int K, void* stream) {
+  if (!x || !position || !live || !rows) return fail(kBadArgument, "NULL pointer");
+  if (M <= 0 || K <= 0 || K % 8 != 0) return fail(kBadArgument, "M and K must be positive, K a multiple of 8");
+  if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows)) & 15u) != 0) return fail(kBadArgument, "matrices must be 16-byte aligned");
+  ce_gather_kernel<<<M, 256, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const uint4*>(x), position, live, static_cast<uint4*>(rows), M,
+                                                                     K / 8);
   return launch_check("cross-entropy gather launch");
 }
 

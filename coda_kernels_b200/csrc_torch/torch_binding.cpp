@@ -551,7 +551,9 @@ void gemm_ragged(const Tensor& A, const Tensor& B, const Tensor& out, const Tens
 }
 
 // Walks the vocabulary in pieces of `piece` columns with one [M, piece] buffer: the piece's softmax gradient, then its
-// rows of dweight, then its share of dx, summed over the pieces in fp32.
+// rows of dweight, then its share of dx, summed over the pieces in fp32.  `r` has the forward's x, and its target or, with live,
+// the labels put first; the rows are put first again here (that copy is small beside the products, but not beside what the node
+// keeps).
 OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tensor& lse, const CeRows& r, const Tensor& weight,
                         int64_t ignore_index, int64_t piece, bool need_dx, bool need_dw, const Tensor& status) {
   const Tensor& x = r.x;
@@ -563,11 +565,18 @@ OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tens
     if (need_dw) dw = at::zeros_like(weight);
     return {dx, dw};
   }
-  const Tensor xs = x.as_strided({M, K}, {K, 1}), ws = weight.as_strided({V, K}, {K, 1});
+  const int32_t* live = live_ptr(r.live);
+  Tensor xs = x.as_strided({M, K}, {K, 1});
+  const Tensor ws = weight.as_strided({V, K}, {K, 1});
+  if (live != nullptr) {
+    xs = new_matrix(x, M, K, at::kBFloat16);
+    check(coda_b200_ce_gather(x.data_ptr(), r.position.data_ptr<int32_t>(), live, xs.data_ptr(), static_cast<int>(M), static_cast<int>(K),
+                              stream_of(x)),
+          "ce_gather");
+  }
   const Tensor dl = dloss.to(at::kFloat);
   const Tensor alpha = at::empty({1}, inv_count.options());
   check(coda_b200_ce_alpha(dl.data_ptr<float>(), inv_count.data_ptr<float>(), alpha.data_ptr<float>(), stream_of(x)), "ce_alpha");
-  const int32_t* live = live_ptr(r.live);
   const int64_t width = std::min(piece, V), ldg = (width + 7) / 8 * 8;
   Tensor g = new_matrix(x, M, ldg, at::kBFloat16);
   if (need_dx) dx = new_matrix(x, M, K, at::kBFloat16);
@@ -611,12 +620,11 @@ OptPair run_ce_backward(const Tensor& dloss, const Tensor& inv_count, const Tens
               "gemm_live");
     }
   }
-  if (need_dx && live != nullptr) {
-    Tensor out = new_matrix(x, M, K, at::kBFloat16);
-    check(coda_b200_ce_scatter(dx->data_ptr(), r.position.data_ptr<int32_t>(), out.data_ptr(), static_cast<int>(M), static_cast<int>(K),
+  if (need_dx && live != nullptr) {  // into the memory of the rows, which are not needed any more
+    check(coda_b200_ce_scatter(dx->data_ptr(), r.position.data_ptr<int32_t>(), xs.data_ptr(), static_cast<int>(M), static_cast<int>(K),
                                stream_of(x)),
           "ce_scatter");
-    dx = out;
+    dx = xs;
   }
   return {dx, dw};
 }
@@ -634,21 +642,21 @@ inline void require_ce(const Tensor& x, const Tensor& weight, const Tensor& targ
   TORCH_CHECK_VALUE(x.size(0) <= INT_MAX && weight.size(0) <= INT_MAX - 256, "extents must fit 31 bits");
 }
 
-// (loss, inv_count, lse, and with `compact` the rows that count, put first, their labels, position and live).  Whether to is
+// (loss, inv_count, lse, and with `compact` the counted rows' labels, put first as lse is, position and live).  Whether to is
 // the caller's to say: a recorded program keeps what it was recorded with, whatever the options are when it runs.
-std::tuple<Tensor, Tensor, Tensor, OptTensor, OptTensor, OptTensor, OptTensor> ce_pieces_fwd(const Tensor& x, const Tensor& weight,
-                                                                                            const Tensor& target, int64_t ignore_index,
-                                                                                            bool mean, bool compact, const Tensor& status) {
+std::tuple<Tensor, Tensor, Tensor, OptTensor, OptTensor, OptTensor> ce_pieces_fwd(const Tensor& x, const Tensor& weight, const Tensor& target,
+                                                                                 int64_t ignore_index, bool mean, bool compact,
+                                                                                 const Tensor& status) {
   require_ce(x, weight, target, ignore_index);
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::cuda::CUDAGuard guard(x.device());
   const CeRows r = ce_rows(aligned16(x), target.contiguous(), ignore_index, compact && x.size(0) > 0);
   auto [loss, inv_count, lse] = run_ce(r, aligned16(weight), ignore_index, mean, status);
-  if (!r.live.defined()) return {loss, inv_count, lse, c10::nullopt, c10::nullopt, c10::nullopt, c10::nullopt};
-  return {loss, inv_count, lse, r.x, r.target, r.position, r.live};
+  if (!r.live.defined()) return {loss, inv_count, lse, c10::nullopt, c10::nullopt, c10::nullopt};
+  return {loss, inv_count, lse, r.target, r.position, r.live};
 }
 
-// x and target: those of the forward, or the rows and labels it put first, with position and live
+// x: the forward's; target too, or the labels it put first, with position and live
 OptPair ce_pieces_bwd(const Tensor& dloss, const Tensor& inv_count, const Tensor& lse, const Tensor& x, const Tensor& weight,
                       const Tensor& target, const OptTensor& position, const OptTensor& live, int64_t ignore_index, int64_t piece, bool need_dx,
                       bool need_dw, const Tensor& status) {
@@ -759,12 +767,12 @@ class CePiecesNode : public torch::autograd::Function<CePiecesNode> {
  public:
   static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& weight_in, const Tensor& target_in, int64_t ignore_index,
                         bool mean, int64_t piece, const Tensor& status) {
-    static const auto op = operator_named<std::tuple<Tensor, Tensor, Tensor, OptTensor, OptTensor, OptTensor, OptTensor>(
+    static const auto op = operator_named<std::tuple<Tensor, Tensor, Tensor, OptTensor, OptTensor, OptTensor>(
         const Tensor&, const Tensor&, const Tensor&, int64_t, bool, bool, const Tensor&)>("coda_b200n::ce_pieces_fwd");
     at::AutoDispatchBelowADInplaceOrView below;
     const Tensor x = x_in.contiguous(), weight = weight_in.contiguous(), target = target_in.contiguous();
-    auto [loss, inv_count, lse, rows, labels, position, live] = op.call(x, weight, target, ignore_index, mean, ce_compacts(x, weight), status);
-    ctx->save_for_backward({rows.value_or(x), weight, labels.value_or(target), lse, inv_count, position.value_or(Tensor()), live.value_or(Tensor())});
+    auto [loss, inv_count, lse, labels, position, live] = op.call(x, weight, target, ignore_index, mean, ce_compacts(x, weight), status);
+    ctx->save_for_backward({x, weight, labels.value_or(target), lse, inv_count, position.value_or(Tensor()), live.value_or(Tensor())});
     ctx->saved_data["ignore_index"] = ignore_index;
     ctx->saved_data["piece"] = piece;
     ctx->saved_data["status"] = status;
@@ -879,7 +887,7 @@ TORCH_LIBRARY(coda_b200n, m) {
   m.def("norm_bwd(Tensor? dout, Tensor? dh, Tensor h, Tensor rstd, Tensor weight, float p, Tensor? rng, int stream, bool need_dx, "
         "bool need_dres, bool need_dw) -> (Tensor?, Tensor?, Tensor?)");
   m.def("ce_pieces_fwd(Tensor x, Tensor weight, Tensor target, int ignore_index, bool mean, bool compact, Tensor status) -> "
-        "(Tensor, Tensor, Tensor, Tensor?, Tensor?, Tensor?, Tensor?)");
+        "(Tensor, Tensor, Tensor, Tensor?, Tensor?, Tensor?)");
   m.def("ce_pieces_bwd(Tensor dloss, Tensor inv_count, Tensor lse, Tensor x, Tensor weight, Tensor target, Tensor? position, Tensor? live, "
         "int ignore_index, int piece, bool need_dx, bool need_dw, Tensor status) -> (Tensor?, Tensor?)");
   m.def("rms_norm(Tensor x, Tensor weight, float eps) -> Tensor");

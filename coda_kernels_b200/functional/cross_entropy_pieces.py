@@ -1,8 +1,8 @@
 """``linear_cross_entropy_pieces``: the LM-head loss for batches whose ``[M, V]`` gradient buffer would not fit.
 
 An extension with no counterpart in the reference.  :func:`linear_cross_entropy` keeps ``softmax - onehot`` of the whole
-batch, ``2 M V`` bytes, from forward to backward.  Here the node keeps the rows' log-sum-exp (``4 M`` bytes); the
-backward walks the vocabulary in pieces, computes each piece's logits again and turns them into its part of the two
+batch, ``2 M V`` bytes, from forward to backward.  Here the node keeps the rows' log-sum-exp, and with the rows that count put
+first their labels and positions (4 bytes a row each), beside the caller's tensors; the backward walks the vocabulary in pieces, computes each piece's logits again and turns them into its part of the two
 gradients.  The price is that one product (a third more work in the backward); what it saves is everything of size
 ``M V`` but one ``[M, piece]`` buffer during the backward.
 
@@ -23,14 +23,15 @@ from ..ops_rows import _require_first_order, call_native
 
 
 class LinearCrossEntropyPieces(torch.autograd.Function):
-    """Saves the rows (``x``, or its rows that count, put first), their labels, the weight, the log-sum-exp and ``inv_count``."""
+    """Saves ``x``, the weight, the labels (those of the rows that count first, with the positions), the log-sum-exp and
+    ``inv_count``."""
 
     @staticmethod
     @input_guard
     @autocast_custom_fwd
     def forward(ctx, x, weight, target, ignore_index: int, reduction: str, piece: int) -> torch.Tensor:
-        loss, inv_count, lse, rows, labels, position, live = ce_pieces_forward(x, weight, target, ignore_index, reduction == "mean")
-        ctx.save_for_backward(rows, weight, labels, lse, inv_count, position, live)
+        loss, inv_count, lse, labels, position, live = ce_pieces_forward(x, weight, target, ignore_index, reduction == "mean")
+        ctx.save_for_backward(x, weight, labels, lse, inv_count, position, live)
         ctx.ignore_index, ctx.piece = ignore_index, piece
         return loss
 
@@ -39,9 +40,9 @@ class LinearCrossEntropyPieces(torch.autograd.Function):
     @autocast_custom_bwd
     def backward(ctx, dloss: torch.Tensor):
         _require_first_order("linear_cross_entropy_pieces")
-        rows, weight, labels, lse, inv_count, position, live = ctx.saved_tensors
+        x, weight, labels, lse, inv_count, position, live = ctx.saved_tensors
         need_dx, need_dw = ctx.needs_input_grad[:2]
-        return (*ce_pieces_backward(dloss, inv_count, lse, rows, weight, labels, position, live, ctx.ignore_index, ctx.piece, need_dx,
+        return (*ce_pieces_backward(dloss, inv_count, lse, x, weight, labels, position, live, ctx.ignore_index, ctx.piece, need_dx,
                                     need_dw), None, None, None, None)
 
 

@@ -56,6 +56,12 @@ def _ce_compact_out(x: Tensor, target: Tensor, ignore_index: int, position: Tens
     )
 
 
+@torch.library.custom_op("coda_b200::ce_gather_out", mutates_args=("rows",), device_types="cuda")
+def _ce_gather_out(x: Tensor, position: Tensor, live: Tensor, rows: Tensor) -> None:
+    check(lib.coda_b200_ce_gather(x.data_ptr(), position.data_ptr(), live.data_ptr(), rows.data_ptr(), x.shape[0], x.shape[1], _stream(x)),
+          "ce_gather")
+
+
 @torch.library.custom_op("coda_b200::ce_mask_out", mutates_args=("rows",), device_types="cuda")
 def _ce_mask_out(x: Tensor, target: Tensor, ignore_index: int, rows: Tensor) -> None:
     check(lib.coda_b200_ce_mask(x.data_ptr(), target.data_ptr(), ignore_index, rows.data_ptr(), x.shape[0], x.shape[1], _stream(x)), "ce_mask")
@@ -104,7 +110,7 @@ def _ce_alpha_out(dloss: Tensor, inv_count: Tensor, alpha: Tensor) -> None:
     check(lib.coda_b200_ce_alpha(dloss.data_ptr(), inv_count.data_ptr(), alpha.data_ptr(), _stream(alpha)), "ce_alpha")
 
 
-for _op in (_ce_loss_out, _ce_alpha_out, _gemm_softmax_grad_out, _ce_compact_out, _ce_mask_out, _ce_scatter_out, _gemm_ragged_out, _gemm_live_out):
+for _op in (_ce_loss_out, _ce_alpha_out, _gemm_softmax_grad_out, _ce_compact_out, _ce_gather_out, _ce_mask_out, _ce_scatter_out, _gemm_ragged_out, _gemm_live_out):
     _op.register_fake(_noop_fake)
 
 
@@ -117,7 +123,7 @@ if _native is not None:  # the compiled operators on fake tensors
     @torch.library.register_fake("coda_b200n::ce_pieces_fwd")
     def _(x, weight, target, ignore_index, mean, compact, status):
         f32 = dict(dtype=torch.float32)
-        rows = [x.new_empty(x.shape), *(target.new_empty(n) for n in (x.shape[0], x.shape[0], 1))] if compact else [None] * 4
+        rows = [target.new_empty(n) for n in (x.shape[0], x.shape[0], 1)] if compact else [None] * 3
         return x.new_empty((), **f32), x.new_empty((), **f32), x.new_empty(x.shape[0], **f32), *rows
 
     @torch.library.register_fake("coda_b200n::ce_pieces_bwd")
@@ -159,15 +165,15 @@ def _compacts(M: int, V: int, K: int) -> bool:
 
 
 def ce_pieces_forward(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, mean: bool):
-    """``(loss, inv_count, lse, rows, labels, position, live)``; nothing of size ``[M, V]`` is written.  ``rows`` and ``labels``
-    are ``x`` and ``target``, or, where that pays, the rows that count put first (``live`` of them, from ``position``)."""
+    """``(loss, inv_count, lse, labels, position, live)``; nothing of size ``[M, V]`` is written.  ``labels`` and ``lse`` are in the
+    order of the rows, or, where that pays, those of the rows that count come first (``live`` of them, from ``position``)."""
     _require_ce(x, weight, target, ignore_index)
     ops._debug_check_targets(target, weight.shape[0], ignore_index)
     M = x.shape[0]
     f32 = dict(dtype=torch.float32, device=x.device)
     if M == 0:  # a sum over nothing, and 0 / 0
         return (torch.full((), float("nan") if mean else 0.0, **f32), torch.zeros((), **f32),
-                torch.empty(0, **f32), x, target, None, None)
+                torch.empty(0, **f32), target, None, None)
     position = live = None
     if _compacts(M, weight.shape[0], x.shape[1]):
         rows, labels, position = torch.empty_like(x), torch.empty_like(target), torch.empty_like(target)
@@ -177,7 +183,7 @@ def ce_pieces_forward(x: Tensor, weight: Tensor, target: Tensor, ignore_index: i
     parts = torch.empty(2 * M * lse_tiles(weight.shape[0]) + 2 * M, **f32)
     lse, loss, inv_count = torch.empty(M, **f32), torch.empty((), **f32), torch.empty((), **f32)
     _ce_loss_out(x, weight, target, ignore_index, mean, live, parts, lse, loss, inv_count)
-    return loss, inv_count, lse, x, target, position, live
+    return loss, inv_count, lse, target, position, live
 
 
 def ce_pieces_backward(dloss: Tensor, inv_count: Tensor, lse: Tensor, x: Tensor, weight: Tensor, target: Tensor, position: Optional[Tensor],
@@ -192,6 +198,10 @@ def ce_pieces_backward(dloss: Tensor, inv_count: Tensor, lse: Tensor, x: Tensor,
     alpha = torch.empty(1, dtype=torch.float32, device=x.device)
     _ce_alpha_out(dloss.to(torch.float32), inv_count, alpha)
     width = min(piece, V)
+    if live is not None:  # (the node does not keep this copy: it is small beside the products, but not beside what the node keeps)
+        rows = torch.empty_like(x)
+        _ce_gather_out(x, position, live, rows)
+        x = rows
     g = torch.empty(M, -(-width // 8) * 8, dtype=x.dtype, device=x.device)
     dx = torch.empty_like(x) if need_dx else None
     dw = torch.empty_like(weight) if need_dw else None
@@ -216,7 +226,7 @@ def ce_pieces_backward(dloss: Tensor, inv_count: Tensor, lse: Tensor, x: Tensor,
                 _gemm_live_out(g, n, x, None, alpha, live, True, dw[c0:c0 + n])
             if need_dx:
                 _gemm_live_out(g, n, w, sum_so_far, alpha, live, False, dx32 if c0 + n < V else dx)
-    if need_dx and live is not None:
-        rows, dx = dx, torch.empty_like(dx)
-        _ce_scatter_out(rows, position, dx)
+    if need_dx and live is not None:  # into the memory of the rows, which are not needed any more
+        _ce_scatter_out(dx, position, x)
+        dx = x
     return dx, dw

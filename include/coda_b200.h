@@ -431,11 +431,13 @@ int coda_b200_gemm_ragged(const void* A, int64_t a_stride_m, int64_t a_stride_k,
  * live, a device int32: how many count.  Row operands are zero from there to the next multiple of 64 and undefined beyond.
  * coda_b200_ce_loss and coda_b200_gemm_softmax_grad then take rows, labels and live for x, target and NULL;
  * coda_b200_gemm_live is the product behind them, and coda_b200_ce_scatter puts rows back: dx[i] = rows[position[i]], or zero.
- * No count is read by the host.  coda_b200_ce_compacts says whether the products are large enough for it to pay (with cta_group
+ * No count is read by the host.  coda_b200_ce_gather makes `rows` again from position and live, for a backward that has not kept
+ * them.  coda_b200_ce_compacts says whether the products are large enough for it to pay (with cta_group
  * 2, which these products need). */
 int coda_b200_ce_compacts(int M, int N, int K);
 int coda_b200_ce_compact(const void* x, const int32_t* target, int ignore_index, int32_t* position, int32_t* labels, int32_t* live,
                          void* rows, int M, int K, void* stream);
+int coda_b200_ce_gather(const void* x, const int32_t* position, const int32_t* live, void* rows, int M, int K, void* stream);
 int coda_b200_ce_scatter(const void* rows, const int32_t* position, void* dx, int M, int K, void* stream);
 
 /* Where the rows are not put together: rows[i] = x[i] (dense bf16 [M, K]), zero where target[i] is ignore_index, so that whatever an

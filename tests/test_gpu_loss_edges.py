@@ -1,6 +1,7 @@
 """``linear_cross_entropy_pieces`` where labels are missing or wrong: gradients of a batch without a label, labels outside the
-vocabulary, ignored rows that hold anything, and traced programs.  Each at a size whose products run over all rows and at one where the rows that count are put first, through the
-compiled operators and through the Python nodes."""
+vocabulary, ignored rows that hold anything; traced programs, and what is held between forward and backward.  Each at a size
+whose products run over all rows and at one where the rows that count are put first, through the compiled operators and
+through the Python nodes."""
 
 from importlib import import_module
 
@@ -122,3 +123,21 @@ def test_compiled_program_leaves_ignored_rows_out(ck):
     loss, plain = traced(x, w, t2), step(x, w, t2)
     for a, b in zip(torch.autograd.grad(loss, (x, w)), torch.autograd.grad(plain, (x, w))):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("binding", ["compiled", "python"])
+def test_memory_held_between_forward_and_backward(ck, binding):
+    """Beside what the caller holds, and with the rows that count put first for the products: log-sum-exp, labels and positions,
+    4 bytes a row each, no copy of the rows (33.5 MB here)."""
+    M, K, V, piece = 4096, 4096, 8200, 4096
+    assert ck._lib.lib.coda_b200_ce_compacts(M, V, K) == 1
+    x, w, t = make(M, K, V)
+    t[::5] = -100
+    fn = loss_of(ck, binding)
+    torch.autograd.grad(fn(x, w, t, "mean", piece), (x, w))
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    loss = fn(x, w, t, "mean", piece)
+    held = torch.cuda.memory_allocated() - before
+    assert held <= 12 * M + 4096, held  # (the allocator rounds each of five tensors up to 512 bytes)
+    torch.autograd.grad(loss, (x, w))
