@@ -19,7 +19,7 @@ import torch
 from .._guards import autocast_custom_bwd, autocast_custom_fwd, input_guard
 from ..ops import _debug_check_targets, _fast, _require, lazy_status_check, status_word
 from ..ops_ce import ce_pieces_backward, ce_pieces_forward, default_piece
-from ..ops_rows import _require_first_order, call_native
+from ..ops_rows import _require_first_order, apart, call_native
 
 
 class LinearCrossEntropyPieces(torch.autograd.Function):
@@ -68,4 +68,4 @@ def linear_cross_entropy_pieces(
         lazy_status_check(x.device)
         _debug_check_targets(target, weight.shape[0], ignore_index)
         return call_native("linear_cross_entropy_pieces", x, weight, target, ignore_index, reduction == "mean", int(piece), status_word(x.device))
-    return LinearCrossEntropyPieces.apply(x, weight, target, ignore_index, reduction, int(piece))
+    return LinearCrossEntropyPieces.apply(*apart(x, weight), target, ignore_index, reduction, int(piece))

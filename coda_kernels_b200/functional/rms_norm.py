@@ -24,6 +24,7 @@ from ..ops_rows import (
     _require_weight,
     add_rmsnorm_backward,
     add_rmsnorm_forward,
+    apart,
     call_native,
     rows_e4m3,
 )
@@ -87,7 +88,7 @@ def rms_norm(x: Tensor, weight: Tensor, eps: float) -> Tensor:
     """``x * rsqrt(mean(x^2) + eps) * weight`` over the last dimension of ``x [..., N]`` (bf16, fp16 or fp32)."""
     if _fast() and x.is_cuda:
         return call_native("rms_norm", x, weight, eps)
-    return RMSNorm.apply(x, weight, float(eps))
+    return RMSNorm.apply(*apart(x, weight), float(eps))
 
 
 def add_rms_norm(x: Tensor, residual: Tensor, weight: Tensor, eps: float, p: float = 0.0, rng: Optional[Tensor] = None,
@@ -97,7 +98,7 @@ def add_rms_norm(x: Tensor, residual: Tensor, weight: Tensor, eps: float, p: flo
     ``p``, ``rng`` and ``stream`` are those of :func:`dropout`, and give the same mask."""
     if _fast() and x.is_cuda:
         return call_native("add_rms_norm", x, residual, weight, eps, p, rng, stream)
-    return AddRMSNorm.apply(x, residual, weight, float(eps), float(p), rng, int(stream))
+    return AddRMSNorm.apply(*apart(x, residual, weight), float(eps), float(p), rng, int(stream))
 
 
 def _rows_e4m3(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], eps: float):

@@ -41,6 +41,12 @@ def call_native(name: str, *args):
         raise
 
 
+def apart(*tensors: Tensor) -> tuple[Tensor, ...]:
+    """The tensors, one that is given again as a view of itself.  A traced ``autograd.Function`` that receives one tensor twice gets
+    the gradient of its first place only."""
+    return tuple(t.view_as(t) if any(t is u for u in tensors[:i]) else t for i, t in enumerate(tensors))
+
+
 def _ptr(t: Optional[Tensor]):
     return None if t is None else t.data_ptr()
 

@@ -211,3 +211,34 @@ def test_recorded_loss_keeps_its_way_when_options_change(ck):
                 assert torch.equal(a, b)
         finally:
             ck.set_option("ce_compact", 1)
+
+
+@pytest.mark.parametrize("dynamic", [False, True])
+@pytest.mark.parametrize("name", ["add_rms_norm", "rms_norm", "linear_cross_entropy_pieces"])
+def test_one_tensor_in_two_places_under_compile(ck, name, dynamic):
+    """Its gradient is the sum of both places', as an eager call gives it (two bf16 numbers, added once)."""
+    a = randn(40) if name == "rms_norm" else randn(24, 64)
+    w, rng = randn(64, seed=1), rng_state()
+    target = torch.arange(24, dtype=torch.int32, device=DEV).flip(0)
+    fn = {
+        "add_rms_norm": lambda a: ck.add_rms_norm(a, a, w, EPS, p=0.2, rng=rng),
+        "rms_norm": lambda a: ck.rms_norm(a, a, EPS),
+        "linear_cross_entropy_pieces": lambda a: ck.linear_cross_entropy_pieces(a, a, target),
+    }[name]
+    two = {
+        "add_rms_norm": lambda a, b: ck.add_rms_norm(a, b, w, EPS, p=0.2, rng=rng),
+        "rms_norm": lambda a, b: ck.rms_norm(a, b, EPS),
+        "linear_cross_entropy_pieces": lambda a, b: ck.linear_cross_entropy_pieces(a, b, target),
+    }[name]
+    a.requires_grad_(True)
+    eager = flat(fn(a))
+    seeds = [torch.ones_like(o) for o in eager]
+    (want,) = torch.autograd.grad(eager, a, seeds)
+    b, c = (a.detach().clone().requires_grad_(True) for _ in range(2))
+    assert torch.equal(want, sum(torch.autograd.grad(flat(two(b, c)), (b, c), seeds)))
+    for traced, args in ((torch.compile(fn, fullgraph=True, dynamic=dynamic), (a,)), (torch.compile(two, fullgraph=True, dynamic=dynamic), (a, a))):
+        outs = flat(traced(*args))
+        for x, y in zip(outs, eager):
+            assert torch.equal(x, y)
+        (got,) = torch.autograd.grad(outs, a, seeds)
+        assert torch.equal(got, want)
