@@ -13,16 +13,21 @@ from torch import Tensor
 
 from . import ops
 from ._lib import check, lib
-from .ops import _native, _noop_fake, _require, _require_cuda_bf16, _stream, lse_tiles, status_word
+from .ops import _aligned16, _native, _noop_fake, _require, _require_cuda_bf16, _stream, lse_tiles, status_word
 
 
 def _ptr(t: Optional[Tensor]):
     return None if t is None else t.data_ptr()
 
 
+# The ops below copy a matrix of the caller's that does not start on a 16-byte boundary, as the compiled form does: only here, where
+# they run, are addresses known (a tracer has none).
+
+
 @torch.library.custom_op("coda_b200::ce_loss_out", mutates_args=("parts", "lse", "loss", "inv_count"), device_types="cuda")
 def _ce_loss_out(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, mean: bool, live: Optional[Tensor], parts: Tensor,
                  lse: Tensor, loss: Tensor, inv_count: Tensor) -> None:
+    x, weight = _aligned16(x), _aligned16(weight)
     M, K = x.shape
     V = weight.shape[0]
     tiles = lse_tiles(V)
@@ -38,6 +43,7 @@ def _ce_loss_out(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, m
 @torch.library.custom_op("coda_b200::gemm_softmax_grad_out", mutates_args=("grad",), device_types="cuda")
 def _gemm_softmax_grad_out(x: Tensor, weight: Tensor, lse: Tensor, target: Tensor, ignore_index: int, col0: int, live: Optional[Tensor],
                            grad: Tensor) -> None:
+    x, weight = _aligned16(x), _aligned16(weight)
     M, K = x.shape
     N = weight.shape[0]
     check(
@@ -49,6 +55,7 @@ def _gemm_softmax_grad_out(x: Tensor, weight: Tensor, lse: Tensor, target: Tenso
 
 @torch.library.custom_op("coda_b200::ce_compact_out", mutates_args=("position", "labels", "live", "rows"), device_types="cuda")
 def _ce_compact_out(x: Tensor, target: Tensor, ignore_index: int, position: Tensor, labels: Tensor, live: Tensor, rows: Tensor) -> None:
+    x = _aligned16(x)
     check(
         lib.coda_b200_ce_compact(x.data_ptr(), target.data_ptr(), ignore_index, position.data_ptr(), labels.data_ptr(), live.data_ptr(),
                                  rows.data_ptr(), x.shape[0], x.shape[1], _stream(x)),
@@ -58,12 +65,14 @@ def _ce_compact_out(x: Tensor, target: Tensor, ignore_index: int, position: Tens
 
 @torch.library.custom_op("coda_b200::ce_gather_out", mutates_args=("rows",), device_types="cuda")
 def _ce_gather_out(x: Tensor, position: Tensor, live: Tensor, rows: Tensor) -> None:
+    x = _aligned16(x)
     check(lib.coda_b200_ce_gather(x.data_ptr(), position.data_ptr(), live.data_ptr(), rows.data_ptr(), x.shape[0], x.shape[1], _stream(x)),
           "ce_gather")
 
 
 @torch.library.custom_op("coda_b200::ce_mask_out", mutates_args=("rows",), device_types="cuda")
 def _ce_mask_out(x: Tensor, target: Tensor, ignore_index: int, rows: Tensor) -> None:
+    x = _aligned16(x)
     check(lib.coda_b200_ce_mask(x.data_ptr(), target.data_ptr(), ignore_index, rows.data_ptr(), x.shape[0], x.shape[1], _stream(x)), "ce_mask")
 
 
@@ -79,6 +88,7 @@ def _gemm_ragged_out(A: Tensor, B: Tensor, C: Optional[Tensor], alpha: Tensor, o
 
 
 def _gemm_ragged(A: Tensor, B: Tensor, C: Optional[Tensor], alpha: Tensor, out: Tensor) -> None:
+    B = _aligned16(B)
     (M, K), N = A.shape, B.shape[1]
     ws_bytes = int(lib.coda_b200_gemm_workspace_bytes(M, N, K)) if C is None else 0
     ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=A.device) if ws_bytes > 0 else None
@@ -93,6 +103,7 @@ def _gemm_ragged(A: Tensor, B: Tensor, C: Optional[Tensor], alpha: Tensor, out: 
 @torch.library.custom_op("coda_b200::gemm_live_out", mutates_args=("out",), device_types="cuda")
 def _gemm_live_out(grad: Tensor, n: int, B: Tensor, C: Optional[Tensor], alpha: Tensor, live: Tensor, along_depth: bool, out: Tensor) -> None:
     """``grad[:, :n] @ B`` over the counted rows, or ``grad[:, :n]^T @ B`` summed over them."""
+    B = _aligned16(B)
     M, N = grad.shape[0], B.shape[1]
     if not along_depth and C is None and lib.coda_b200_gemm_workspace_bytes(M, N, n) > 0:  # few tiles, cut along the contraction: all rows
         _gemm_ragged(grad[:, :n], B, None, alpha, out)

@@ -110,6 +110,7 @@ def _rows_e4m3_out(x: Tensor, residual: Optional[Tensor], weight: Optional[Tenso
 
 @torch.library.custom_op("coda_b200::gemm_e4m3_out", mutates_args=("out",), device_types="cuda")
 def _gemm_e4m3_out(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor, out: Tensor) -> None:
+    x, weight = _dense16(x), _dense16(weight)
     M, K = x.shape
     N = weight.shape[0]
     ws_bytes = int(lib.coda_b200_gemm_e4m3_workspace_bytes(M, N, K))
@@ -264,7 +265,7 @@ def gemm_e4m3(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor, 
     _require(weight.shape[0] > 0 and weight.shape[0] % 8 == 0, "the number of weight rows must be a positive multiple of 8")
     for name, s, n in (("x_scale", x_scale, x.shape[0]), ("weight_scale", weight_scale, weight.shape[0])):
         _require(s.dtype == torch.float32 and tuple(s.shape) == (n,), f"{name} must be float32 with one entry per row")
-    x, x_scale, weight, weight_scale = _aligned16(x), x_scale.contiguous(), _aligned16(weight), weight_scale.contiguous()
+    x, x_scale, weight, weight_scale = x.contiguous(), x_scale.contiguous(), weight.contiguous(), weight_scale.contiguous()
     out = torch.empty(x.shape[0], weight.shape[0], dtype=out_dtype, device=x.device)
     if x.shape[0] > 0:
         _gemm_e4m3_out(x, x_scale, weight, weight_scale, out)

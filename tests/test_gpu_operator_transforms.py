@@ -149,6 +149,8 @@ def test_selective_checkpointing_runs_the_policy(ck):
     """A policy that keeps the norm's outputs finds the norm, and the gradients are those without checkpointing."""
     from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selective_checkpoint_contexts
 
+    if not ck.ops._fast():
+        pytest.skip("the Python nodes' ops write into buffers they are given, which a policy cannot keep")
     x, res, w = (randn(*s, seed=i).requires_grad_(True) for i, s in enumerate(((24, 64), (24, 64), (64,))))
     rng, asked = rng_state(), []
 
@@ -242,3 +244,35 @@ def test_one_tensor_in_two_places_under_compile(ck, name, dynamic):
             assert torch.equal(x, y)
         (got,) = torch.autograd.grad(outs, a, seeds)
         assert torch.equal(got, want)
+
+
+def off_boundary(t):
+    """The same values in memory that starts one element behind a 16-byte boundary."""
+    whole = torch.empty(t.numel() + 16, dtype=t.dtype, device=DEV)
+    view = whole[1:1 + t.numel()].view(t.shape)
+    return view.copy_(t)
+
+
+@pytest.mark.parametrize("large", [False, True])
+def test_matrices_off_a_16_byte_boundary_under_compile(ck, large):
+    """They are copied there as in an eager call, not refused."""
+    M, K, V, piece = (1500, 2048, 8195, 3000) if large else (24, 64, 72, 32)
+    g = torch.Generator().manual_seed(0)
+    x, w = (off_boundary(torch.randn(*s, generator=g).bfloat16().to(DEV)).requires_grad_(True) for s in ((M, K), (V, K)))
+    assert x.data_ptr() % 16 and w.data_ptr() % 16
+    target = torch.randint(0, V, (M,), generator=g, dtype=torch.int32).to(DEV)
+    target[::3] = -100
+
+    def f(x, w):
+        return ck.linear_cross_entropy_pieces(x, w, target, piece=piece)
+
+    want, got = f(x, w), torch.compile(f, fullgraph=True, dynamic=False)(x, w)
+    assert torch.equal(want, got)
+    for a, b in zip(torch.autograd.grad(want, (x, w)), torch.autograd.grad(got, (x, w))):
+        assert torch.equal(a, b)
+    if not large:
+        q, s = ck.quantize_e4m3(x.detach())
+        w8, ws = ck.quantize_e4m3(w.detach())
+        q, w8 = (off_boundary(t.view(torch.uint8)).view(t.dtype) for t in (q, w8))
+        with torch.no_grad():
+            assert torch.equal(ck.linear_e4m3(q, s, w8, ws), torch.compile(ck.linear_e4m3, fullgraph=True, dynamic=False)(q, s, w8, ws))
