@@ -79,6 +79,9 @@ SIGNATURES = {
     ),
     "coda_b200_dropout": (_I, [_P, _P, _L, _L, _I, _D, _P, _L, _P, _P]),
     "coda_b200_add_rmsnorm_fwd": (_I, [_P, _P, _P, _F, _D, _P, _L, _P, _P, _P, _P, _L, _L, _I, _P]),
+    "coda_b200_add_rmsnorm_low_bytes": (_L, [_L, _L]),
+    "coda_b200_add_rmsnorm_fwd_low": (_I, [_P, _P, _P, _F, _D, _P, _L, _P, _P, _P, _P, _P, _L, _L, _I, _P]),
+    "coda_b200_add_rmsnorm_bwd_low": (_I, [_P, _P, _P, _P, _P, _P, _D, _P, _L, _P, _P, _P, _P, _L, _L, _L, _I, _P]),
     "coda_b200_add_rmsnorm_bwd_scratch_bytes": (_L, [_L, _L]),
     "coda_b200_add_rmsnorm_bwd": (_I, [_P, _P, _P, _P, _P, _D, _P, _L, _P, _P, _P, _P, _L, _L, _L, _I, _P]),
     "coda_b200_rows_e4m3": (_I, [_P, _P, _P, _F, _P, _P, _P, _L, _L, _I, _P]),

@@ -128,6 +128,63 @@ __device__ __forceinline__ void store_chunk(T* p, const float* v, const Span<kSh
   }
 }
 
+// ------------------------------------------------------------------ the bits of h below its 2-byte type
+// h is stored in T, half a step off; what is summed over rows of it (the weight gradient) would carry that rounding beside its
+// own, 1.4 times the error.  So the forward also leaves four bits an element.  With v the fp32 value and hi = v rounded to T, the
+// difference of their bit patterns (sign and magnitude, so it is monotone across binades) lies within the half step kHalf; n =
+// floor((hi - v + kHalf) 15 / (2 kHalf)) is 0 .. 15, 7 where they are equal, and hi + (7 - n) kUnit gives v back to half a unit:
+// 2^-11 of its size (bf16; fp16 2^-14, for normal numbers), a fifteenth of the half step, which does not show in a sum's error
+// (16384 x 4096, against 64 bits: bf16 2.3e-3 without these bits, 1.7e-3 with them, which is the rounding of the sum).
+// n is the top nibble of a product with a power of two times 15, and is shifted from there into the chunk's word, the first element's
+// into the top.
+// The words follow the chunks, and where two rows may share a chunk its place moves on by one a row, so that no word belongs to two.
+template <typename T>
+struct Low;
+template <>
+struct Low<__nv_bfloat16> {
+  static constexpr int kHalf = 1 << 15, kUnit = 4369;
+};
+template <>
+struct Low<__half> {
+  static constexpr int kHalf = 1 << 12, kUnit = 546;
+};
+constexpr long long low_words(long long rows, long long cols) { return cols % 8 == 0 ? rows * (cols / 8) : (rows * cols + 7) / 8 + rows; }
+// the word of the chunk of `row` that begins at element e of the matrix
+template <bool kShift>
+__device__ __forceinline__ long long low_at(long long e, long long row) {
+  return (e >> 3) + (kShift ? row : 0);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t low_word(const float* v) {
+  Chunk<T> c;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c.w[j] = pack2(v[2 * j], v[2 * j + 1], T());
+  uint32_t word = 0u;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    int u = __float_as_int(chunk_get(c, j)) - __float_as_int(v[j]) + Low<T>::kHalf;
+    // below its normal numbers and above its largest fp16 is further off
+    if constexpr (std::is_same<T, __half>::value) u = min(max(u, 0), 2 * Low<T>::kHalf);
+    word = __funnelshift_l(static_cast<uint32_t>(u) * (0x78000000u / Low<T>::kHalf), word, 4);
+  }
+  return word;
+}
+// The nibbles of a word as bytes: of the odd elements and of the even ones, the last pair's first.
+struct LowBytes {
+  uint32_t odd, even;
+  __device__ __forceinline__ explicit LowBytes(uint32_t word) : odd(word & 0x0f0f0f0fu), even((word >> 4) & 0x0f0f0f0fu) {}
+  __device__ __forceinline__ int get(int j) const { return static_cast<int>(__byte_perm(j & 1 ? odd : even, 0u, 0x4440 | (3 - (j >> 1)))); }
+};
+// element j of a chunk with the bits below its type (7 kUnit = 0x7777 fits the bits that bf16 leaves empty)
+__device__ __forceinline__ float chunk_get_whole(const Chunk<__nv_bfloat16>& c, const LowBytes& low, int j) {
+  const uint32_t top = j & 1 ? (c.w[j >> 1] & 0xffff0000u) | 0x7777u : __byte_perm(c.w[j >> 1], 0x7777u, 0x1054);
+  return __int_as_float(static_cast<int>(top) - low.get(j) * Low<__nv_bfloat16>::kUnit);
+}
+__device__ __forceinline__ float chunk_get_whole(const Chunk<__half>& c, const LowBytes& low, int j) {
+  return __int_as_float(__float_as_int(chunk_get(c, j)) + (7 - low.get(j)) * Low<__half>::kUnit);
+}
+
 // max that keeps NaN
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -442,7 +499,7 @@ struct RowLoop {
 template <typename T, bool kShift, bool kDrop, int kLanes, int kChunks, bool kE4M3>
 __global__ void __maxnreg__(fwd_regs(sizeof(T), kShift, kChunks, kE4M3))
 norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T* __restrict__ weight, float eps, Dropout d,
-                long long* __restrict__ used, T* __restrict__ h, T* __restrict__ out, float* __restrict__ rstd,
+                long long* __restrict__ used, T* __restrict__ h, uint32_t* __restrict__ low, T* __restrict__ out, float* __restrict__ rstd,
                 __nv_fp8_e4m3* __restrict__ q, float* __restrict__ scale, long long rows, int cols) {
   __shared__ float red[kLanes != 0 ? 1 : 128];
   int turn = 0;
@@ -498,7 +555,12 @@ norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T
     if (at.row + at.step < rows) load(at.row + at.step);
     if (h != nullptr) {
 #pragma unroll
-      for (int k = 0; k < kChunks; ++k) store_chunk(h + base + span(k).c0, v[k], span(k));
+      for (int k = 0; k < kChunks; ++k) {
+        store_chunk(h + base + span(k).c0, v[k], span(k));
+        if constexpr (!kE4M3 && sizeof(T) == 2) {
+          if (low != nullptr && span(k).any()) low[low_at<kShift>(base + span(k).c0, at.row)] = low_word<T>(v[k]);
+        }
+      }
     }
     row_reduce<kLanes, kE4M3>(sq, top, red, turn);
     const float r = weight != nullptr ? rsqrtf(sq / static_cast<float>(cols) + eps) : 1.0f;
@@ -522,15 +584,17 @@ norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T
 
 // ------------------------------------------------------------------ its backward
 // g = dout * w, xh = h * rstd, c = mean(g * xh): dres = dh + rstd * (g - xh * c), dx = dropout(dres), dw = sum(dout * xh).
-// h is the stored one: in a 2-byte type dw and xh carry its half step.  (Forming h again from x and residual would read one
-// more tensor, ten instead of nine tensor passes a step.)
+// h is the stored one, with the bits below a 2-byte type where the forward has left them.  (Half a byte an element more each way:
+// 16384 x 4096 bf16 198 us a step without them, 210 with; 231 and 250 with dropout.  The other times of residual norms in
+// this file's comments were taken without them.  Forming h again from x and residual would read one tensor more, and the node
+// would keep one more.)
 //
 // Bound by HBM, and laid out as the forward; dw is summed in registers over a thread's rows and leaves as one partial row a
 // block, which fold_rows_kernel adds in a fixed order.
-template <typename T, bool kShift, bool kDrop, int kLanes, int kChunks>
+template <typename T, bool kShift, bool kDrop, bool kLow, int kLanes, int kChunks>
 __global__ void __maxnreg__(bwd_regs(sizeof(T), kShift, kDrop, kChunks))
-norm_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* __restrict__ h, const float* __restrict__ rstd,
-                const T* __restrict__ weight, Dropout d, T* __restrict__ dx, T* __restrict__ dres, float* __restrict__ partial,
+norm_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* __restrict__ h, const uint32_t* __restrict__ low,
+                const float* __restrict__ rstd, const T* __restrict__ weight, Dropout d, T* __restrict__ dx, T* __restrict__ dres, float* __restrict__ partial,
                 long long rows, int cols) {
   // the next row's loads need as many registers again
   constexpr bool kPrefetch = !kShift && sizeof(T) == 2;
@@ -545,6 +609,7 @@ norm_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* _
   auto span = [&](int k) { return Span<kShift>(8 * (at.tid + k * at.width) - off, cols); };
   struct Row {
     Chunk<T> o[kChunks], h[kChunks], e[kChunks];
+    uint32_t low[kLow ? kChunks : 1];
     float r;
   };
   auto load = [&](long long row, Row& in) {
@@ -555,6 +620,7 @@ norm_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* _
       const long long e = row * cols + s.c0;
       in.o[k] = load_chunk(dout + e, s, total - e);
       in.h[k] = load_chunk(h + e, s, total - e);
+      if constexpr (kLow) in.low[k] = s.any() ? low[low_at<kShift>(e, row)] : 0u;
       if (dh != nullptr) in.e[k] = load_chunk(dh + e, s, total - e);
     }
   };
@@ -576,14 +642,17 @@ norm_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* _
     }
     const long long base = at.row * cols;
     const float r = cur.r;
-    float dot = 0.f, unused = 0.f;
+    float dot = 0.f, unused = 0.f, xh[kChunks][8];
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
       mask_chunk(cur.o[k], span(k));
       mask_chunk(cur.h[k], span(k));
+      const LowBytes bits(kLow ? cur.low[k] : 0u);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float t = chunk_get(cur.o[k], j) * (chunk_get(cur.h[k], j) * r);
+        if constexpr (kLow) xh[k][j] = chunk_get_whole(cur.h[k], bits, j) * r;
+        else xh[k][j] = chunk_get(cur.h[k], j) * r;
+        const float t = chunk_get(cur.o[k], j) * xh[k][j];
         acc[k][j] += t;
         dot = fmaf(t, chunk_get(w[k], j), dot);
       }
@@ -596,7 +665,7 @@ norm_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* _
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[j] = r * (chunk_get(cur.o[k], j) * chunk_get(w[k], j) - chunk_get(cur.h[k], j) * r * m);
+        v[j] = r * (chunk_get(cur.o[k], j) * chunk_get(w[k], j) - xh[k][j] * m);
         if (dh != nullptr) v[j] += chunk_get(cur.e[k], j);
       }
       if (dres != nullptr) store_chunk(dres + base + s.c0, v, s);
@@ -643,7 +712,7 @@ constexpr int kLongThreads = 1024;
 template <typename T, bool kShift, bool kDrop, bool kE4M3>
 __global__ void __launch_bounds__(kLongThreads)
 norm_fwd_long_kernel(const T* __restrict__ x, const T* __restrict__ residual, const T* __restrict__ weight, float eps, Dropout d,
-                     long long* __restrict__ used, T* __restrict__ h, T* __restrict__ out, float* __restrict__ rstd,
+                     long long* __restrict__ used, T* __restrict__ h, uint32_t* __restrict__ low, T* __restrict__ out, float* __restrict__ rstd,
                      __nv_fp8_e4m3* __restrict__ q, float* __restrict__ scale, long long rows, int cols) {
   __shared__ float red[128];
   int turn = 0;
@@ -676,6 +745,9 @@ norm_fwd_long_kernel(const T* __restrict__ x, const T* __restrict__ residual, co
       const Span<kShift> s(c, cols);
       value(s, v);
       if (h != nullptr) store_chunk(h + base + c, v, s);
+      if constexpr (!kE4M3 && sizeof(T) == 2) {
+        if (low != nullptr && s.any()) low[low_at<kShift>(base + c, at.row)] = low_word<T>(v);
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) sq = fmaf(v[j], v[j], sq);
       if (kE4M3) {
@@ -729,10 +801,10 @@ __device__ __forceinline__ void add_sums(float* sums, const float* v, const Span
   }
 }
 
-template <typename T, bool kShift, bool kDrop>
+template <typename T, bool kShift, bool kDrop, bool kLow>
 __global__ void __launch_bounds__(kLongThreads, 2)
-norm_bwd_long_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* __restrict__ h, const float* __restrict__ rstd,
-                     const T* __restrict__ weight, Dropout d, T* __restrict__ dx, T* __restrict__ dres, float* __restrict__ partial,
+norm_bwd_long_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const T* __restrict__ h, const uint32_t* __restrict__ low,
+                     const float* __restrict__ rstd, const T* __restrict__ weight, Dropout d, T* __restrict__ dx, T* __restrict__ dres, float* __restrict__ partial,
                      long long rows, int cols) {
   __shared__ float red[128];
   int turn = 0;
@@ -746,23 +818,28 @@ norm_bwd_long_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const
     const long long base = at.row * cols;
     const int first = 8 * at.tid - (kShift ? at.offset(cols) : 0);
     const float r = rstd[at.row];
-    auto operands = [&](const Span<kShift>& s, Chunk<T>& o, Chunk<T>& hh, Chunk<T>& w) {
+    auto operands = [&](const Span<kShift>& s, Chunk<T>& o, Chunk<T>& hh, Chunk<T>& w) {  // and the bits below hh
       const long long e = base + s.c0;
       o = load_chunk(dout + e, s, total - e);
       hh = load_chunk(h + e, s, total - e);
       mask_chunk(o, s);
       mask_chunk(hh, s);
       w = kShift ? load_some(weight + s.c0, s.lo, s.hi) : load_chunk(weight + s.c0, s, 8);
+      return LowBytes(kLow && s.any() ? low[low_at<kShift>(e, at.row)] : 0u);
+    };
+    auto whole = [&](const Chunk<T>& hh, const LowBytes& bits, int j) {
+      if constexpr (kLow) return chunk_get_whole(hh, bits, j);
+      else return chunk_get(hh, j);
     };
     float dot = 0.f, unused = 0.f, v[8];
     Chunk<T> o, hh, w;
     // a column may pass from one thread to another between rows: row_reduce's synchronisation lies between the two
     for (int c = first; c < cols; c += 8 * kLongThreads) {
       const Span<kShift> s(c, cols);
-      operands(s, o, hh, w);
+      const LowBytes bits = operands(s, o, hh, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float t = chunk_get(o, j) * (chunk_get(hh, j) * r);
+        const float t = chunk_get(o, j) * (whole(hh, bits, j) * r);
         dot = fmaf(t, chunk_get(w, j), dot);
         v[j] = t;
       }
@@ -775,9 +852,9 @@ norm_bwd_long_kernel(const T* __restrict__ dout, const T* __restrict__ dh, const
     const float m = dot / static_cast<float>(cols);
     for (int c = first; c < cols; c += 8 * kLongThreads) {
       const Span<kShift> s(c, cols);
-      operands(s, o, hh, w);
+      const LowBytes bits = operands(s, o, hh, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = r * (chunk_get(o, j) * chunk_get(w, j) - chunk_get(hh, j) * r * m);
+      for (int j = 0; j < 8; ++j) v[j] = r * (chunk_get(o, j) * chunk_get(w, j) - whole(hh, bits, j) * r * m);
       if (dh != nullptr) {
         const Chunk<T> e = load_chunk(dh + base + c, s, total - base - c);
 #pragma unroll
@@ -911,8 +988,8 @@ int by_shape(const RowPlan& p, F&& f) {
 }
 
 template <bool kE4M3>
-int launch_norm_fwd(const void* x, const void* residual, const void* weight, float eps, const Dropout& d, int64_t* used, void* h, void* out,
-                    float* rstd, void* q, float* scale, int64_t rows, int64_t cols, int dtype, void* stream) {
+int launch_norm_fwd(const void* x, const void* residual, const void* weight, float eps, const Dropout& d, int64_t* used, void* h, void* low,
+                    void* out, float* rstd, void* q, float* scale, int64_t rows, int64_t cols, int dtype, void* stream) {
   const RowPlan plan = row_plan(rows, cols, dtype, false, d.rng != nullptr, kE4M3);
   return by_dtype(dtype, [&](auto t) {
     return by_flag(plan.shift, [&](auto shift) {
@@ -927,7 +1004,7 @@ int launch_norm_fwd(const void* x, const void* residual, const void* weight, flo
           }();
           kern<<<static_cast<int>(plan.grid), plan.threads, 0, static_cast<cudaStream_t>(stream)>>>(
               static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const T*>(weight), eps, d,
-              reinterpret_cast<long long*>(used), static_cast<T*>(h), static_cast<T*>(out), rstd, static_cast<__nv_fp8_e4m3*>(q), scale, rows,
+              reinterpret_cast<long long*>(used), static_cast<T*>(h), static_cast<uint32_t*>(low), static_cast<T*>(out), rstd, static_cast<__nv_fp8_e4m3*>(q), scale, rows,
               static_cast<int>(cols));
           return launch_check(kE4M3 ? "e4m3 rows launch" : "add_rmsnorm forward launch");
         });
@@ -968,6 +1045,12 @@ extern "C" int coda_b200_dropout(const void* x, void* out, int64_t rows, int64_t
 extern "C" int coda_b200_add_rmsnorm_fwd(const void* x, const void* residual, const void* weight, float eps, double p, const int64_t* rng,
                                          int64_t stream_id, int64_t* rng_used, void* h, void* out, float* rstd, int64_t rows,
                                          int64_t cols, int dtype, void* stream) {
+  return coda_b200_add_rmsnorm_fwd_low(x, residual, weight, eps, p, rng, stream_id, rng_used, h, nullptr, out, rstd, rows, cols, dtype, stream);
+}
+
+extern "C" int coda_b200_add_rmsnorm_fwd_low(const void* x, const void* residual, const void* weight, float eps, double p, const int64_t* rng,
+                                             int64_t stream_id, int64_t* rng_used, void* h, void* h_low, void* out, float* rstd,
+                                             int64_t rows, int64_t cols, int dtype, void* stream) {
   int rc = check_norm_extents(rows, cols, dtype);
   if (rc != kOk) return rc;
   Dropout d;
@@ -975,9 +1058,10 @@ extern "C" int coda_b200_add_rmsnorm_fwd(const void* x, const void* residual, co
   if (rc != kOk) return rc;
   if (rows == 0) return kOk;
   if (!x || !weight || !out || !rstd) return fail(kBadArgument, "NULL pointer");
-  rc = check_aligned({x, residual, weight, h, out});
+  if (h_low != nullptr && (h == nullptr || dtype == 2)) return fail(kBadArgument, "h_low goes with an h of a 2-byte type");
+  rc = check_aligned({x, residual, weight, h, h_low, out});
   if (rc != kOk) return rc;
-  return launch_norm_fwd<false>(x, residual, weight, eps, d, rng_used, h, out, rstd, nullptr, nullptr, rows, cols, dtype, stream);
+  return launch_norm_fwd<false>(x, residual, weight, eps, d, rng_used, h, h_low, out, rstd, nullptr, nullptr, rows, cols, dtype, stream);
 }
 
 extern "C" int coda_b200_rows_e4m3(const void* x, const void* residual, const void* weight, float eps, void* h, void* q, float* scale,
@@ -989,8 +1073,10 @@ extern "C" int coda_b200_rows_e4m3(const void* x, const void* residual, const vo
   rc = check_aligned({x, residual, weight, h, q});
   if (rc != kOk) return rc;
   const Dropout d{nullptr, 0u, 0u, 1.0f};
-  return launch_norm_fwd<true>(x, residual, weight, eps, d, nullptr, h, nullptr, nullptr, q, scale, rows, cols, dtype, stream);
+  return launch_norm_fwd<true>(x, residual, weight, eps, d, nullptr, h, nullptr, nullptr, nullptr, q, scale, rows, cols, dtype, stream);
 }
+
+extern "C" int64_t coda_b200_add_rmsnorm_low_bytes(int64_t rows, int64_t cols) { return rows <= 0 || cols <= 0 ? 0 : 4 * low_words(rows, cols); }
 
 extern "C" int64_t coda_b200_add_rmsnorm_bwd_scratch_bytes(int64_t rows, int64_t cols) {
   return rows <= 0 || cols <= 0 ? 0 : most_partial_rows(rows, cols) * cols * static_cast<int64_t>(sizeof(float));
@@ -999,6 +1085,14 @@ extern "C" int64_t coda_b200_add_rmsnorm_bwd_scratch_bytes(int64_t rows, int64_t
 extern "C" int coda_b200_add_rmsnorm_bwd(const void* dout, const void* dh, const void* h, const float* rstd, const void* weight, double p,
                                          const int64_t* rng, int64_t stream_id, void* dx, void* dres, void* dweight, void* scratch,
                                          int64_t scratch_bytes, int64_t rows, int64_t cols, int dtype, void* stream) {
+  return coda_b200_add_rmsnorm_bwd_low(dout, dh, h, nullptr, rstd, weight, p, rng, stream_id, dx, dres, dweight, scratch, scratch_bytes, rows,
+                                       cols, dtype, stream);
+}
+
+extern "C" int coda_b200_add_rmsnorm_bwd_low(const void* dout, const void* dh, const void* h, const void* h_low, const float* rstd,
+                                             const void* weight, double p, const int64_t* rng, int64_t stream_id, void* dx, void* dres,
+                                             void* dweight, void* scratch, int64_t scratch_bytes, int64_t rows, int64_t cols, int dtype,
+                                             void* stream) {
   int rc = check_norm_extents(rows, cols, dtype);
   if (rc != kOk) return rc;
   Dropout d;
@@ -1008,7 +1102,8 @@ extern "C" int coda_b200_add_rmsnorm_bwd(const void* dout, const void* dh, const
   if (!dout || !h || !rstd || !weight) return fail(kBadArgument, "NULL pointer");
   if (dweight != nullptr && (scratch == nullptr || scratch_bytes < coda_b200_add_rmsnorm_bwd_scratch_bytes(rows, cols)))
     return fail(kBadArgument, "the weight gradient needs coda_b200_add_rmsnorm_bwd_scratch_bytes of scratch");
-  rc = check_aligned({dout, dh, h, weight, dx, dres, scratch});
+  if (h_low != nullptr && dtype == 2) return fail(kBadArgument, "h_low goes with an h of a 2-byte type");
+  rc = check_aligned({dout, dh, h, h_low, weight, dx, dres, scratch});
   if (rc != kOk) return rc;
   const RowPlan plan = row_plan(rows, cols, dtype, true, d.rng != nullptr);
   const int n = static_cast<int>(cols);
@@ -1017,24 +1112,27 @@ extern "C" int coda_b200_add_rmsnorm_bwd(const void* dout, const void* dh, const
     using T = decltype(t);
     const int rc2 = by_flag(plan.shift, [&](auto shift) {
       return by_flag(d.rng != nullptr, [&](auto drop) {
-        return by_shape<true>(plan, [&](auto shape) {
-          constexpr bool kShift = decltype(shift)::value, kDrop = decltype(drop)::value;
-          constexpr int kLanes = decltype(shape)::kLanes, kChunks = decltype(shape)::kChunks;
-          auto kern = [] {
-            if constexpr (kChunks == 0) return norm_bwd_long_kernel<T, kShift, kDrop>;
-            else return norm_bwd_kernel<T, kShift, kDrop, kLanes, kChunks>;
-          }();
-          int shared = 0;
-          if (kChunks == 0 && dweight != nullptr && cols <= kSharedCols) {
-            shared = n * static_cast<int>(sizeof(float));
-            const cudaError_t e =
-                cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedCols * static_cast<int>(sizeof(float)));
-            if (e != cudaSuccess) return fail(kCudaError, std::string("cudaFuncSetAttribute(smem): ") + cudaGetErrorString(e));
-          }
-          kern<<<static_cast<int>(plan.grid), plan.threads, shared, st>>>(
-              static_cast<const T*>(dout), static_cast<const T*>(dh), static_cast<const T*>(h), rstd, static_cast<const T*>(weight), d,
-              static_cast<T*>(dx), static_cast<T*>(dres), dweight != nullptr ? static_cast<float*>(scratch) : nullptr, rows, n);
-          return launch_check("add_rmsnorm backward launch");
+        return by_flag(h_low != nullptr, [&](auto bits) {
+          return by_shape<true>(plan, [&](auto shape) {
+            constexpr bool kShift = decltype(shift)::value, kDrop = decltype(drop)::value, kLow = sizeof(T) == 2 && decltype(bits)::value;
+            constexpr int kLanes = decltype(shape)::kLanes, kChunks = decltype(shape)::kChunks;
+            auto kern = [] {
+              if constexpr (kChunks == 0) return norm_bwd_long_kernel<T, kShift, kDrop, kLow>;
+              else return norm_bwd_kernel<T, kShift, kDrop, kLow, kLanes, kChunks>;
+            }();
+            int shared = 0;
+            if (kChunks == 0 && dweight != nullptr && cols <= kSharedCols) {
+              shared = n * static_cast<int>(sizeof(float));
+              const cudaError_t e =
+                  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedCols * static_cast<int>(sizeof(float)));
+              if (e != cudaSuccess) return fail(kCudaError, std::string("cudaFuncSetAttribute(smem): ") + cudaGetErrorString(e));
+            }
+            kern<<<static_cast<int>(plan.grid), plan.threads, shared, st>>>(
+                static_cast<const T*>(dout), static_cast<const T*>(dh), static_cast<const T*>(h),
+                static_cast<const uint32_t*>(h_low), rstd, static_cast<const T*>(weight), d,
+                static_cast<T*>(dx), static_cast<T*>(dres), dweight != nullptr ? static_cast<float*>(scratch) : nullptr, rows, n);
+            return launch_check("add_rmsnorm backward launch");
+          });
         });
       });
     });

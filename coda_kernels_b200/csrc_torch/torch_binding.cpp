@@ -384,9 +384,11 @@ std::tuple<Tensor, Tensor> dropout_fwd(const Tensor& x, double p, const OptTenso
   return {out, used};
 }
 
-// (out, h or nothing without a residual, rstd, the [seed, step] used or nothing without dropout)
-std::tuple<Tensor, OptTensor, Tensor, OptTensor> norm_fwd(const Tensor& x_in, const OptTensor& residual_in, const Tensor& weight_in, double eps,
-                                                          double p, const OptTensor& rng_in, int64_t stream) {
+// (out, h or nothing without a residual, rstd, the [seed, step] used or nothing without dropout, and with keep_low the bits of h
+// below a 2-byte type)
+std::tuple<Tensor, OptTensor, Tensor, OptTensor, OptTensor> norm_fwd(const Tensor& x_in, const OptTensor& residual_in, const Tensor& weight_in,
+                                                                     double eps, double p, const OptTensor& rng_in, int64_t stream,
+                                                                     bool keep_low) {
   require_rows(x_in);
   if (residual_in.has_value()) require_like(*residual_in, x_in, "residual");
   require_weight(weight_in, x_in);
@@ -397,18 +399,20 @@ std::tuple<Tensor, OptTensor, Tensor, OptTensor> norm_fwd(const Tensor& x_in, co
   const Tensor x = aligned16(x_in), residual = dense(residual_in), weight = aligned16(weight_in), rng = dense(rng_in);
   const int64_t cols = x.size(-1), rows = x.numel() / cols;
   Tensor out = at::empty_like(x), rstd = at::empty({rows}, x.options().dtype(at::kFloat));
-  OptTensor h, used;
+  OptTensor h, used, low;
   if (residual.defined()) h = at::empty_like(x);
+  if (keep_low && h.has_value() && x.element_size() == 2) low = at::empty({coda_b200_add_rmsnorm_low_bytes(rows, cols) / 4}, x.options().dtype(at::kInt));
   if (p > 0.0) used = at::empty({2}, x.options().dtype(at::kLong));
-  check(coda_b200_add_rmsnorm_fwd(x.data_ptr(), ptr_or_null(residual), weight.data_ptr(), static_cast<float>(eps), p, rng_ptr(rng), stream,
-                                  used.has_value() ? used->data_ptr<int64_t>() : nullptr, h.has_value() ? h->data_ptr() : nullptr,
-                                  out.data_ptr(), rstd.data_ptr<float>(), rows, cols, row_dtype(x), stream_of(x)),
+  auto to = [](const OptTensor& t) { return t.has_value() ? t->data_ptr() : nullptr; };
+  check(coda_b200_add_rmsnorm_fwd_low(x.data_ptr(), ptr_or_null(residual), weight.data_ptr(), static_cast<float>(eps), p, rng_ptr(rng), stream,
+                                      static_cast<int64_t*>(to(used)), to(h), to(low), out.data_ptr(), rstd.data_ptr<float>(), rows, cols,
+                                      row_dtype(x), stream_of(x)),
         "add_rmsnorm");
-  return {out, h, rstd, used};
+  return {out, h, rstd, used, low};
 }
 // (dx, dres, dweight), nothing where not wanted; dout undefined: only h was used
-std::tuple<OptTensor, OptTensor, OptTensor> norm_bwd(const OptTensor& dout_in, const OptTensor& dh_in, const Tensor& h_in, const Tensor& rstd,
-                                                     const Tensor& weight_in, double p, const OptTensor& rng_in, int64_t stream, bool need_dx,
+std::tuple<OptTensor, OptTensor, OptTensor> norm_bwd(const OptTensor& dout_in, const OptTensor& dh_in, const Tensor& h_in,
+                                                     const OptTensor& low_in, const Tensor& rstd, const Tensor& weight_in, double p, const OptTensor& rng_in, int64_t stream, bool need_dx,
                                                      bool need_dres, bool need_dw) {
   require_rows(h_in);
   if (dout_in.has_value()) require_like(*dout_in, h_in, "dout");
@@ -417,7 +421,11 @@ std::tuple<OptTensor, OptTensor, OptTensor> norm_bwd(const OptTensor& dout_in, c
   require_dropout(h_in, p, rng_in, stream);
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::cuda::CUDAGuard guard(h_in.device());
-  const Tensor h = aligned16(h_in), weight = aligned16(weight_in), rng = dense(rng_in), dh = dense(dh_in);
+  if (low_in.has_value())
+    TORCH_CHECK_VALUE(low_in->device() == h_in.device() && low_in->scalar_type() == at::kInt &&
+                          4 * low_in->numel() == coda_b200_add_rmsnorm_low_bytes(h_in.numel() / h_in.size(-1), h_in.size(-1)),
+                      "the bits below h must be int32, as many as the forward left");
+  const Tensor h = aligned16(h_in), weight = aligned16(weight_in), rng = dense(rng_in), dh = dense(dh_in), low = dense(low_in);
   const Tensor dout = dout_in.has_value() ? aligned16(*dout_in) : at::zeros_like(h);
   const int64_t cols = h.size(-1), rows = h.numel() / cols;
   TORCH_CHECK_VALUE(rstd.device() == h.device() && rstd.scalar_type() == at::kFloat && rstd.is_contiguous() && rstd.numel() == rows,
@@ -433,18 +441,18 @@ std::tuple<OptTensor, OptTensor, OptTensor> norm_bwd(const OptTensor& dout_in, c
     scratch = at::empty({scratch_bytes / 4}, h.options().dtype(at::kFloat));
   }
   auto to = [](const OptTensor& t) { return t.has_value() ? t->data_ptr() : nullptr; };
-  check(coda_b200_add_rmsnorm_bwd(dout.data_ptr(), ptr_or_null(dh), h.data_ptr(), rstd.data_ptr<float>(), weight.data_ptr(), p, rng_ptr(rng),
-                                  stream, to(dx), to(dres), to(dw), ptr_or_null(scratch), scratch_bytes, rows, cols, row_dtype(h),
-                                  stream_of(h)),
+  check(coda_b200_add_rmsnorm_bwd_low(dout.data_ptr(), ptr_or_null(dh), h.data_ptr(), ptr_or_null(low), rstd.data_ptr<float>(),
+                                      weight.data_ptr(), p, rng_ptr(rng), stream, to(dx), to(dres), to(dw), ptr_or_null(scratch),
+                                      scratch_bytes, rows, cols, row_dtype(h), stream_of(h)),
         "add_rmsnorm backward");
   return {dx, dres, dw};
 }
 Tensor rms_norm(const Tensor& x, const Tensor& weight, double eps) {
-  return std::get<0>(norm_fwd(x, c10::nullopt, weight, eps, 0.0, c10::nullopt, 0));
+  return std::get<0>(norm_fwd(x, c10::nullopt, weight, eps, 0.0, c10::nullopt, 0, false));
 }
 std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps, double p,
                                         const OptTensor& rng, int64_t stream) {
-  auto f = norm_fwd(x, residual, weight, eps, p, rng, stream);
+  auto f = norm_fwd(x, residual, weight, eps, p, rng, stream, false);
   return {std::get<0>(f), *std::get<1>(f)};
 }
 
@@ -688,19 +696,20 @@ Tensor call_dropout(const Tensor& x, double p, const OptTensor& rng, int64_t str
   at::AutoDispatchBelowADInplaceOrView below;
   return op.call(x, p, rng, stream);
 }
-auto call_norm_fwd(const Tensor& x, const OptTensor& residual, const Tensor& weight, double eps, double p, const OptTensor& rng, int64_t stream) {
-  static const auto op = operator_named<std::tuple<Tensor, OptTensor, Tensor, OptTensor>(
-      const Tensor&, const OptTensor&, const Tensor&, double, double, const OptTensor&, int64_t)>("coda_b200n::norm_fwd");
+auto call_norm_fwd(const Tensor& x, const OptTensor& residual, const Tensor& weight, double eps, double p, const OptTensor& rng, int64_t stream,
+                   bool keep_low) {
+  static const auto op = operator_named<std::tuple<Tensor, OptTensor, Tensor, OptTensor, OptTensor>(
+      const Tensor&, const OptTensor&, const Tensor&, double, double, const OptTensor&, int64_t, bool)>("coda_b200n::norm_fwd");
   at::AutoDispatchBelowADInplaceOrView below;
-  return op.call(x, residual, weight, eps, p, rng, stream);
+  return op.call(x, residual, weight, eps, p, rng, stream, keep_low);
 }
-auto call_norm_bwd(const OptTensor& dout, const OptTensor& dh, const Tensor& h, const Tensor& rstd, const Tensor& weight, double p,
-                   const OptTensor& rng, int64_t stream, bool need_dx, bool need_dres, bool need_dw) {
-  static const auto op =
-      operator_named<std::tuple<OptTensor, OptTensor, OptTensor>(const OptTensor&, const OptTensor&, const Tensor&, const Tensor&, const Tensor&,
-                                                                 double, const OptTensor&, int64_t, bool, bool, bool)>("coda_b200n::norm_bwd");
+auto call_norm_bwd(const OptTensor& dout, const OptTensor& dh, const Tensor& h, const OptTensor& low, const Tensor& rstd, const Tensor& weight,
+                   double p, const OptTensor& rng, int64_t stream, bool need_dx, bool need_dres, bool need_dw) {
+  static const auto op = operator_named<std::tuple<OptTensor, OptTensor, OptTensor>(
+      const OptTensor&, const OptTensor&, const Tensor&, const OptTensor&, const Tensor&, const Tensor&, double, const OptTensor&, int64_t, bool,
+      bool, bool)>("coda_b200n::norm_bwd");
   at::AutoDispatchBelowADInplaceOrView below;
-  return op.call(dout, dh, h, rstd, weight, p, rng, stream, need_dx, need_dres, need_dw);
+  return op.call(dout, dh, h, low, rstd, weight, p, rng, stream, need_dx, need_dres, need_dw);
 }
 
 class DropoutNode : public torch::autograd::Function<DropoutNode> {
@@ -727,14 +736,14 @@ class RMSNormNode : public torch::autograd::Function<RMSNormNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& weight, double eps) {
     at::AutoDispatchBelowADInplaceOrView below;
     const Tensor x = x_in.contiguous();
-    auto f = call_norm_fwd(x, c10::nullopt, weight, eps, 0.0, c10::nullopt, 0);
+    auto f = call_norm_fwd(x, c10::nullopt, weight, eps, 0.0, c10::nullopt, 0, false);
     ctx->save_for_backward({x, weight, std::get<2>(f)});
     return std::get<0>(f);
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     require_first_order("rms_norm");
     const auto saved = ctx->get_saved_variables();
-    auto g = call_norm_bwd(grads[0], c10::nullopt, saved[0], saved[2], saved[1], 0.0, c10::nullopt, 0, false, ctx->needs_input_grad(0),
+    auto g = call_norm_bwd(grads[0], c10::nullopt, saved[0], c10::nullopt, saved[2], saved[1], 0.0, c10::nullopt, 0, false, ctx->needs_input_grad(0),
                            ctx->needs_input_grad(1));
     return {std::get<1>(g).value_or(Tensor()), std::get<2>(g).value_or(Tensor()), Tensor()};
   }
@@ -744,9 +753,9 @@ class AddRMSNormNode : public torch::autograd::Function<AddRMSNormNode> {
  public:
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const Tensor& weight, double eps, double p,
                                const OptTensor& rng, int64_t stream) {
-    auto f = call_norm_fwd(x, residual, weight, eps, p, rng, stream);
+    auto f = call_norm_fwd(x, residual, weight, eps, p, rng, stream, true);
     const Tensor &out = std::get<0>(f), &h = *std::get<1>(f);
-    ctx->save_for_backward({h, weight, std::get<2>(f), std::get<3>(f).value_or(Tensor())});
+    ctx->save_for_backward({h, weight, std::get<2>(f), std::get<3>(f).value_or(Tensor()), std::get<4>(f).value_or(Tensor())});
     ctx->saved_data["p"] = p;
     ctx->saved_data["stream"] = stream;
     ctx->set_materialize_grads(false);
@@ -755,7 +764,7 @@ class AddRMSNormNode : public torch::autograd::Function<AddRMSNormNode> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     require_first_order("add_rms_norm");
     const auto saved = ctx->get_saved_variables();
-    auto g = call_norm_bwd(optional(grads[0]), optional(grads[1]), saved[0], saved[2], saved[1], ctx->saved_data["p"].toDouble(),
+    auto g = call_norm_bwd(optional(grads[0]), optional(grads[1]), saved[0], optional(saved[4]), saved[2], saved[1], ctx->saved_data["p"].toDouble(),
                            optional(saved[3]), ctx->saved_data["stream"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1),
                            ctx->needs_input_grad(2));
     return {std::get<0>(g).value_or(Tensor()), std::get<1>(g).value_or(Tensor()), std::get<2>(g).value_or(Tensor()), Tensor(), Tensor(), Tensor(),
@@ -883,8 +892,9 @@ TORCH_LIBRARY(coda_b200n, m) {
 
   m.def("dropout(Tensor x, float p, Tensor? rng, int stream) -> Tensor");
   m.def("dropout_fwd(Tensor x, float p, Tensor? rng, int stream) -> (Tensor, Tensor)");
-  m.def("norm_fwd(Tensor x, Tensor? residual, Tensor weight, float eps, float p, Tensor? rng, int stream) -> (Tensor, Tensor?, Tensor, Tensor?)");
-  m.def("norm_bwd(Tensor? dout, Tensor? dh, Tensor h, Tensor rstd, Tensor weight, float p, Tensor? rng, int stream, bool need_dx, "
+  m.def("norm_fwd(Tensor x, Tensor? residual, Tensor weight, float eps, float p, Tensor? rng, int stream, bool keep_low) -> "
+        "(Tensor, Tensor?, Tensor, Tensor?, Tensor?)");
+  m.def("norm_bwd(Tensor? dout, Tensor? dh, Tensor h, Tensor? low, Tensor rstd, Tensor weight, float p, Tensor? rng, int stream, bool need_dx, "
         "bool need_dres, bool need_dw) -> (Tensor?, Tensor?, Tensor?)");
   m.def("ce_pieces_fwd(Tensor x, Tensor weight, Tensor target, int ignore_index, bool mean, bool compact, Tensor status) -> "
         "(Tensor, Tensor, Tensor, Tensor?, Tensor?, Tensor?)");

@@ -2,7 +2,8 @@
 
 Extensions with no counterpart in the reference, whose norms live inside the fused layer blocks.
 ``add_rms_norm`` ends a sublayer: ``h = residual + dropout(x)`` is the new residual stream and ``out`` its RMS norm, the
-next linear's input.  The statistic and ``out`` come from the unrounded ``h``; the backward works from the stored one
+next linear's input.  The statistic and ``out`` come from the unrounded ``h``; the backward works from the stored one, from the
+bits of ``h`` below a 2-byte type (half a byte an element, without which ``dweight`` carries the rounding of ``h`` beside its own)
 and from ``rstd``, and makes the dropout mask again.
 """
 
@@ -39,7 +40,7 @@ class RMSNorm(torch.autograd.Function):
     def forward(ctx, x: Tensor, weight: Tensor, eps: float) -> Tensor:
         _require_rows(x)
         _require_weight(weight, x)
-        out, _, rstd, _ = add_rmsnorm_forward(x, None, weight, eps, 0.0, None, 0)
+        out, _, rstd, _, _ = add_rmsnorm_forward(x, None, weight, eps, 0.0, None, 0)
         ctx.save_for_backward(x, weight, rstd)
         return out
 
@@ -50,12 +51,12 @@ class RMSNorm(torch.autograd.Function):
         _require_first_order("rms_norm")
         x, weight, rstd = ctx.saved_tensors
         need_dx, need_dw = ctx.needs_input_grad[:2]
-        _, dx, dw = add_rmsnorm_backward(dout, None, x, rstd, weight, 0.0, None, 0, False, need_dx, need_dw)
+        _, dx, dw = add_rmsnorm_backward(dout, None, x, None, rstd, weight, 0.0, None, 0, False, need_dx, need_dw)
         return dx, dw, None
 
 
 class AddRMSNorm(torch.autograd.Function):
-    """Saves ``(h, weight, rstd)`` and the 16 bytes the dropout mask was made from."""
+    """Saves ``(h, weight, rstd)``, the bits below ``h`` and the 16 bytes the dropout mask was made from."""
 
     @staticmethod
     @input_guard
@@ -65,8 +66,8 @@ class AddRMSNorm(torch.autograd.Function):
         _require_like(residual, x, "residual")
         _require_weight(weight, x)
         _require_dropout(x, p, rng, stream)
-        out, h, rstd, used = add_rmsnorm_forward(x, residual, weight, eps, p, rng, stream)
-        ctx.save_for_backward(h, weight, rstd, used)
+        out, h, rstd, used, low = add_rmsnorm_forward(x, residual, weight, eps, p, rng, stream)
+        ctx.save_for_backward(h, weight, rstd, used, low)
         ctx.p, ctx.stream = p, stream
         ctx.set_materialize_grads(False)
         return out, h
@@ -76,11 +77,11 @@ class AddRMSNorm(torch.autograd.Function):
     @autocast_custom_bwd
     def backward(ctx, dout: Optional[Tensor], dh: Optional[Tensor]):
         _require_first_order("add_rms_norm")
-        h, weight, rstd, used = ctx.saved_tensors
+        h, weight, rstd, used, low = ctx.saved_tensors
         need_dx, need_dres, need_dw = ctx.needs_input_grad[:3]
         if dout is None:  # only h was used
             dout = torch.zeros_like(h)
-        dx, dres, dw = add_rmsnorm_backward(dout, dh, h, rstd, weight, ctx.p, used, ctx.stream, need_dx, need_dres, need_dw)
+        dx, dres, dw = add_rmsnorm_backward(dout, dh, h, low, rstd, weight, ctx.p, used, ctx.stream, need_dx, need_dres, need_dw)
         return dx, dres, dw, None, None, None, None
 
 

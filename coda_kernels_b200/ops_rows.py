@@ -51,6 +51,12 @@ def _ptr(t: Optional[Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _low_like(x: Tensor) -> Tensor:
+    """Room for the bits of ``h`` below its type, four an element: ``coda_b200_add_rmsnorm_low_bytes``."""
+    cols, rows = x.shape[-1], x.shape[:-1].numel()
+    return x.new_empty(rows * cols // 8 if cols % 8 == 0 else (rows * cols + 7) // 8 + rows, dtype=torch.int32)
+
+
 def _dense16(t: Optional[Tensor]) -> Optional[Tensor]:
     """What the row kernels take: dense and 16-byte aligned (a view that starts elsewhere is copied)."""
     return None if t is None else _aligned16(t)
@@ -68,30 +74,32 @@ def _dropout_out(x: Tensor, p: float, rng: Optional[Tensor], stream_id: int, out
     )
 
 
-@torch.library.custom_op("coda_b200::add_rmsnorm_out", mutates_args=("h", "out", "rstd", "used"), device_types="cuda")
+@torch.library.custom_op("coda_b200::add_rmsnorm_out", mutates_args=("h", "low", "out", "rstd", "used"), device_types="cuda")
 def _add_rmsnorm_out(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float, p: float, rng: Optional[Tensor], stream_id: int,
-                     h: Optional[Tensor], out: Tensor, rstd: Tensor, used: Optional[Tensor]) -> None:
+                     h: Optional[Tensor], low: Optional[Tensor], out: Tensor, rstd: Tensor, used: Optional[Tensor]) -> None:
     x, residual, weight = _dense16(x), _dense16(residual), _dense16(weight)
     cols = x.shape[-1]
     check(
-        lib.coda_b200_add_rmsnorm_fwd(x.data_ptr(), _ptr(residual), weight.data_ptr(), float(eps), float(p), _ptr(rng), stream_id, _ptr(used),
-                                      _ptr(h), out.data_ptr(), rstd.data_ptr(), x.numel() // cols, cols, _DTYPE_CODES[x.dtype], _stream(x)),
+        lib.coda_b200_add_rmsnorm_fwd_low(x.data_ptr(), _ptr(residual), weight.data_ptr(), float(eps), float(p), _ptr(rng), stream_id,
+                                          _ptr(used), _ptr(h), _ptr(low), out.data_ptr(), rstd.data_ptr(), x.numel() // cols, cols,
+                                          _DTYPE_CODES[x.dtype], _stream(x)),
         "add_rmsnorm",
     )
 
 
 @torch.library.custom_op("coda_b200::add_rmsnorm_bwd_out", mutates_args=("dx", "dres", "dweight"), device_types="cuda")
-def _add_rmsnorm_bwd_out(dout: Tensor, dh: Optional[Tensor], h: Tensor, rstd: Tensor, weight: Tensor, p: float, rng: Optional[Tensor],
-                         stream_id: int, dx: Optional[Tensor], dres: Optional[Tensor], dweight: Optional[Tensor]) -> None:
-    dout, dh, h, weight = _dense16(dout), _dense16(dh), _dense16(h), _dense16(weight)
+def _add_rmsnorm_bwd_out(dout: Tensor, dh: Optional[Tensor], h: Tensor, low: Optional[Tensor], rstd: Tensor, weight: Tensor, p: float,
+                         rng: Optional[Tensor], stream_id: int, dx: Optional[Tensor], dres: Optional[Tensor],
+                         dweight: Optional[Tensor]) -> None:
+    dout, dh, h, low, weight = _dense16(dout), _dense16(dh), _dense16(h), _dense16(low), _dense16(weight)
     cols = h.shape[-1]
     rows = h.numel() // cols
     scratch_bytes = int(lib.coda_b200_add_rmsnorm_bwd_scratch_bytes(rows, cols)) if dweight is not None else 0
     scratch = torch.empty(scratch_bytes // 4, dtype=torch.float32, device=h.device) if dweight is not None else None
     check(
-        lib.coda_b200_add_rmsnorm_bwd(dout.data_ptr(), _ptr(dh), h.data_ptr(), rstd.data_ptr(), weight.data_ptr(), float(p), _ptr(rng),
-                                      stream_id, _ptr(dx), _ptr(dres), _ptr(dweight), _ptr(scratch), scratch_bytes, rows, cols,
-                                      _DTYPE_CODES[h.dtype], _stream(h)),
+        lib.coda_b200_add_rmsnorm_bwd_low(dout.data_ptr(), _ptr(dh), h.data_ptr(), _ptr(low), rstd.data_ptr(), weight.data_ptr(), float(p),
+                                          _ptr(rng), stream_id, _ptr(dx), _ptr(dres), _ptr(dweight), _ptr(scratch), scratch_bytes, rows,
+                                          cols, _DTYPE_CODES[h.dtype], _stream(h)),
         "add_rmsnorm backward",
     )
 
@@ -146,12 +154,13 @@ if _native is not None:
         return _like(x), x.new_empty(2, dtype=torch.int64)
 
     @torch.library.register_fake("coda_b200n::norm_fwd")
-    def _(x, residual, weight, eps, p, rng, stream):
+    def _(x, residual, weight, eps, p, rng, stream, keep_low):
         h = None if residual is None else _like(x)
-        return _like(x), h, _rows_like(x), x.new_empty(2, dtype=torch.int64) if p > 0.0 else None
+        low = _low_like(x) if keep_low and h is not None and x.dtype.itemsize == 2 else None
+        return _like(x), h, _rows_like(x), x.new_empty(2, dtype=torch.int64) if p > 0.0 else None, low
 
     @torch.library.register_fake("coda_b200n::norm_bwd")
-    def _(dout, dh, h, rstd, weight, p, rng, stream, need_dx, need_dres, need_dw):
+    def _(dout, dh, h, low, rstd, weight, p, rng, stream, need_dx, need_dres, need_dw):
         return _like(h) if need_dx else None, _like(h) if need_dres else None, _like(weight) if need_dw else None
 
     @torch.library.register_fake("coda_b200n::rms_norm")
@@ -222,24 +231,26 @@ def dropout_rows(x: Tensor, p: float, rng: Optional[Tensor], stream: int) -> tup
 
 
 def add_rmsnorm_forward(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float, p: float, rng: Optional[Tensor], stream: int):
-    """``(out, h or None, rstd, used or None)``; ``h`` is ``None`` when it would be ``x`` itself."""
+    """``(out, h or None, rstd, used or None, low or None)``; ``h`` is ``None`` when it would be ``x`` itself, ``low`` holds the bits
+    of ``h`` below a 2-byte type."""
     out = torch.empty_like(x)
     h = torch.empty_like(x) if residual is not None or p > 0.0 else None
     rstd = torch.empty(x.numel() // x.shape[-1], dtype=torch.float32, device=x.device)
     used = torch.empty(2, dtype=torch.int64, device=x.device) if p > 0.0 else None
-    _add_rmsnorm_out(x, residual, weight, eps, p, rng, stream, h, out, rstd, used)
-    return out, h, rstd, used
+    low = _low_like(x) if h is not None and x.dtype.itemsize == 2 else None
+    _add_rmsnorm_out(x, residual, weight, eps, p, rng, stream, h, low, out, rstd, used)
+    return out, h, rstd, used, low
 
 
-def add_rmsnorm_backward(dout: Tensor, dh: Optional[Tensor], h: Tensor, rstd: Tensor, weight: Tensor, p: float, rng: Optional[Tensor],
-                         stream: int, need_dx: bool, need_dres: bool, need_dw: bool):
+def add_rmsnorm_backward(dout: Tensor, dh: Optional[Tensor], h: Tensor, low: Optional[Tensor], rstd: Tensor, weight: Tensor, p: float,
+                         rng: Optional[Tensor], stream: int, need_dx: bool, need_dres: bool, need_dw: bool):
     """``(dx, dresidual, dweight)``, ``None`` where not wanted."""
     dx = torch.empty_like(h) if need_dx else None
     dres = torch.empty_like(h) if need_dres else None
     dw = None
     if need_dw:
         dw = torch.empty_like(weight) if h.numel() > 0 else torch.zeros_like(weight)
-    _add_rmsnorm_bwd_out(dout, dh, h, rstd, weight, p, rng, stream, dx, dres, dw)
+    _add_rmsnorm_bwd_out(dout, dh, h, low, rstd, weight, p, rng, stream, dx, dres, dw)
     return dx, dres, dw
 
 

@@ -374,6 +374,12 @@ int coda_b200_add_rmsnorm_fwd(const void* x, const void* residual, const void* w
                               int64_t stream_id, int64_t* rng_used, void* h, void* out, float* rstd, int64_t rows,
                               int64_t cols, int dtype, void* stream);
 
+/* The same, leaving in h_low (coda_b200_add_rmsnorm_low_bytes, 16-byte aligned, or NULL; dtype bf16 or fp16 with an h) the bits of h below its type, four an element, for the backward alone to read. */
+int64_t coda_b200_add_rmsnorm_low_bytes(int64_t rows, int64_t cols);
+int coda_b200_add_rmsnorm_fwd_low(const void* x, const void* residual, const void* weight, float eps, double p, const int64_t* rng,
+                                  int64_t stream_id, int64_t* rng_used, void* h, void* h_low, void* out, float* rstd, int64_t rows,
+                                  int64_t cols, int dtype, void* stream);
+
 /* Backward of the above from dout and dh (NULL: zero): with g = dout * weight and xh = h * rstd,
  * dres = dh + rstd * (g - xh * mean(g * xh)), dx = dropout(dres), dweight = sum over rows of dout * xh (in `dtype`,
  * summed in fp32 in a fixed order).  dx, dres and dweight may each be NULL; dweight needs
@@ -382,6 +388,13 @@ int64_t coda_b200_add_rmsnorm_bwd_scratch_bytes(int64_t rows, int64_t cols);
 int coda_b200_add_rmsnorm_bwd(const void* dout, const void* dh, const void* h, const float* rstd, const void* weight, double p,
                               const int64_t* rng, int64_t stream_id, void* dx, void* dres, void* dweight, void* scratch,
                               int64_t scratch_bytes, int64_t rows, int64_t cols, int dtype, void* stream);
+
+/* The same with the forward's h_low (or NULL), from h to 2^-11 (bf16) or 2^-14 (fp16) of its size instead of the stored one, half a
+ * step of its type off, which shows in dweight. */
+int coda_b200_add_rmsnorm_bwd_low(const void* dout, const void* dh, const void* h, const void* h_low, const float* rstd,
+                                  const void* weight, double p, const int64_t* rng, int64_t stream_id, void* dx, void* dres,
+                                  void* dweight, void* scratch, int64_t scratch_bytes, int64_t rows, int64_t cols, int dtype,
+                                  void* stream);
 
 /* Rows as e4m3 values with one fp32 scale each: y = residual + x, normalised and weighted as above when weight != NULL
  * (residual and h may be NULL; h receives residual + x); scale = max(max|y| / 448, 2^-126) and q = y / scale, both
