@@ -421,8 +421,8 @@ struct EpiLse {
 // ------------------------------------------------------------------ softmax gradient of one vocabulary piece
 // G[r, j] = exp(z_rj - lse_r) - (j + col0 == target_r) in bf16, zero in rows whose target is ignored: the gradient of the
 // summed row losses w.r.t. the logits of columns col0 .. col0 + N - 1, given the log-sum-exp over ALL columns.  The logits
-// exist only as this tile's accumulator.  bf16 holds a probability to half a step (2^-9 relative), which is also what
-// the two GEMMs behind it take; the subtraction is done before that rounding.
+// exist only as this tile's accumulator.  bf16 holds a gradient to half a step (2^-8 relative), which is what the two GEMMs
+// behind it take; the subtraction is done before that rounding.
 struct EpiSoftmaxGrad {
   static constexpr uint32_t kLoadRingBytes = 0;
   struct Params {

@@ -149,10 +149,11 @@ inline int launch_check(const char* what) {
 
 }  // namespace
 
-// A whole step, all rows against the rows that count, none / 30 % / 70 % of the rows ignored, in ms: 8192 x 4096 x 128256 26.3
-// and 25.5 / 25.1 and 17.8 / 24.5 and 8.8; 2048 x 2048 x 50257 1.30 and 1.33 / 1.27 and 1.05 / 1.22 and 0.70; 1003 x 1032 x
-// 32003 0.32 and 0.34 / 0.31 and 0.28 / 0.30 and 0.23.  Smaller products do not repay three more launches, and with a small vocabulary the two copies of
-// the rows weigh too much beside them.
+// A whole step, all rows against the rows that count, none / 30 % / 70 % of the rows ignored, in ms: 8192 x 4096 x 128256 26.4
+// and 26.9 / 26.3 and 19.2 / 24.8 and 8.6; 2048 x 2048 x 50257 1.40 and 1.39 / 1.34 and 1.11 / 1.29 and 0.76; 1003 x 1032 x
+// 32003 0.38 and 0.39 / 0.34 and 0.31 / 0.33 and 0.26.  Smaller products do not repay three more launches (they take one, the
+// masked copy of the rows: 512 x 1024 x 32000 0.172 ms, 0.168 without), and with a small vocabulary the copies of the rows weigh too
+// much beside them.
 extern "C" int coda_b200_ce_compacts(int M, int N, int K) {
   return options().ce_compact.load() != 0 && options().cta_group.load() == 2 && N >= 8192 && 2.0 * M * N * K >= 5e10 ? 1 : 0;
 }
