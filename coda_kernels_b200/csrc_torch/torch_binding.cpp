@@ -401,7 +401,8 @@ std::tuple<Tensor, OptTensor, Tensor, OptTensor, OptTensor> norm_fwd(const Tenso
   Tensor out = at::empty_like(x), rstd = at::empty({rows}, x.options().dtype(at::kFloat));
   OptTensor h, used, low;
   if (residual.defined()) h = at::empty_like(x);
-  if (keep_low && h.has_value() && x.element_size() == 2) low = at::empty({coda_b200_add_rmsnorm_low_bytes(rows, cols) / 4}, x.options().dtype(at::kInt));
+  if (keep_low && h.has_value() && x.element_size() == 2)
+    low = at::empty({coda_b200_add_rmsnorm_low_bytes(rows, cols) / 4}, x.options().dtype(at::kInt));
   if (p > 0.0) used = at::empty({2}, x.options().dtype(at::kLong));
   auto to = [](const OptTensor& t) { return t.has_value() ? t->data_ptr() : nullptr; };
   check(coda_b200_add_rmsnorm_fwd_low(x.data_ptr(), ptr_or_null(residual), weight.data_ptr(), static_cast<float>(eps), p, rng_ptr(rng), stream,
@@ -412,8 +413,8 @@ std::tuple<Tensor, OptTensor, Tensor, OptTensor, OptTensor> norm_fwd(const Tenso
 }
 // (dx, dres, dweight), nothing where not wanted; dout undefined: only h was used
 std::tuple<OptTensor, OptTensor, OptTensor> norm_bwd(const OptTensor& dout_in, const OptTensor& dh_in, const Tensor& h_in,
-                                                     const OptTensor& low_in, const Tensor& rstd, const Tensor& weight_in, double p, const OptTensor& rng_in, int64_t stream, bool need_dx,
-                                                     bool need_dres, bool need_dw) {
+                                                     const OptTensor& low_in, const Tensor& rstd, const Tensor& weight_in, double p,
+                                                     const OptTensor& rng_in, int64_t stream, bool need_dx, bool need_dres, bool need_dw) {
   require_rows(h_in);
   if (dout_in.has_value()) require_like(*dout_in, h_in, "dout");
   if (dh_in.has_value()) require_like(*dh_in, h_in, "dh");
@@ -513,6 +514,7 @@ struct CeRows {
   Tensor x, target, position, live;
 };
 inline bool ce_compacts(const Tensor& x, const Tensor& weight) {
+  if (x.dim() != 2 || weight.dim() != 2) return false;  // (refused where the arguments are checked)
   for (const int64_t n : {x.size(0), weight.size(0), x.size(-1)})
     if (n < 1 || n > INT_MAX) return false;
   return coda_b200_ce_compacts(static_cast<int>(x.size(0)), static_cast<int>(weight.size(0)), static_cast<int>(x.size(-1))) != 0;
@@ -743,8 +745,8 @@ class RMSNormNode : public torch::autograd::Function<RMSNormNode> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     require_first_order("rms_norm");
     const auto saved = ctx->get_saved_variables();
-    auto g = call_norm_bwd(grads[0], c10::nullopt, saved[0], c10::nullopt, saved[2], saved[1], 0.0, c10::nullopt, 0, false, ctx->needs_input_grad(0),
-                           ctx->needs_input_grad(1));
+    auto g = call_norm_bwd(grads[0], c10::nullopt, saved[0], c10::nullopt, saved[2], saved[1], 0.0, c10::nullopt, 0, false,
+                           ctx->needs_input_grad(0), ctx->needs_input_grad(1));
     return {std::get<1>(g).value_or(Tensor()), std::get<2>(g).value_or(Tensor()), Tensor()};
   }
 };
@@ -764,9 +766,9 @@ class AddRMSNormNode : public torch::autograd::Function<AddRMSNormNode> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     require_first_order("add_rms_norm");
     const auto saved = ctx->get_saved_variables();
-    auto g = call_norm_bwd(optional(grads[0]), optional(grads[1]), saved[0], optional(saved[4]), saved[2], saved[1], ctx->saved_data["p"].toDouble(),
-                           optional(saved[3]), ctx->saved_data["stream"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1),
-                           ctx->needs_input_grad(2));
+    auto g = call_norm_bwd(optional(grads[0]), optional(grads[1]), saved[0], optional(saved[4]), saved[2], saved[1],
+                           ctx->saved_data["p"].toDouble(), optional(saved[3]), ctx->saved_data["stream"].toInt(), ctx->needs_input_grad(0),
+                           ctx->needs_input_grad(1), ctx->needs_input_grad(2));
     return {std::get<0>(g).value_or(Tensor()), std::get<1>(g).value_or(Tensor()), std::get<2>(g).value_or(Tensor()), Tensor(), Tensor(), Tensor(),
             Tensor()};
   }

@@ -61,6 +61,7 @@ def linear_cross_entropy_pieces(
     ``dx`` and ``dweight`` NaN; ``"mean"`` over no label at all is NaN, with gradients of zero."""
     assert reduction in ("mean", "sum")
     assert target.dtype == torch.int32
+    _require(x.dim() == 2 and weight.dim() == 2, "x [M, K] and weight [V, K] expected")
     if piece is None:
         piece = default_piece(x.shape[0], weight.shape[0])
     _require(piece >= 1, "piece must be at least 1")

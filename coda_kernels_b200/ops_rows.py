@@ -53,7 +53,8 @@ def _ptr(t: Optional[Tensor]):
 
 def _low_like(x: Tensor) -> Tensor:
     """Room for the bits of ``h`` below its type, four an element: ``coda_b200_add_rmsnorm_low_bytes``."""
-    cols, rows = x.shape[-1], x.shape[:-1].numel()
+    cols = x.shape[-1]
+    rows = x.numel() // cols
     return x.new_empty(rows * cols // 8 if cols % 8 == 0 else (rows * cols + 7) // 8 + rows, dtype=torch.int32)
 
 
@@ -140,7 +141,7 @@ def _like(x: Tensor) -> Tensor:
 
 
 def _rows_like(x: Tensor) -> Tensor:
-    return x.new_empty(x.shape[:-1].numel(), dtype=torch.float32)
+    return x.new_empty(x.numel() // x.shape[-1], dtype=torch.float32)
 
 
 if _native is not None:

@@ -276,3 +276,29 @@ def test_matrices_off_a_16_byte_boundary_under_compile(ck, large):
         q, w8 = (off_boundary(t.view(torch.uint8)).view(t.dtype) for t in (q, w8))
         with torch.no_grad():
             assert torch.equal(ck.linear_e4m3(q, s, w8, ws), torch.compile(ck.linear_e4m3, fullgraph=True, dynamic=False)(q, s, w8, ws))
+
+
+def test_symbolic_trace_of_a_norm_step_runs_on_other_extents(ck):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    rng = rng_state()
+
+    def step(x, r, w):
+        leaves = [t.detach().requires_grad_(True) for t in (x, r, w)]
+        out, h = ck.add_rms_norm(*leaves, EPS, p=0.2, rng=rng)
+        return [out.detach(), h.detach(), *torch.autograd.grad((out, h), leaves, (torch.ones_like(out), torch.ones_like(h)))]
+
+    graph = make_fx(step, tracing_mode="symbolic", _allow_non_fake_inputs=True)(randn(24, 64), randn(24, 64, seed=1), randn(64, seed=2))
+    for rows in (24, 7, 300):
+        args = randn(rows, 64, seed=3), randn(rows, 64, seed=4), randn(64, seed=5)
+        for a, b in zip(step(*args), graph(*args)):
+            assert torch.equal(a, b)
+
+
+def test_shapes_of_the_loss_are_refused_as_arguments(ck):
+    """Whatever the number of dimensions, with a piece given."""
+    x, v, t = randn(24, 64), randn(72, 64, seed=1), torch.zeros(24, dtype=torch.int32, device=DEV)
+    for bad in ((x[0], v, t), (x, v[0], t), (x[None], v, t), (x, v[0, 0], t), (x[0, 0], v, t), (x, v, t[None])):
+        for grad in (False, True):
+            with pytest.raises(ValueError):
+                ck.linear_cross_entropy_pieces(*(a.clone().requires_grad_(grad) for a in bad[:2]), bad[2], piece=32)
